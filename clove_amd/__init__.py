@@ -32,7 +32,7 @@ LIB_PATH = os.path.join(_HERE, "libclove_hip.so")
 # Status codes (clove_hip.h)
 OK = 0
 ERR_INVALID, ERR_SHAPE, ERR_HIP, ERR_JIT, ERR_OOM, ERR_NOT_INIT, ERR_RANGE = 1, 2, 3, 4, 5, 6, 7
-F32, I32 = 0, 1
+F32, I32, E4M3 = 0, 1, 2  # numpy has no e4m3: its codes are uint8 arrays
 
 # Opcodes (clove_hip.h, the hot-path subset of backend.rs:85-127)
 OP = dict(
@@ -114,6 +114,11 @@ def _declare(lib: C.CDLL) -> None:
                                                         C.c_int, C.c_int, vp, C.c_int, vp,
                                                         C.c_int, f, vp]),
         "clove_hip_paged_kv_append": (C.c_int, [vp, vp, vp, vp, vp]),
+        "clove_hip_paged_kv8_append": (C.c_int, [vp] * 7),
+        "clove_hip_paged_kv8_read": (C.c_int, [vp, vp, vp, vp, vp, sz, C.POINTER(vp),
+                                               C.POINTER(vp)]),
+        "clove_hip_paged_kv8_attention": (vp, [vp, vp, vp, vp, vp, vp, f, vp, C.POINTER(vp)]),
+        "clove_hip_paged_evict": (C.c_int, [vp, vp, vp] + [C.c_int] * 4 + [C.POINTER(vp)] * 4),
         "clove_hip_relu_backward": (vp, [vp, vp]),
         "clove_hip_gelu_backward": (vp, [vp, vp]),
         "clove_hip_softmax_backward": (vp, [vp, vp]),
@@ -217,6 +222,10 @@ def memory_reserved() -> int:
 # tensors
 # ---------------------------------------------------------------------------
 
+def _dtype_code(dtype) -> int:
+    return {np.dtype(np.int32): I32, np.dtype(np.uint8): E4M3}.get(np.dtype(dtype), F32)
+
+
 def _shape_arr(shape: Sequence[int]):
     return (C.c_size_t * max(1, len(shape)))(*[int(s) for s in shape])
 
@@ -257,7 +266,8 @@ class Tensor:
 
     @property
     def dtype(self):
-        return np.float32 if lib().clove_hip_tensor_dtype(self._h) == F32 else np.int32
+        return {F32: np.float32, E4M3: np.uint8}.get(lib().clove_hip_tensor_dtype(self._h),
+                                                     np.int32)
 
     @property
     def device_ptr(self) -> int:
@@ -291,7 +301,8 @@ class Tensor:
 
 
 def tensor(data, dtype=None) -> Tensor:
-    """Uploads a numpy array (f32, or int32 for block tables / lengths)."""
+    """Uploads a numpy array (f32, int32 for block tables / lengths, or with
+    dtype=np.uint8 the e4m3 codes of an 8-bit cache)."""
     a = np.asarray(data)
     if dtype is None:
         dtype = np.int32 if a.dtype.kind in "iu" else np.float32
@@ -300,6 +311,10 @@ def tensor(data, dtype=None) -> Tensor:
     if dtype == np.int32:
         p = lib().clove_hip_tensor_create_i32(a.ctypes.data_as(C.POINTER(C.c_int32)),
                                               _shape_arr(shape), len(shape))
+    elif dtype == np.uint8:
+        t = empty(shape, np.uint8)
+        t.write(0, a)
+        return t
     else:
         p = lib().clove_hip_tensor_create_nd(a.ctypes.data_as(C.POINTER(C.c_float)),
                                              _shape_arr(shape), len(shape))
@@ -309,9 +324,8 @@ def tensor(data, dtype=None) -> Tensor:
 def wrap(device_ptr: int, shape, dtype=np.float32) -> Tensor:
     """Borrows device memory the caller owns (clove_hip_tensor_wrap); the
     memory must outlive the handle, and freeing the handle leaves it alone."""
-    code = 1 if dtype == np.int32 else 0
     return _handle(lib().clove_hip_tensor_wrap(C.c_void_p(device_ptr), _shape_arr(shape),
-                                               len(shape), code))
+                                               len(shape), _dtype_code(dtype)))
 
 
 def tensor2d(data) -> Tensor:
@@ -324,7 +338,7 @@ def tensor2d(data) -> Tensor:
 
 def empty(shape: Sequence[int], dtype=np.float32) -> Tensor:
     return _handle(lib().clove_hip_tensor_empty(_shape_arr(shape), len(shape),
-                                                I32 if dtype == np.int32 else F32))
+                                                _dtype_code(dtype)))
 
 
 # ---------------------------------------------------------------------------
@@ -496,6 +510,70 @@ def paged_gather_indices(block_tables: Tensor, context_lens: Tensor, block_size:
                          max_ctx: int) -> Tensor:
     return _handle(lib().clove_hip_paged_gather_indices(block_tables.handle, context_lens.handle,
                                                         block_size, max_ctx))
+
+
+# ---- the paged KV cache in 8 bits ------------------------------------------
+
+def paged_kv8_cache(num_blocks: int, heads: int, block_size: int, head_dim: int):
+    """An empty cache: (codes, exps) as the paged_kv8 functions take them."""
+    return (empty((2, num_blocks, heads, block_size, head_dim), np.uint8),
+            empty((2, num_blocks, heads), np.int32))
+
+
+def _opt(t: Optional[Tensor]):
+    return t.handle if t is not None else None
+
+
+def paged_kv8_append(codes: Tensor, exps: Tensor, k: Tensor, v: Tensor, block_tables: Tensor,
+                     context_lens: Tensor, row_starts: Optional[Tensor] = None) -> None:
+    """Stores the rows' keys and values (f32 [rows, H*D]) at the last positions
+    of their contexts, in 8 bits with one power-of-two scale per block and
+    head.  row_starts (int32 [B + 1]): sequence b's rows; None: one each."""
+    _check(lib().clove_hip_paged_kv8_append(codes.handle, exps.handle, k.handle, v.handle,
+                                            block_tables.handle, context_lens.handle,
+                                            _opt(row_starts)))
+
+
+def paged_kv8_read(codes: Tensor, exps: Tensor, block_tables: Tensor, context_lens: Tensor,
+                   row_starts: Optional[Tensor] = None, rows: Optional[int] = None):
+    """(k, v), f32 [rows, H*D]: what the cache holds for the rows."""
+    if rows is None:
+        if row_starts is not None:
+            raise ValueError("paged_kv8_read: row_starts needs rows, how many there are")
+        rows = context_lens.numel
+    k, v = C.c_void_p(), C.c_void_p()
+    _check(lib().clove_hip_paged_kv8_read(codes.handle, exps.handle, block_tables.handle,
+                                          context_lens.handle, _opt(row_starts), rows,
+                                          C.byref(k), C.byref(v)))
+    return Tensor(k.value), Tensor(v.value)
+
+
+def paged_kv8_attention(q: Tensor, codes: Tensor, exps: Tensor, block_tables: Tensor,
+                        context_lens: Tensor, row_starts: Optional[Tensor] = None,
+                        scale: float = 0.0, weights: Optional[Tensor] = None):
+    """Causal attention of the rows over the cache (scale 0 = 1/sqrt(D)).  With
+    weights (f32 [B, max_blocks]) the result is (out, new weights): each
+    block's attention weight of this call added to it."""
+    if weights is None:
+        return _handle(lib().clove_hip_paged_kv8_attention(
+            q.handle, codes.handle, exps.handle, block_tables.handle, context_lens.handle,
+            _opt(row_starts), scale, None, None))
+    w = C.c_void_p()
+    out = _handle(lib().clove_hip_paged_kv8_attention(
+        q.handle, codes.handle, exps.handle, block_tables.handle, context_lens.handle,
+        _opt(row_starts), scale, weights.handle, C.byref(w)))
+    return out, Tensor(w.value)
+
+
+def paged_evict(block_tables: Tensor, context_lens: Tensor, weights: Tensor, block_size: int,
+                budget: int, first: int = 1, last: int = 1):
+    """(tables, lens, weights, evicted ids) after each sequence of more than
+    `budget` blocks keeps its first and last ones and the heaviest between."""
+    outs = [C.c_void_p() for _ in range(4)]
+    _check(lib().clove_hip_paged_evict(block_tables.handle, context_lens.handle, weights.handle,
+                                       block_size, budget, first, last,
+                                       *[C.byref(o) for o in outs]))
+    return tuple(Tensor(o.value) for o in outs)
 
 
 class FusedChain:

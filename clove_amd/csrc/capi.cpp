@@ -76,6 +76,21 @@ CTensor guarded_tensor(F &&f) {
     return out;
 }
 
+// Hands n result tensors out, or none when the call failed.
+template <class F>
+int guarded_outputs(CTensor *const *outs, TensorNode *made, int n, F &&f) {
+    for (int i = 0; i < n; ++i)
+        if (outs[i]) *outs[i] = nullptr;
+    return guarded([&] {
+        f();
+        std::vector<std::unique_ptr<TensorNode>> cells(n);
+        for (int i = 0; i < n; ++i)
+            if (outs[i] && made[i]) cells[i] = std::make_unique<TensorNode>(std::move(made[i]));
+        for (int i = 0; i < n; ++i)
+            if (outs[i]) *outs[i] = cells[i].release();
+    });
+}
+
 }  // namespace
 
 extern "C" {
@@ -141,14 +156,14 @@ CTensor clove_hip_tensor_wrap(void *device_ptr, const size_t *shape, size_t ndim
     return guarded_tensor([&] {
         clove::ctx();
         if (!device_ptr) clove::fail(CLOVE_HIP_ERR_INVALID, "device_ptr is NULL");
-        if (dtype != CLOVE_HIP_F32 && dtype != CLOVE_HIP_I32)
+        if (!clove::known_dtype(dtype))
             clove::fail(CLOVE_HIP_ERR_INVALID, "unknown dtype");
         auto t = std::make_shared<Tensor>();
         t->data = device_ptr;
         t->shape = shape_of(shape, ndim);
         t->dtype = dtype;
         t->numel = clove::numel_of(t->shape);
-        t->bytes = t->numel * 4;
+        t->bytes = t->numel * clove::elem_size(dtype);
         t->owned = false;
         return t;
     });
@@ -164,6 +179,8 @@ int clove_hip_tensor_data(CTensor t, float *out) {
     return guarded([&] {
         const Tensor &x = deref(t, "tensor");
         if (!out) clove::fail(CLOVE_HIP_ERR_INVALID, "out is NULL");
+        if (x.dtype == CLOVE_HIP_E4M3)
+            clove::fail(CLOVE_HIP_ERR_INVALID, "tensor_data: e4m3 codes are read with tensor_read");
         clove::download(x, out, 0, x.numel);
     });
 }
@@ -343,6 +360,66 @@ int clove_hip_paged_kv_append(CTensor kv_cache, CTensor k, CTensor v, CTensor bl
         HipBackend::paged_kv_append(deref(kv_cache, "kv_cache"), deref(k, "k"), deref(v, "v"),
                                     deref(block_tables, "block_tables"),
                                     deref(context_lens, "context_lens"));
+    });
+}
+
+// ---- the 8-bit paged cache and eviction ------------------------------------
+
+int clove_hip_paged_kv8_append(CTensor codes, CTensor exps, CTensor k, CTensor v,
+                               CTensor block_tables, CTensor context_lens, CTensor row_starts) {
+    return guarded([&] {
+        HipBackend::paged_kv8_append(deref(codes, "codes"), deref(exps, "exps"), deref(k, "k"),
+                                     deref(v, "v"), deref(block_tables, "block_tables"),
+                                     deref(context_lens, "context_lens"),
+                                     row_starts ? &deref(row_starts, "row_starts") : nullptr);
+    });
+}
+
+int clove_hip_paged_kv8_read(CTensor codes, CTensor exps, CTensor block_tables,
+                             CTensor context_lens, CTensor row_starts, size_t rows, CTensor *k,
+                             CTensor *v) {
+    CTensor *const outs[2] = {k, v};
+    TensorNode made[2];
+    return guarded_outputs(outs, made, 2, [&] {
+        if (!k || !v) clove::fail(CLOVE_HIP_ERR_INVALID, "k or v is NULL");
+        HipBackend::paged_kv8_read(deref(codes, "codes"), deref(exps, "exps"),
+                                   deref(block_tables, "block_tables"),
+                                   deref(context_lens, "context_lens"),
+                                   row_starts ? &deref(row_starts, "row_starts") : nullptr, rows,
+                                   &made[0], &made[1]);
+    });
+}
+
+CTensor clove_hip_paged_kv8_attention(CTensor q, CTensor codes, CTensor exps,
+                                      CTensor block_tables, CTensor context_lens,
+                                      CTensor row_starts, float scale, CTensor weights,
+                                      CTensor *weights_out) {
+    CTensor out = nullptr;
+    CTensor *const outs[2] = {&out, weights_out};
+    TensorNode made[2];
+    guarded_outputs(outs, made, 2, [&] {
+        if ((weights == nullptr) != (weights_out == nullptr))
+            clove::fail(CLOVE_HIP_ERR_INVALID, "pass both weights and weights_out, or neither");
+        made[0] = HipBackend::paged_kv8_attention(
+            deref(q, "q"), deref(codes, "codes"), deref(exps, "exps"),
+            deref(block_tables, "block_tables"), deref(context_lens, "context_lens"),
+            row_starts ? &deref(row_starts, "row_starts") : nullptr, scale,
+            weights ? &deref(weights, "weights") : nullptr, &made[1]);
+    });
+    return out;
+}
+
+int clove_hip_paged_evict(CTensor block_tables, CTensor context_lens, CTensor weights,
+                          int block_size, int budget, int first, int last, CTensor *tables_out,
+                          CTensor *lens_out, CTensor *weights_out, CTensor *evicted) {
+    CTensor *const outs[4] = {tables_out, lens_out, weights_out, evicted};
+    TensorNode made[4];
+    return guarded_outputs(outs, made, 4, [&] {
+        if (!tables_out || !lens_out || !weights_out || !evicted)
+            clove::fail(CLOVE_HIP_ERR_INVALID, "an output pointer is NULL");
+        HipBackend::paged_evict(deref(block_tables, "block_tables"),
+                                deref(context_lens, "context_lens"), deref(weights, "weights"),
+                                block_size, budget, first, last, made);
     });
 }
 

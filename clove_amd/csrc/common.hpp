@@ -53,6 +53,7 @@ struct Tensor {
     ~Tensor();
 
     float *f32() const { return static_cast<float *>(data); }
+    uint8_t *u8() const { return static_cast<uint8_t *>(data); }
     int32_t *i32() const { return static_cast<int32_t *>(data); }
     size_t dim(int i) const { return shape[i < 0 ? shape.size() + i : i]; }
 };
@@ -61,6 +62,11 @@ struct Tensor {
 using TensorNode = std::shared_ptr<Tensor>;
 
 size_t numel_of(const std::vector<size_t> &shape);
+// Bytes of one element of a dtype: 4 (f32, int32) or 1 (e4m3).
+inline size_t elem_size(int dtype) { return dtype == CLOVE_HIP_E4M3 ? 1 : 4; }
+inline bool known_dtype(int dtype) {
+    return dtype == CLOVE_HIP_F32 || dtype == CLOVE_HIP_I32 || dtype == CLOVE_HIP_E4M3;
+}
 std::string shape_str(const std::vector<size_t> &shape);
 
 // Allocates a device tensor through the caching allocator.

@@ -760,7 +760,7 @@ std::vector<TensorNode> Model::execute(const std::vector<TensorNode> &in, const 
         const Tensor *src = arg(outputs[i]);
         TensorNode t = new_tensor(src->shape, src->dtype);
         if (src->numel)
-            CLOVE_HIP_CHECK(hipMemcpyAsync(t->data, src->data, src->numel * 4,
+            CLOVE_HIP_CHECK(hipMemcpyAsync(t->data, src->data, src->numel * elem_size(src->dtype),
                                            hipMemcpyDeviceToDevice, ctx().stream));
         result[i] = t;
     }

@@ -1,0 +1,157 @@
+// kv8.h -- what the kernels over the 8-bit paged cache share: where a
+// sequence's rows, context and tiles lie, and the e4m3 conversions.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "launch.hpp"
+
+namespace clove {
+namespace k {
+
+constexpr int kKv8MinExp = -60, kKv8MaxExp = 119;
+constexpr float kE4m3Max = 448.0f;
+
+// Sequence b's context length inside its table's capacity.
+__device__ __forceinline__ int kv8_context(const Kv8Args &a, int b) {
+    return min(max(a.context_lens[b], 0), a.max_blocks * a.block_size);
+}
+
+// Sequence b's rows [*first, *first + *n), none where row_starts is not a
+// range inside the rows.
+__device__ __forceinline__ void kv8_rows(const Kv8Args &a, int b, int *first, int *n) {
+    if (!a.row_starts) {
+        *first = b;
+        *n = 1;
+        return;
+    }
+    const int s0 = a.row_starts[b], s1 = a.row_starts[b + 1];
+    const bool ok = s0 >= 0 && s0 <= s1 && s1 <= a.rows;
+    *first = ok ? s0 : 0;
+    *n = ok ? s1 - s0 : 0;
+}
+
+// Reports contexts and row ranges that the two functions above clamped; one
+// wave of a launch calls it.
+__device__ __forceinline__ void kv8_check(const Kv8Args &a) {
+    int bad = 0;
+    for (int b = threadIdx.x & 63; b < a.num_seqs; b += 64) {
+        if (a.context_lens[b] != kv8_context(a, b)) bad |= kErrPagedRange;
+        if (a.row_starts) {
+            const int s0 = a.row_starts[b], s1 = a.row_starts[b + 1];
+            if (s0 < 0 || s0 > s1 || s1 > a.rows) bad |= kErrRowStarts;
+        }
+    }
+    if (bad) atomicOr(a.err_flag, bad);
+}
+
+// Work items of `per` units, `mul` units a row (`extra` more items than
+// floor(units / per) at most).  Sequence b's items get the slots from
+// floor(mul * row_starts[b] / per) + extra * b on: never more than the next
+// sequence's first slot, so kv8_slots() slots serve any split of the rows
+// without the host knowing it.  Returns the sequence a slot belongs to and the
+// item's number within it.
+__host__ __device__ __forceinline__ int64_t kv8_slots(const Kv8Args &a, int per, int mul,
+                                                      int extra) {
+    if (!a.row_starts) return (int64_t)a.num_seqs * ((mul + per - 1) / per);
+    return (int64_t)a.rows * mul / per + (int64_t)extra * a.num_seqs;
+}
+__device__ __forceinline__ int kv8_slot(const Kv8Args &a, int slot, int per, int mul, int extra,
+                                        int *item) {
+    if (!a.row_starts) {
+        const int each = (mul + per - 1) / per;
+        *item = slot % each;
+        return slot / each;
+    }
+    auto base = [&](int b) {
+        const int64_t s = min(max(a.row_starts[b], 0), a.rows);
+        return (int)(s * mul / per) + extra * b;
+    };
+    int lo = 0, hi = a.num_seqs;  // the last b with base(b) <= slot
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (base(mid) <= slot)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    *item = slot - base(lo);
+    return lo;
+}
+
+// The sequence that row r belongs to, or -1.
+__device__ __forceinline__ int kv8_seq_of_row(const Kv8Args &a, int r) {
+    if (a.num_seqs == 0) return -1;
+    if (!a.row_starts) return r;
+    int lo = 0, hi = a.num_seqs;  // the last b with row_starts[b] <= r
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.row_starts[mid] <= r)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    int first, n;
+    kv8_rows(a, lo, &first, &n);
+    return r >= first && r < first + n ? lo : -1;
+}
+
+// Block j of sequence b, or -1 (reported) when its id lies outside the pool.
+__device__ __forceinline__ int64_t kv8_block(const Kv8Args &a, int b, int j, bool report) {
+    const int64_t id = a.block_tables[(size_t)b * a.max_blocks + j];
+    if (id < 0 || id >= a.num_blocks) {
+        if (report) atomicOr(a.err_flag, kErrPagedRange);
+        return -1;
+    }
+    return id;
+}
+
+// Tile (plane, block, head): its number, and the offset of its first code.
+__device__ __forceinline__ size_t kv8_tile(const Kv8Args &a, int plane, int64_t block, int h) {
+    return ((size_t)plane * a.num_blocks + block) * a.num_heads + h;
+}
+__device__ __forceinline__ size_t kv8_tile_offset(const Kv8Args &a, size_t tile) {
+    return tile * (size_t)(a.block_size * a.head_dim);
+}
+
+// 2^e for e in [-126, 127], and for an exponent as stored (what the append
+// never writes is clamped).
+__device__ __forceinline__ float kv8_pow2(int e) {
+    return __uint_as_float((unsigned)(e + 127) << 23);
+}
+__device__ __forceinline__ float kv8_scale(int e) {
+    return kv8_pow2(min(max(e, kKv8MinExp), kKv8MaxExp));
+}
+
+// The smallest e in [-60, 119] with amax <= 448 * 2^e; amax finite, >= 0.  448
+// = 1.75 * 2^8, so the fraction bits decide between exponent - 8 and - 7.
+__device__ __forceinline__ int kv8_exp_of(float amax) {
+    const unsigned u = __float_as_uint(amax);
+    const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return min(max(e, kKv8MinExp), kKv8MaxExp);
+}
+
+__device__ __forceinline__ bool kv8_finite(float x) {
+    return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
+}
+
+// Four floats, already over their tile's scale, as four codes: nearest, ties
+// to even; past +-448 (infinities, values over 448 * 2^119) saturates, NaN is 0.
+__device__ __forceinline__ unsigned kv8_encode4(float a, float b, float c, float d) {
+    auto in = [](float x) { return x != x ? 0.0f : fminf(fmaxf(x, -kE4m3Max), kE4m3Max); };
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(in(a), in(b), 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(in(c), in(d), w, true);
+    return (unsigned)w;
+}
+__device__ __forceinline__ uint8_t kv8_encode(float x) {
+    return (uint8_t)(kv8_encode4(x, 0.f, 0.f, 0.f) & 0xffu);
+}
+__device__ __forceinline__ float kv8_decode(uint8_t code) {
+    return __builtin_amdgcn_cvt_f32_fp8((int)code, 0);
+}
+
+}  // namespace k
+}  // namespace clove

@@ -174,6 +174,8 @@ enum : int32_t {
     kErrPagedRange = 1,  // a block-table entry outside the pool / a context past the table
     kErrClassRange = 2,  // a cross-entropy target >= the number of classes
     kErrIndexValue = 4,  // an f32 index tensor held a value that is not an integer in [0, 2^24)
+    kErrRowStarts = 8,   // row_starts that decrease or leave [0, rows]
+    kErrNotFinite = 16,  // a key or value appended to an 8-bit cache was not finite
 };
 
 // paged_attention.hip
@@ -233,6 +235,52 @@ void paged_slots(const int32_t *block_tables, const int32_t *context_lens, int32
 void paged_index_from_f32(const float *bt_f, int32_t *bt_out, const float *cl_f,
                           const int32_t *cl_i, int32_t *cl_out, int num_seqs, int max_blocks,
                           int block_size, int32_t *err_flag, hipStream_t s);
+
+// kv8_cache.hip, kv8_attention.hip -- the paged cache in 8 bits.  Element
+// (plane p, block n, head h, slot s, dim d) is the e4m3 value of
+// codes[(((p * num_blocks + n) * H + h) * bs + s) * D + d] times
+// 2^exps[(p * num_blocks + n) * H + h]; plane 0 holds keys, plane 1 values.
+// Sequence b's rows are row_starts[b] .. row_starts[b + 1] - 1 (row b alone when
+// row_starts is null) and stand at the last positions of its context.
+struct Kv8Args {
+    uint8_t *codes;
+    int32_t *exps;
+    const int32_t *block_tables;  // [B, max_blocks]
+    const int32_t *context_lens;  // [B]
+    const int32_t *row_starts;    // [B + 1] or null
+    int32_t *err_flag;
+    int64_t num_blocks;
+    int num_seqs, max_blocks, block_size, num_heads, head_dim;
+    int rows;                     // rows of k, v, q or out
+};
+constexpr int kKv8MaxHeadDim = 256;
+// k, v [rows, H * D] into the cache.
+void kv8_append(const Kv8Args &a, const float *k, const float *v, hipStream_t s);
+// The rows' keys and values out of it; rows of no sequence are zeros.
+void kv8_read(const Kv8Args &a, float *k, float *v, hipStream_t s);
+struct Kv8Attention {
+    Kv8Args c;
+    const float *q;    // [rows, q_heads * D]
+    float *out;        // [rows, q_heads * D]
+    int q_heads;       // a multiple of c.num_heads
+    float scale;
+    const float *w_in; // [B, max_blocks] or null
+    float *w_out;
+    float *ws;         // kv8_attention_workspace() bytes
+};
+size_t kv8_attention_workspace(const Kv8Attention &a, int num_cus);
+void kv8_attention(const Kv8Attention &a, int num_cus, hipStream_t s);
+
+// kv8_evict.hip -- eviction of the lightest blocks.
+struct EvictArgs {
+    const int32_t *tables, *lens;
+    const float *weights;
+    int32_t *tables_out, *lens_out, *evicted;
+    float *weights_out;
+    int32_t *err_flag;
+    int num_seqs, max_blocks, block_size, budget, first, last;
+};
+void paged_evict(const EvictArgs &a, hipStream_t s);
 
 }  // namespace k
 }  // namespace clove

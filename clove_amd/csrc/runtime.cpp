@@ -139,13 +139,13 @@ Tensor::~Tensor() {
 }
 
 TensorNode new_tensor(const std::vector<size_t> &shape, int dtype) {
-    CLOVE_REQUIRE(dtype == CLOVE_HIP_F32 || dtype == CLOVE_HIP_I32, CLOVE_HIP_ERR_INVALID,
+    CLOVE_REQUIRE(known_dtype(dtype), CLOVE_HIP_ERR_INVALID,
                   "unknown dtype " + std::to_string(dtype));
     auto t = std::make_shared<Tensor>();
     t->shape = shape;
     t->dtype = dtype;
     t->numel = numel_of(shape);
-    t->data = dev_alloc(t->numel * 4, &t->bytes);
+    t->data = dev_alloc(t->numel * elem_size(dtype), &t->bytes);
     return t;
 }
 
@@ -231,6 +231,12 @@ void synchronize() {
         if (flag & k::kErrIndexValue)
             msg += " an f32 block_tables/context_lens value that is not an integer in "
                    "[0, 2^24) (read as -1: its tokens were skipped);";
+        if (flag & k::kErrRowStarts)
+            msg += " row_starts that decrease or lie outside the rows (those sequences had no "
+                   "rows);";
+        if (flag & k::kErrNotFinite)
+            msg += " a key or value that is not finite, appended to an 8-bit cache (NaN stored as "
+                   "0, an infinity as the largest value of its tile);";
         msg.pop_back();
         fail(CLOVE_HIP_ERR_RANGE, msg);
     }
@@ -250,7 +256,8 @@ void upload(Tensor &t, const void *src, size_t offset, size_t count) {
                       ") past numel " + std::to_string(t.numel));
     if (!count) return;
     Context &c = ctx();
-    CLOVE_HIP_CHECK(hipMemcpyAsync(static_cast<char *>(t.data) + offset * 4, src, count * 4,
+    const size_t es = elem_size(t.dtype);
+    CLOVE_HIP_CHECK(hipMemcpyAsync(static_cast<char *>(t.data) + offset * es, src, count * es,
                                    hipMemcpyHostToDevice, c.stream));
     CLOVE_HIP_CHECK(hipStreamSynchronize(c.stream));
 }
@@ -260,9 +267,10 @@ void download(const Tensor &t, void *dst, size_t offset, size_t count) {
                   "read of [" + std::to_string(offset) + ", " + std::to_string(offset + count) +
                       ") past numel " + std::to_string(t.numel));
     Context &c = ctx();
+    const size_t es = elem_size(t.dtype);
     if (count)
-        CLOVE_HIP_CHECK(hipMemcpyAsync(dst, static_cast<const char *>(t.data) + offset * 4,
-                                       count * 4, hipMemcpyDeviceToHost, c.stream));
+        CLOVE_HIP_CHECK(hipMemcpyAsync(dst, static_cast<const char *>(t.data) + offset * es,
+                                       count * es, hipMemcpyDeviceToHost, c.stream));
     synchronize();
 }
 

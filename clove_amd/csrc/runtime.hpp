@@ -111,6 +111,24 @@ struct HipBackend {
                                            const TensorNode &context_lens, int block_size,
                                            int max_ctx);
 
+    // The paged KV cache in 8 bits and block eviction (kv8.cpp).
+    static void paged_kv8_append(const Tensor &codes, const Tensor &exps, const Tensor &k,
+                                 const Tensor &v, const Tensor &block_tables,
+                                 const Tensor &context_lens, const Tensor *row_starts);
+    static void paged_kv8_read(const Tensor &codes, const Tensor &exps,
+                               const Tensor &block_tables, const Tensor &context_lens,
+                               const Tensor *row_starts, size_t rows, TensorNode *k,
+                               TensorNode *v);
+    static TensorNode paged_kv8_attention(const Tensor &q, const Tensor &codes,
+                                          const Tensor &exps, const Tensor &block_tables,
+                                          const Tensor &context_lens, const Tensor *row_starts,
+                                          float scale, const Tensor *weights,
+                                          TensorNode *weights_out);
+    // out: the tables, lengths and weights of the kept blocks, the evicted ids.
+    static void paged_evict(const Tensor &block_tables, const Tensor &context_lens,
+                            const Tensor &weights, int block_size, int budget, int first,
+                            int last, TensorNode out[4]);
+
     // Backward passes and losses (grad.cpp; the autograd closures of
     // backend.rs).
     static TensorNode relu_backward(const TensorNode &x, const TensorNode &grad_out);

@@ -7,7 +7,7 @@
  * sizes and opaque handles; no C++ or torch types cross it.
  *
  * Conventions
- *   - A CTensor is an opaque handle to one device allocation (f32 or int32)
+ *   - A CTensor is an opaque handle to one device allocation (f32, int32 or e4m3)
  *     plus its shape, mirroring ffi.rs:35 `pub type CTensor = *mut c_void`.
  *   - Ops return a NEW handle that the caller frees with clove_hip_tensor_free
  *     (ffi.rs:119-266).  On any error they return NULL and record a message
@@ -45,7 +45,9 @@ enum clove_hip_status {
     CLOVE_HIP_ERR_RANGE = 7      /* an index (block table, context length) is out of range */
 };
 
-enum clove_hip_dtype { CLOVE_HIP_F32 = 0, CLOVE_HIP_I32 = 1 };
+/* E4M3: one byte an element (the codes of an 8-bit KV cache: sign, 4 exponent
+ * bits of bias 7, 3 fraction bits; no infinities, 0x7F and 0xFF are NaN). */
+enum clove_hip_dtype { CLOVE_HIP_F32 = 0, CLOVE_HIP_I32 = 1, CLOVE_HIP_E4M3 = 2 };
 
 /* Opcodes: the hot-path subset of Clove's IR (backend.rs:85-127), used by the
  * fused-chain entry and by the graph builder. */
@@ -119,7 +121,7 @@ CTensor clove_hip_tensor_wrap(void *device_ptr, const size_t *shape, size_t ndim
 void clove_hip_tensor_free(CTensor t);
 /* ffi.rs:99-113 clove_tensor_data: downloads all elements (f32 tensors). */
 int clove_hip_tensor_data(CTensor t, float *out);
-/* Element-range download / upload for either dtype (offset and count in elements). */
+/* Element-range download / upload for any dtype (offset and count in elements). */
 int clove_hip_tensor_read(CTensor t, void *out, size_t offset, size_t count);
 int clove_hip_tensor_write(CTensor t, const void *src, size_t offset, size_t count);
 size_t clove_hip_tensor_ndim(CTensor t);
@@ -229,6 +231,76 @@ int clove_hip_paged_kv_append(CTensor kv_cache, CTensor k, CTensor v, CTensor bl
  * on the device by the same index code the attention kernel uses. */
 CTensor clove_hip_paged_gather_indices(CTensor block_tables, CTensor context_lens,
                                        int block_size, int max_ctx);
+
+/* ---------------------------------------------------------------------- */
+/* The paged KV cache in 8 bits (no counterpart in the reference): a       */
+/* quarter of the f32 cache's memory and traffic, query heads in groups,   */
+/* several rows of a sequence in one call, and eviction of light blocks.   */
+/* ---------------------------------------------------------------------- */
+
+/* The cache is two tensors the caller creates:
+ *   codes  e4m3  [2, num_blocks, H, block_size, D]  (plane 0 keys, 1 values)
+ *   exps   int32 [2, num_blocks, H]
+ * and an element stands for its code times 2^exp of its tile (one head of one
+ * block).  D is 1..256, block_size >= 1.  Neither needs initialising.
+ *
+ * Rows.  context_lens[b] (int32 [B]) counts sequence b's tokens, the rows of
+ * the call among them.  row_starts (int32 [B + 1]) says that rows
+ * row_starts[b] .. row_starts[b + 1] - 1 are sequence b's; they stand at its
+ * last n_b positions, context_lens[b] - n_b and up.  Rows at negative
+ * positions (n_b > context_lens[b]) are skipped: not stored, read as zeros,
+ * attended as zeros; so are rows that belong to no sequence.  NULL means one
+ * row for each sequence (rows == B).  block_tables is int32 [B, max_blocks].
+ *
+ * Errors that only the device sees (a block id outside the pool, a context
+ * past its table, row_starts that decrease or leave [0, rows]) skip the tokens
+ * or rows concerned and are reported as CLOVE_HIP_ERR_RANGE by the next
+ * synchronising call, as for the f32 cache. */
+
+/* Stores the rows' keys and values (f32 [rows, H*D]).  A tile's exponent is the
+ * smallest e in [-60, 119] with |x| <= 448 * 2^e for what it holds; codes are
+ * x * 2^-e rounded to nearest, ties to even, so an element is off by at most
+ * 2^-4 of itself (half of 2^(e-9) for the smallest).  A tile whose first slot is among the new rows
+ * starts afresh; otherwise its exponent only grows, and when it does the tokens
+ * it held are rounded again under the new one (their exponents shift: bits are
+ * lost only where a code becomes subnormal).  Slots behind the new rows keep their bytes.
+ * NaN is stored as 0 and an infinity as the largest value of its tile, and both
+ * are reported like an index error.  No two sequences of a call may write the
+ * same block (such a block's tile holds a mixture, always finite). */
+int clove_hip_paged_kv8_append(CTensor codes, CTensor exps, CTensor k, CTensor v,
+                               CTensor block_tables, CTensor context_lens, CTensor row_starts);
+/* The inverse: *k and *v receive new f32 [rows, H*D] tensors with the values
+ * that the cache holds for the rows (B rows when row_starts is NULL). */
+int clove_hip_paged_kv8_read(CTensor codes, CTensor exps, CTensor block_tables,
+                             CTensor context_lens, CTensor row_starts, size_t rows, CTensor *k,
+                             CTensor *v);
+/* Attention of the rows over the cache, which holds them already (append
+ * first).  q is f32 [rows, Hq*D] with Hq a multiple G of H; query head h reads
+ * key head h / G.  A row sees the tokens up to its own position; out (q's
+ * shape) = softmax(scale * q.K^T) V, scale <= 0 selects 1/sqrt(D).  Without
+ * row_starts this is the decode step, with them a later chunk of a prompt, a
+ * whole prompt, speculated tokens, or any mixture.
+ * weights (f32 [B, max_blocks]) and weights_out go together, both or neither:
+ * *weights_out receives a new tensor weights[b][j] + the sum, over the rows and
+ * query heads of sequence b and the tokens of its block j, of the softmax
+ * weights; entries past a context are copied.  Sums run in a fixed order. */
+CTensor clove_hip_paged_kv8_attention(CTensor q, CTensor codes, CTensor exps,
+                                      CTensor block_tables, CTensor context_lens,
+                                      CTensor row_starts, float scale, CTensor weights,
+                                      CTensor *weights_out);
+/* Cuts every sequence of more than `budget` blocks down to `budget`: its
+ * `first` first and `last` last blocks (last >= 1: the newest block may be part
+ * full) stay, and of those between them the ones of greatest weight (equal
+ * weights: the earlier block; NaN ranks below every number).  The kept blocks
+ * keep their order; only tables change, no cache memory moves.  New tensors:
+ * *tables_out (int32 [B, max_blocks], -1 behind), *lens_out (int32 [B]),
+ * *weights_out (f32 [B, max_blocks], 0 behind) and *evicted (int32
+ * [B, max_blocks], the ids of the blocks that are free now, in order, -1 behind).
+ * Works on the tables of either cache; positions inside keys (RoPE) stay what
+ * they were when the keys were stored. */
+int clove_hip_paged_evict(CTensor block_tables, CTensor context_lens, CTensor weights,
+                          int block_size, int budget, int first, int last, CTensor *tables_out,
+                          CTensor *lens_out, CTensor *weights_out, CTensor *evicted);
 
 /* ---------------------------------------------------------------------- */
 /* Backward passes and losses: the autograd closures WgpuBackend attaches  */
