@@ -153,5 +153,57 @@ __device__ __forceinline__ float kv8_decode(uint8_t code) {
     return __builtin_amdgcn_cvt_f32_fp8((int)code, 0);
 }
 
+// ---- attention: how a call is cut into workgroups ---------------------------
+
+// Query rows of one kv head are its sequence's (row, query head of the group)
+// pairs, u = i * G + g; a tile is `tile` of them, a part `part_tokens` tokens.
+struct Kv8Split {
+    int kind;          // one of the KV8_ kernels
+    int dp;            // head_dim the kernel is laid out for
+    int tile;
+    int parts, part_tokens;
+    unsigned slots;    // row tiles (kv8_slots)
+    int stored;        // rows of a partial result
+    int sums;          // tokens to a stored sum of weights, 0: none stored
+    int groups;        // such sums a row
+    // in the workspace, in floats; partial (slot, head, part) is `stored` rows
+    size_t o_at, ml_at;      // partial sums over V [D], (maximum, sum) pairs
+    size_t row_ml_at;        // (maximum, 1 / sum) of every row and query head
+    size_t sums_at;          // [row, query head][groups] (sum, maximum) pairs
+    size_t floats;
+};
+enum { KV8_ANY = 0, KV8_STREAM = 1, KV8_TILE = 2 };
+
+// The rows of a tile and the tokens they see.
+struct Kv8Tile {
+    int first, n, ctx;   // the sequence's rows and context
+    int r0, rows;        // the tile's first (row, head) pair and how many it has
+    int low, high;       // tokens its first row sees, and its last
+};
+// The slot of sequence b's first item.
+__device__ __forceinline__ int kv8_first_slot(const Kv8Args &a, int b, int per, int mul,
+                                              int extra) {
+    if (!a.row_starts) return b * ((mul + per - 1) / per);
+    const int64_t s = min(max(a.row_starts[b], 0), a.rows);
+    return (int)(s * mul / per) + extra * b;
+}
+// False where the slot holds no tile.
+__device__ __forceinline__ bool kv8_tile_of(const Kv8Args &c, int G, int slot, int tile, int *b,
+                                            Kv8Tile *t) {
+    int item;
+    *b = kv8_slot(c, slot, tile, G, 1, &item);
+    kv8_rows(c, *b, &t->first, &t->n);
+    t->ctx = kv8_context(c, *b);
+    const int R = t->n * G;
+    t->r0 = item * tile;
+    if (item < 0 || t->r0 >= R) return false;
+    t->rows = min(tile, R - t->r0);
+    t->low = t->ctx - t->n + t->r0 / G + 1;
+    t->high = t->ctx - t->n + (t->r0 + t->rows - 1) / G + 1;
+    return true;
+}
+
+void kv8_stream(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
+
 }  // namespace k
 }  // namespace clove
