@@ -156,23 +156,33 @@ __device__ __forceinline__ float kv8_decode(uint8_t code) {
 // ---- attention: how a call is cut into workgroups ---------------------------
 
 // Query rows of one kv head are its sequence's (row, query head of the group)
-// pairs, u = i * G + g; a tile is `tile` of them, a part `part_tokens` tokens.
+// pairs, u = i * G + g; a tile is `tile` of them.
+//
+// KV8_STREAM cuts all tiles' contexts into steps of kKv8Step tokens, numbers the
+// steps sequence by sequence, tile by tile, head by head, and gives each
+// workgroup an equal run of them, whatever the lengths are: `share` steps, known
+// on the device alone.  A tile that one workgroup holds whole is written by it;
+// of a tile cut in pieces every workgroup stores its piece, at most one at
+// the front of its run and one at its end.
 struct Kv8Split {
     int kind;          // one of the KV8_ kernels
     int dp;            // head_dim the kernel is laid out for
     int tile;
-    int parts, part_tokens;
-    unsigned slots;    // row tiles (kv8_slots)
-    int stored;        // rows of a partial result
+    int grid;          // KV8_STREAM: workgroups that share the steps
+    bool join;         // whether a tile may be cut
+    int stored;        // rows of a piece
     int sums;          // tokens to a stored sum of weights, 0: none stored
     int groups;        // such sums a row
-    // in the workspace, in floats; partial (slot, head, part) is `stored` rows
-    size_t o_at, ml_at;      // partial sums over V [D], (maximum, sum) pairs
+    // in the workspace, in floats
+    size_t o_at, ml_at;      // piece 2w (+ 1: at the end of the run) of workgroup w:
+                             // `stored` sums over V [D], and (maximum, sum) pairs
+    size_t start_at;         // [slot, head] first step of the tile (int64), then share
     size_t row_ml_at;        // (maximum, 1 / sum) of every row and query head
     size_t sums_at;          // [row, query head][groups] (sum, maximum) pairs
     size_t floats;
 };
-enum { KV8_ANY = 0, KV8_STREAM = 1, KV8_TILE = 2 };
+enum { KV8_ANY = 0, KV8_STREAM = 1 };
+constexpr int kKv8Step = 128;
 
 // The rows of a tile and the tokens they see.
 struct Kv8Tile {
@@ -187,13 +197,11 @@ __device__ __forceinline__ int kv8_first_slot(const Kv8Args &a, int b, int per, 
     const int64_t s = min(max(a.row_starts[b], 0), a.rows);
     return (int)(s * mul / per) + extra * b;
 }
-// False where the slot holds no tile.
-__device__ __forceinline__ bool kv8_tile_of(const Kv8Args &c, int G, int slot, int tile, int *b,
+// Tile `item` of sequence b; false where there is none.
+__device__ __forceinline__ bool kv8_tile_of(const Kv8Args &c, int G, int b, int item, int tile,
                                             Kv8Tile *t) {
-    int item;
-    *b = kv8_slot(c, slot, tile, G, 1, &item);
-    kv8_rows(c, *b, &t->first, &t->n);
-    t->ctx = kv8_context(c, *b);
+    kv8_rows(c, b, &t->first, &t->n);
+    t->ctx = kv8_context(c, b);
     const int R = t->n * G;
     t->r0 = item * tile;
     if (item < 0 || t->r0 >= R) return false;
@@ -203,6 +211,8 @@ __device__ __forceinline__ bool kv8_tile_of(const Kv8Args &c, int G, int slot, i
     return true;
 }
 
+// Workgroups of the stream kernel that a CU holds.
+int kv8_stream_residents(int dp, int tile);
 void kv8_stream(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
 
 }  // namespace k

@@ -114,59 +114,6 @@ __global__ void __launch_bounds__(256) kv8_weights_any_kernel(Kv8Attention a, co
     if (threadIdx.x == 0) a.w_out[at] = a.w_in[at] + part[0];
 }
 
-// Joins the parts of one row and query head; the workgroup's waves take parts
-// in turn, a lane up to four dims.
-__global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split p) {
-    const Kv8Args &c = a.c;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
-    const int hq = blockIdx.x % a.q_heads, row = blockIdx.x / a.q_heads;
-    const int D = c.head_dim, G = a.q_heads / c.num_heads, h = hq / G;
-    const size_t rh = (size_t)row * a.q_heads + hq;
-    __shared__ float s_o[16][kKv8MaxHeadDim], s_l[16];
-    const int b = kv8_seq_of_row(c, row);
-    int np = 0;
-    size_t base = 0;
-    if (b >= 0) {
-        int first, n;
-        kv8_rows(c, b, &first, &n);
-        const int u = (row - first) * G + hq % G, item = u / p.tile;
-        const int last = (min((item + 1) * p.tile, n * G) - 1) / G;
-        const int high = kv8_context(c, b) - n + last + 1;
-        np = high > 0 ? (high + p.part_tokens - 1) / p.part_tokens : 0;
-        const size_t slot = kv8_first_slot(c, b, p.tile, G, 1) + item;
-        base = ((slot * c.num_heads + h) * p.parts) * p.stored + u % p.tile;
-    }
-    const float2 *ml = reinterpret_cast<const float2 *>(a.ws + p.ml_at) + base;
-    const float *o = a.ws + p.o_at + base * D;
-    float top = -INFINITY;
-    for (int i = lane; i < np; i += 64) top = fmaxf(top, ml[(size_t)i * p.stored].x);
-    top = wave_max(top);
-    float l = 0.0f, x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int i = wave; i < np; i += waves) {
-        const float2 v = ml[(size_t)i * p.stored];
-        const float f = v.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v.x - top);
-        l += v.y * f;
-        const float *oi = o + (size_t)i * p.stored * D;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (lane + 64 * e < D) x[e] = fmaf(oi[lane + 64 * e], f, x[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (lane + 64 * e < D) s_o[wave][lane + 64 * e] = x[e];
-    if (lane == 0) s_l[wave] = l;
-    __syncthreads();
-    l = 0.0f;
-    for (int w = 0; w < waves; ++w) l += s_l[w];
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    for (int d = tid; d < D; d += blockDim.x) {
-        float sum = 0.0f;
-        for (int w = 0; w < waves; ++w) sum += s_o[w][d];
-        a.out[rh * D + d] = sum * inv;
-    }
-    if (tid == 0 && p.sums) reinterpret_cast<float2 *>(a.ws + p.row_ml_at)[rh] = make_float2(top, inv);
-}
-
 // The weight of each block from the sums stored on the way: lanes take 64
 // blocks, the four waves a sequence's rows and heads in turn.
 __global__ void __launch_bounds__(256) kv8_weights_kernel(Kv8Attention a, Kv8Split p) {
@@ -211,9 +158,12 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
         p.floats += (size_t)((n + 3) / 4 * 4);
         return at;
     };
-    const bool fast = D % 16 == 0 && bs % 4 == 0 && bs <= 4096 && c.num_seqs > 0 &&
-                      c.rows > 0 && c.num_blocks > 0 && c.max_blocks > 0 &&
-                      (reinterpret_cast<uintptr_t>(c.codes) & 15) == 0;
+    // 16-byte pieces of every row, four tokens to a block, rows of the pool
+    // numbered in 32 bits, grids within theirs
+    const bool fast = D % 16 == 0 && bs % 4 == 0 && c.num_seqs > 0 && c.rows > 0 &&
+                      c.num_blocks > 0 && c.max_blocks > 0 && rh < (1 << 24) &&
+                      c.num_blocks * c.num_heads * bs < (1ll << 32) &&
+                      ((reinterpret_cast<uintptr_t>(c.codes) | reinterpret_cast<uintptr_t>(a.q)) & 15) == 0;
     if (!fast) {
         if (a.w_out) p.row_ml_at = take(2 * rh);
         return p;
@@ -224,26 +174,14 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
     const int64_t units = ((int64_t)c.rows * G + c.num_seqs - 1) / c.num_seqs;
     p.tile = units <= 16 || p.dp == 256 ? 16 : 32;
     p.stored = !c.row_starts && G < p.tile ? G : p.tile;
-    const int64_t slots = kv8_slots(c, p.tile, G, 1);
-    const int64_t cap = (int64_t)c.max_blocks * bs;
-    // enough workgroups to fill the chip a few times over, parts of 256 tokens
-    // at least and of as many blocks as a workgroup's table holds at most
-    const int64_t want = std::max<int64_t>(1, (int64_t)cus * 8 / std::max<int64_t>(1, slots * c.num_heads));
-    int64_t tokens = std::max<int64_t>(256, (cap + want - 1) / want);
-    tokens = std::min<int64_t>(tokens, (int64_t)1000 * bs);
-    tokens = std::max<int64_t>(128, tokens / 128 * 128);
-    p.part_tokens = (int)tokens;
-    p.parts = (int)((cap + tokens - 1) / tokens);
-    const int64_t wgs = slots * c.num_heads * p.parts;
-    if (wgs >= (1 << 23) || rh >= (1 << 22)) {  // past a grid: the plain kernel
-        p = Kv8Split{};
-        if (a.w_out) p.row_ml_at = take(2 * rh);
-        return p;
-    }
-    p.slots = (unsigned)slots;
-    if (p.parts > 1) {
-        p.o_at = take(wgs * p.stored * D);
-        p.ml_at = take(wgs * p.stored * 2);
+    const int64_t tiles = kv8_slots(c, p.tile, G, 1) * c.num_heads;
+    const int64_t cap = (int64_t)c.max_blocks * bs, steps = (cap + kKv8Step - 1) / kKv8Step;
+    p.join = steps > 1;
+    p.grid = (int)std::min<int64_t>(std::min(1024, cus * kv8_stream_residents(p.dp, p.tile)), tiles * steps);
+    if (p.join) {
+        p.o_at = take((int64_t)2 * p.grid * p.stored * D);
+        p.ml_at = take((int64_t)2 * p.grid * p.stored * 2);
+        p.start_at = take(2 * (1 + tiles));
     }
     if (a.w_out) {
         p.sums = bs % 16 == 0 ? 16 : 4;
@@ -272,10 +210,6 @@ void kv8_attention(const Kv8Attention &a, int cus, hipStream_t s) {
         return;
     }
     kv8_stream(a, p, s);
-    if (p.parts > 1) {
-        const int waves = std::min(16, std::max(1, p.parts / 8));
-        kv8_join_kernel<<<(unsigned)c.rows * a.q_heads, 64 * waves, 0, s>>>(a, p);
-    }
     if (weights)
         kv8_weights_kernel<<<dim3((c.max_blocks + 63) / 64, c.num_seqs), 256, 0, s>>>(a, p);
 }
