@@ -158,17 +158,18 @@ __device__ __forceinline__ float kv8_decode(uint8_t code) {
 // Query rows of one kv head are its sequence's (row, query head of the group)
 // pairs, u = i * G + g; a tile is `tile` of them.
 //
-// KV8_STREAM cuts all tiles' contexts into steps of kKv8Step tokens, numbers the
-// steps sequence by sequence, tile by tile, head by head, and gives each
-// workgroup an equal run of them, whatever the lengths are: `share` steps, known
-// on the device alone.  A tile that one workgroup holds whole is written by it;
-// of a tile cut in pieces every workgroup stores its piece, at most one at
-// the front of its run and one at its end.
+// All tiles' contexts are cut into steps of `step` tokens, numbered sequence by
+// sequence, tile by tile, head by head, and each workgroup gets an equal run of
+// them, whatever the lengths are: `share` steps, known on the device alone.  A
+// tile that one workgroup holds whole is written by it; of a tile cut in pieces
+// every workgroup stores its piece, at most one at the front of its run and
+// one at its end, and kv8_join puts them together.
 struct Kv8Split {
     int kind;          // one of the KV8_ kernels
     int dp;            // head_dim the kernel is laid out for
     int tile;
-    int grid;          // KV8_STREAM: workgroups that share the steps
+    int step;
+    int grid;          // workgroups that share the steps, at most kKv8MaxGrid
     bool join;         // whether a tile may be cut
     int stored;        // rows of a piece
     int sums;          // tokens to a stored sum of weights, 0: none stored
@@ -181,8 +182,8 @@ struct Kv8Split {
     size_t sums_at;          // [row, query head][groups] (sum, maximum) pairs
     size_t floats;
 };
-enum { KV8_ANY = 0, KV8_STREAM = 1 };
-constexpr int kKv8Step = 128;
+enum { KV8_ANY = 0, KV8_STREAM = 1, KV8_TILE = 2 };
+constexpr int kKv8StreamStep = 128, kKv8TileStep = 64, kKv8MaxGrid = 1024;
 
 // The rows of a tile and the tokens they see.
 struct Kv8Tile {
@@ -211,9 +212,122 @@ __device__ __forceinline__ bool kv8_tile_of(const Kv8Args &c, int G, int b, int 
     return true;
 }
 
+// Steps of a tile whose last row sees `high` tokens.
+__device__ __forceinline__ int kv8_steps(int high, int step) { return (max(high, 0) + step - 1) / step; }
+
+// Where a workgroup's run of steps begins.
+struct Kv8Place {
+    int b, item, h, step;
+    int64_t share, total;
+};
+
+// All 256 threads: the steps before each sequence are summed up (in one order
+// everywhere), and step `share * w` is looked up in them.
+__device__ __forceinline__ Kv8Place kv8_find_place(const Kv8Args &c, int G, int tile, int step,
+                                                    int grid, int w, int64_t *s_wave,
+                                                    Kv8Place *s_place) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, H = c.num_heads;
+    const int per = (c.num_seqs + 255) / 256;
+    auto steps = [&](int b) {
+        int64_t sum = 0;
+        Kv8Tile t;
+        for (int item = 0; kv8_tile_of(c, G, b, item, tile, &t); ++item) sum += kv8_steps(t.high, step);
+        return sum * H;
+    };
+    int64_t mine = 0;
+    for (int b = tid * per; b < min((tid + 1) * per, c.num_seqs); ++b) mine += steps(b);
+    int64_t inc = mine;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t up = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += up;
+    }
+    if (lane == 63) s_wave[wave] = inc;
+    if (tid == 0) s_place->b = -1;
+    __syncthreads();
+    const int64_t total = s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
+    int64_t at = inc - mine;
+    for (int i = 0; i < wave; ++i) at += s_wave[i];
+    const int64_t share = max((total + grid - 1) / grid, (int64_t)1);
+    const int64_t want = share * w;
+    if (want >= at && want < at + mine) {
+        for (int b = tid * per; b < min((tid + 1) * per, c.num_seqs); ++b) {
+            Kv8Tile t;
+            for (int item = 0; kv8_tile_of(c, G, b, item, tile, &t); ++item) {
+                const int n = kv8_steps(t.high, step);
+                if (want >= at && want < at + (int64_t)n * H) {
+                    s_place->b = b;
+                    s_place->item = item;
+                    s_place->h = (int)((want - at) / n);
+                    s_place->step = (int)((want - at) % n);
+                }
+                at += (int64_t)n * H;
+            }
+        }
+    }
+    __syncthreads();
+    Kv8Place p = *s_place;
+    p.share = share;
+    p.total = total;
+    return p;
+}
+
+// Moves `at` on to the next tile with steps; false behind the last.
+__device__ __forceinline__ bool kv8_next_tile(const Kv8Args &c, int G, int tile, Kv8Place *at,
+                                              Kv8Tile *T) {
+    if (at->h >= c.num_heads) {
+        at->h = 0;
+        ++at->item;
+    }
+    while (at->b < c.num_seqs) {
+        if (!kv8_tile_of(c, G, at->b, at->item, tile, T)) {
+            ++at->b;
+            at->item = 0;
+        } else if (T->high <= 0) {
+            ++at->item;
+        } else {
+            return true;
+        }
+    }
+    return false;
+}
+
+// Workgroups behind the others, of 256 threads, a wave a row: zeros for the rows
+// of no sequence and those without a token to see.
+inline unsigned kv8_zero_grid(const Kv8Args &c) { return (c.rows + 3) / 4; }
+__device__ __forceinline__ void kv8_zero_rows(const Kv8Attention &a, int block) {
+    const Kv8Args &c = a.c;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = block * 4 + wave;
+    if (block == 0 && wave == 0) kv8_check(c);
+    if (r >= c.rows) return;
+    const int b = kv8_seq_of_row(c, r);
+    int see = 0;
+    if (b >= 0) {
+        int first, n;
+        kv8_rows(c, b, &first, &n);
+        see = kv8_context(c, b) - n + (r - first) + 1;
+    }
+    if (see > 0) return;
+    const int X = a.q_heads * c.head_dim;
+    for (int d = lane; d < X; d += 64) a.out[(size_t)r * X + d] = 0.0f;
+}
+
+constexpr float kKv8Slack = 8.0f;  // a maximum moves when a score exceeds it by this (base 2)
+constexpr float kLog2e = 1.44269504088896341f;
+
+// Two e4m3 codes, times a power of two, as two bf16: exact.
+template <bool HIGH>
+__device__ __forceinline__ unsigned kv8_widen(unsigned codes, float scale) {
+    return __builtin_bit_cast(unsigned,
+                              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, HIGH));
+}
+
 // Workgroups of the stream kernel that a CU holds.
 int kv8_stream_residents(int dp, int tile);
 void kv8_stream(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
+void kv8_tiles(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
+// The weights of the blocks, the scores computed again (kv8_tiles has left every
+// row's maximum and sum).
+void kv8_tile_weights(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
 
 }  // namespace k
 }  // namespace clove

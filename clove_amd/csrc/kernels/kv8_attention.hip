@@ -114,6 +114,76 @@ __global__ void __launch_bounds__(256) kv8_weights_any_kernel(Kv8Attention a, co
     if (threadIdx.x == 0) a.w_out[at] = a.w_in[at] + part[0];
 }
 
+// Joins the pieces of one row and query head, the workgroup's waves in turn, a
+// lane up to four dims.
+__global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split p) {
+    const Kv8Args &c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+    const int hq = blockIdx.x % a.q_heads, row = blockIdx.x / a.q_heads;
+    const int D = c.head_dim, H = c.num_heads, G = a.q_heads / H, h = hq / G;
+    __shared__ float s_o[16][kKv8MaxHeadDim], s_f[kKv8MaxGrid], s_l[16], s_top[16];
+    const int b = kv8_seq_of_row(c, row);
+    if (b < 0) return;
+    int first, n;
+    kv8_rows(c, b, &first, &n);
+    const int u = (row - first) * G + hq % G;
+    Kv8Tile T;
+    if (!kv8_tile_of(c, G, b, u / p.tile, p.tile, &T) || T.high <= 0) return;
+    const int64_t *starts = reinterpret_cast<const int64_t *>(a.ws + p.start_at);
+    const int64_t share = starts[0];
+    const size_t slot = kv8_first_slot(c, b, p.tile, G, 1) + u / p.tile;
+    const int64_t start = starts[1 + slot * H + h], end = start + kv8_steps(T.high, p.step);
+    const int64_t w0 = start / share;
+    const int np = (int)((end - 1) / share - w0) + 1;
+    if (np == 1) return;  // written whole
+    // the first piece ends its workgroup's run unless the run begins with it
+    auto place = [&](int i) {
+        const int64_t w = w0 + i;
+        return (size_t)(2 * w + (i == 0 && start != w * share ? 1 : 0)) * p.stored + u % p.tile;
+    };
+    const float2 *ml = reinterpret_cast<const float2 *>(a.ws + p.ml_at);
+    float top = -INFINITY, x[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.0f;
+    for (int i = tid; i < np; i += blockDim.x) {
+        s_f[i] = ml[place(i)].x;
+        top = fmaxf(top, s_f[i]);
+    }
+    top = wave_max(top);
+    if (lane == 0) s_top[wave] = top;
+    __syncthreads();
+    for (int w = 0; w < waves; ++w) top = fmaxf(top, s_top[w]);
+    for (int i = tid; i < np; i += blockDim.x) {
+        const float f = s_f[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_f[i] - top);
+        l += ml[place(i)].y * f;
+        s_f[i] = f;
+    }
+    l = wave_sum(l);
+    __syncthreads();
+    const float *o = a.ws + p.o_at;
+#pragma unroll 4
+    for (int i = wave; i < np; i += waves) {
+        const float f = s_f[i], *oi = o + place(i) * D;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (lane + 64 * e < D) x[e] = fmaf(oi[lane + 64 * e], f, x[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (lane + 64 * e < D) s_o[wave][lane + 64 * e] = x[e];
+    if (lane == 0) s_l[wave] = l;
+    __syncthreads();
+    l = 0.0f;
+    for (int w = 0; w < waves; ++w) l += s_l[w];
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const size_t rh = (size_t)row * a.q_heads + hq;
+    for (int d = tid; d < D; d += blockDim.x) {
+        float sum = 0.0f;
+        for (int w = 0; w < waves; ++w) sum += s_o[w][d];
+        a.out[rh * D + d] = sum * inv;
+    }
+    if (tid == 0 && a.w_out)
+        reinterpret_cast<float2 *>(a.ws + p.row_ml_at)[rh] = make_float2(top, inv);
+}
+
 // The weight of each block from the sums stored on the way: lanes take 64
 // blocks, the four waves a sequence's rows and heads in turn.
 __global__ void __launch_bounds__(256) kv8_weights_kernel(Kv8Attention a, Kv8Split p) {
@@ -168,26 +238,43 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
         if (a.w_out) p.row_ml_at = take(2 * rh);
         return p;
     }
-    p.kind = KV8_STREAM;
     p.dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
     // rows of one sequence and kv head, on the average
     const int64_t units = ((int64_t)c.rows * G + c.num_seqs - 1) / c.num_seqs;
-    p.tile = units <= 16 || p.dp == 256 ? 16 : 32;
+    const int64_t cap = (int64_t)c.max_blocks * bs;
+    int residents;
+    if (units <= (p.dp == 256 ? 16 : 32)) {
+        p.kind = KV8_STREAM;
+        p.tile = units <= 16 || p.dp == 256 ? 16 : 32;
+        p.step = kKv8StreamStep;
+        residents = kv8_stream_residents(p.dp, p.tile);
+    } else {
+        p.kind = KV8_TILE;
+        p.tile = units <= 64 || p.dp == 256 ? 64 : 128;
+        p.step = p.dp == 256 ? 32 : kKv8TileStep;
+        residents = 2;
+    }
     p.stored = !c.row_starts && G < p.tile ? G : p.tile;
     const int64_t tiles = kv8_slots(c, p.tile, G, 1) * c.num_heads;
-    const int64_t cap = (int64_t)c.max_blocks * bs, steps = (cap + kKv8Step - 1) / kKv8Step;
-    p.join = steps > 1;
-    p.grid = (int)std::min<int64_t>(std::min(1024, cus * kv8_stream_residents(p.dp, p.tile)), tiles * steps);
+    const int64_t steps = (cap + p.step - 1) / p.step;
+    const int64_t room = std::min(kKv8MaxGrid, cus * residents);
+    p.join = steps > 1 && (p.kind == KV8_STREAM || tiles < 2 * room);
+    p.grid = (int)(p.join || p.kind == KV8_STREAM ? std::min<int64_t>(room, tiles * steps) : tiles);
     if (p.join) {
         p.o_at = take((int64_t)2 * p.grid * p.stored * D);
         p.ml_at = take((int64_t)2 * p.grid * p.stored * 2);
         p.start_at = take(2 * (1 + tiles));
     }
     if (a.w_out) {
-        p.sums = bs % 16 == 0 ? 16 : 4;
-        p.groups = (int)((cap + p.sums - 1) / p.sums);
         p.row_ml_at = take(2 * rh);
-        p.sums_at = take(2 * rh * p.groups);
+        if (p.kind == KV8_STREAM) {
+            p.sums = bs % 16 == 0 ? 16 : 4;
+            p.groups = (int)((cap + p.sums - 1) / p.sums);
+            p.sums_at = take(2 * rh * p.groups);
+        } else {
+            p.groups = (int)((cap + 3) / 4);
+            p.sums_at = take((int64_t)c.num_seqs * c.num_heads * p.groups);
+        }
     }
     return p;
 }
@@ -209,8 +296,18 @@ void kv8_attention(const Kv8Attention &a, int cus, hipStream_t s) {
             kv8_weights_any_kernel<<<dim3(c.max_blocks, c.num_seqs), 256, 0, s>>>(a, ml);
         return;
     }
-    kv8_stream(a, p, s);
-    if (weights)
+    if (p.kind == KV8_STREAM)
+        kv8_stream(a, p, s);
+    else
+        kv8_tiles(a, p, s);
+    if (p.join) {
+        // one workgroup a row and head; many waves where few rows have many pieces
+        const unsigned n = (unsigned)c.rows * a.q_heads;
+        kv8_join_kernel<<<n, n <= 64 ? 1024 : n <= 1024 ? 256 : 64, 0, s>>>(a, p);
+    }
+    if (weights && p.kind == KV8_TILE)
+        kv8_tile_weights(a, p, s);
+    else if (weights)
         kv8_weights_kernel<<<dim3((c.max_blocks + 63) / 64, c.num_seqs), 256, 0, s>>>(a, p);
 }
 

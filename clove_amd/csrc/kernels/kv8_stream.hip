@@ -25,8 +25,7 @@ namespace k {
 namespace {
 
 constexpr int kChunk = 4096;    // tokens whose rows a workgroup's table holds
-constexpr int kMaxGrid = 1024;   // workgroups that share the steps
-constexpr float kSlack = 8.0f;  // a maximum moves when a score exceeds it by this (base 2)
+constexpr int kStep = kKv8StreamStep;
 
 template <int BYTES>
 struct Row {
@@ -48,73 +47,9 @@ __device__ __forceinline__ Row<BYTES> load_row(const uint8_t *p) {
         return __builtin_bit_cast(Row<16>, load16(p));
 }
 
-template <bool HIGH>
-__device__ __forceinline__ unsigned widen(unsigned codes, float scale) {
-    return __builtin_bit_cast(unsigned,
-                              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, HIGH));
-}
-
 __device__ __forceinline__ cl_f4 mfma(u4 a, u4 b, cl_f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a),
                                                    __builtin_bit_cast(bf8, b), c, 0, 0, 0);
-}
-
-// Steps of a tile whose last row sees `high` tokens.
-__device__ __forceinline__ int steps_of(int high) { return (max(high, 0) + kKv8Step - 1) / kKv8Step; }
-
-// Where a workgroup's run of steps begins.
-struct Place {
-    int b, item, h, step;
-    int64_t share, total;
-};
-
-// All 256 threads: the steps before each sequence are summed up (in one order
-// everywhere), and step `share * w` is looked up in them.
-__device__ __forceinline__ Place find_place(const Kv8Args &c, int G, int tile, int grid, int w,
-                                            int64_t *s_wave, Place *s_place) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, H = c.num_heads;
-    const int per = (c.num_seqs + 255) / 256;
-    auto steps = [&](int b) {
-        int64_t sum = 0;
-        Kv8Tile t;
-        for (int item = 0; kv8_tile_of(c, G, b, item, tile, &t); ++item) sum += steps_of(t.high);
-        return sum * H;
-    };
-    int64_t mine = 0;
-    for (int b = tid * per; b < min((tid + 1) * per, c.num_seqs); ++b) mine += steps(b);
-    int64_t inc = mine;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t up = __shfl_up(inc, o, 64);
-        if (lane >= o) inc += up;
-    }
-    if (lane == 63) s_wave[wave] = inc;
-    if (tid == 0) s_place->b = -1;
-    __syncthreads();
-    const int64_t total = s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
-    int64_t at = inc - mine;
-    for (int i = 0; i < wave; ++i) at += s_wave[i];
-    const int64_t share = max((total + grid - 1) / grid, (int64_t)1);
-    const int64_t want = share * w;
-    if (want >= at && want < at + mine) {
-        for (int b = tid * per; b < min((tid + 1) * per, c.num_seqs); ++b) {
-            Kv8Tile t;
-            for (int item = 0; kv8_tile_of(c, G, b, item, tile, &t); ++item) {
-                const int n = steps_of(t.high);
-                if (want >= at && want < at + (int64_t)n * H) {
-                    s_place->b = b;
-                    s_place->item = item;
-                    s_place->h = (int)((want - at) / n);
-                    s_place->step = (int)((want - at) % n);
-                }
-                at += (int64_t)n * H;
-            }
-        }
-    }
-    __syncthreads();
-    Place p = *s_place;
-    p.share = share;
-    p.total = total;
-    return p;
 }
 
 template <int DP, int NC, int SUMS>
@@ -138,52 +73,25 @@ __global__ void __launch_bounds__(256, DP * NC > 128 ? 2 : 3)
     } sh;
     __shared__ float s_m[4][16], s_l[4][16];
     __shared__ int64_t s_wave[4];
-    __shared__ Place s_place;
+    __shared__ Kv8Place s_place;
 
     if ((int)blockIdx.x >= p.grid) {
-        // rows of no sequence, or without a token to see
-        const int r0 = ((int)blockIdx.x - p.grid) * 4 + wave;
-        if (blockIdx.x == (unsigned)p.grid && wave == 0) kv8_check(c);
-        if (r0 >= c.rows) return;
-        const int b = kv8_seq_of_row(c, r0);
-        int see = 0;
-        if (b >= 0) {
-            int first, n;
-            kv8_rows(c, b, &first, &n);
-            see = kv8_context(c, b) - n + (r0 - first) + 1;
-        }
-        if (see <= 0)
-            for (int d = lane; d < a.q_heads * D; d += 64)
-                a.out[(size_t)r0 * a.q_heads * D + d] = 0.0f;
+        kv8_zero_rows(a, blockIdx.x - p.grid);
         return;
     }
-    Place at = find_place(c, G, p.tile, p.grid, blockIdx.x, s_wave, &s_place);
+    Kv8Place at =
+        kv8_find_place(c, G, p.tile, p.step, p.grid, blockIdx.x, s_wave, &s_place);
     int64_t *starts = reinterpret_cast<int64_t *>(a.ws + p.start_at);
     if (p.join && blockIdx.x == 0 && tid == 0) starts[0] = at.share;
     int64_t left = min(at.share, at.total - at.share * blockIdx.x);
     bool front = true;
 
     while (left > 0) {
-        // the next tile with steps
         Kv8Tile T;
-        if (at.h >= H) {
-            at.h = 0;
-            ++at.item;
-        }
-        while (at.b < c.num_seqs) {
-            if (!kv8_tile_of(c, G, at.b, at.item, p.tile, &T)) {
-                ++at.b;
-                at.item = 0;
-            } else if (T.high <= 0) {
-                ++at.item;
-            } else {
-                break;
-            }
-        }
-        if (at.b >= c.num_seqs) return;  // (there are as many steps as were counted)
-        const int h = at.h, all = steps_of(T.high);
+        if (!kv8_next_tile(c, G, p.tile, &at, &T)) return;
+        const int h = at.h, all = kv8_steps(T.high, kStep);
         const int s0 = at.step, s1 = (int)min((int64_t)all, s0 + left);
-        const int t_end = min(s1 * kKv8Step, T.high);
+        const int t_end = min(s1 * kStep, T.high);
         const int64_t run0 = at.share * blockIdx.x + (min(at.share, at.total - at.share * blockIdx.x) - left);
         if (p.join && s0 == 0 && tid == 0)
             starts[1 + (size_t)(kv8_first_slot(c, at.b, p.tile, G, 1) + at.item) * H + h] = run0;
@@ -198,8 +106,8 @@ __global__ void __launch_bounds__(256, DP * NC > 128 ? 2 : 3)
                 const int tok = (T.r0 + u) / G, g = (T.r0 + u) % G;
                 const cl_f4 *qr = reinterpret_cast<const cl_f4 *>(
                     a.q + ((size_t)(T.first + tok) * a.q_heads + h * G + g) * D + d);
-                lo = qr[0] * (a.scale * 1.44269504088896341f);
-                hi = qr[1] * (a.scale * 1.44269504088896341f);
+                lo = qr[0] * (a.scale * kLog2e);
+                hi = qr[1] * (a.scale * kLog2e);
             }
             u4 w[3];
 #pragma unroll
@@ -242,13 +150,13 @@ __global__ void __launch_bounds__(256, DP * NC > 128 ? 2 : 3)
         for (int i = 0; i < KS; ++i) koff[i] = 64 * i + 16 * q < D ? 64 * i + 16 * q : 0;
         const uint8_t *vbase = c.codes + (size_t)c.num_blocks * H * bs * D + (JB * r < D ? JB * r : 0);
 
-        for (int c0 = s0 * kKv8Step; c0 < t_end; c0 += kChunk) {
+        for (int c0 = s0 * kStep; c0 < t_end; c0 += kChunk) {
             const int c1 = min(c0 + kChunk, t_end);
-            if (c0 > s0 * kKv8Step) __syncthreads();  // the chunk before is done with
+            if (c0 > s0 * kStep) __syncthreads();  // the chunk before is done with
             // tokens behind the end take the chunk's first place (and no part in
             // what follows), so that every load lies in the pool
             int bad = 0;
-            for (int i = tid; i < (c1 - c0 + kKv8Step - 1) / kKv8Step * (kKv8Step / 4); i += 256) {
+            for (int i = tid; i < (c1 - c0 + kStep - 1) / kStep * (kStep / 4); i += 256) {
                 const int t = c0 + 4 * i < c1 ? c0 + 4 * i : c0;
                 const int64_t id = kv8_block(c, at.b, t / bs, h == 0);
                 uint2 e = {0, 0};
@@ -292,8 +200,8 @@ __global__ void __launch_bounds__(256, DP * NC > 128 ? 2 : 3)
                 load_k(kb);
                 load_v(kb);
             }
-            for (; kb < c1; kb += kKv8Step) {
-                const bool more = kb + kKv8Step < c1;
+            for (; kb < c1; kb += kStep) {
+                const bool more = kb + kStep < c1;
                 cl_f4 s[NC][2];
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
@@ -305,8 +213,8 @@ __global__ void __launch_bounds__(256, DP * NC > 128 ? 2 : 3)
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const unsigned w0 = kk[u][i / 2][2 * (i & 1)], w1 = kk[u][i / 2][2 * (i & 1) + 1];
-                        kf[u] = (u4){widen<false>(w0, ks[u]), widen<true>(w0, ks[u]),
-                                     widen<false>(w1, ks[u]), widen<true>(w1, ks[u])};
+                        kf[u] = (u4){kv8_widen<false>(w0, ks[u]), kv8_widen<true>(w0, ks[u]),
+                                     kv8_widen<false>(w1, ks[u]), kv8_widen<true>(w1, ks[u])};
                     }
 #pragma unroll
                     for (int cc = 0; cc < NC; ++cc)
@@ -317,7 +225,7 @@ __global__ void __launch_bounds__(256, DP * NC > 128 ? 2 : 3)
                             for (int u = 0; u < 2; ++u) s[cc][u] = mfma(kf[u], qf, s[cc][u]);
                         }
                 }
-                if (more) load_k(kb + kKv8Step);
+                if (more) load_k(kb + kStep);
                 if (bad || kb + 32 > min(T.low, c1)) {
                     asm volatile("");  // (a branch, not selects that every step pays for)
 #pragma unroll
@@ -340,12 +248,12 @@ __global__ void __launch_bounds__(256, DP * NC > 128 ? 2 : 3)
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) top = fmaxf(top, s[cc][u][i]);
-                    if (__any(top > m[cc] + kSlack)) {
+                    if (__any(top > m[cc] + kKv8Slack)) {
                         // a row moves its maximum by its own scores alone, so that
                         // its bits do not depend on the rows beside it
                         top = fmaxf(top, __shfl_xor(top, 16, 64));
                         top = fmaxf(top, __shfl_xor(top, 32, 64));
-                        const float m_new = top > m[cc] + kSlack ? top : m[cc];
+                        const float m_new = top > m[cc] + kKv8Slack ? top : m[cc];
                         const float f0 =
                             m_new == m[cc] ? 1.0f : __builtin_amdgcn_exp2f(m[cc] - m_new);
                         l[cc] *= f0;
@@ -394,8 +302,8 @@ __global__ void __launch_bounds__(256, DP * NC > 128 ? 2 : 3)
                     for (int e = 0; e < 4; ++e) {
                         const float sc = vs[e / 2];
                         const unsigned wa = vv[2 * e].w[jb / 4], wb = vv[2 * e + 1].w[jb / 4];
-                        const unsigned xa = widen<false>(wa, sc), xb = widen<false>(wb, sc);
-                        const unsigned ya = widen<true>(wa, sc), yb = widen<true>(wb, sc);
+                        const unsigned xa = kv8_widen<false>(wa, sc), xb = kv8_widen<false>(wb, sc);
+                        const unsigned ya = kv8_widen<true>(wa, sc), yb = kv8_widen<true>(wb, sc);
                         v[0][e] = __builtin_amdgcn_perm(xb, xa, 0x05040100u);
                         v[1][e] = __builtin_amdgcn_perm(xb, xa, 0x07060302u);
                         v[2][e] = __builtin_amdgcn_perm(yb, ya, 0x05040100u);
@@ -409,7 +317,7 @@ __global__ void __launch_bounds__(256, DP * NC > 128 ? 2 : 3)
                             for (int i = 0; i < 4; ++i)
                                 o[cc][jb + i] = mfma(v[i], pf[cc][x], o[cc][jb + i]);
                 }
-                if (more) load_v(kb + kKv8Step);
+                if (more) load_v(kb + kStep);
             }
         }
 
@@ -477,75 +385,6 @@ __global__ void __launch_bounds__(256, DP * NC > 128 ? 2 : 3)
     }
 }
 
-// Joins the pieces of one row and query head, the workgroup's waves in turn, a
-// lane up to four dims.
-__global__ void __launch_bounds__(1024) join_kernel(Kv8Attention a, Kv8Split p) {
-    const Kv8Args &c = a.c;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
-    const int hq = blockIdx.x % a.q_heads, row = blockIdx.x / a.q_heads;
-    const int D = c.head_dim, H = c.num_heads, G = a.q_heads / H, h = hq / G;
-    __shared__ float s_o[16][kKv8MaxHeadDim], s_f[kMaxGrid], s_l[16], s_top[16];
-    const int b = kv8_seq_of_row(c, row);
-    if (b < 0) return;
-    int first, n;
-    kv8_rows(c, b, &first, &n);
-    const int u = (row - first) * G + hq % G;
-    Kv8Tile T;
-    if (!kv8_tile_of(c, G, b, u / p.tile, p.tile, &T) || T.high <= 0) return;
-    const int64_t *starts = reinterpret_cast<const int64_t *>(a.ws + p.start_at);
-    const int64_t share = starts[0];
-    const size_t slot = kv8_first_slot(c, b, p.tile, G, 1) + u / p.tile;
-    const int64_t start = starts[1 + slot * H + h], end = start + steps_of(T.high);
-    const int64_t w0 = start / share;
-    const int np = (int)((end - 1) / share - w0) + 1;
-    if (np == 1) return;  // written whole
-    // the first piece ends its workgroup's run unless the run begins with it
-    auto place = [&](int i) {
-        const int64_t w = w0 + i;
-        return (size_t)(2 * w + (i == 0 && start != w * share ? 1 : 0)) * p.stored + u % p.tile;
-    };
-    const float2 *ml = reinterpret_cast<const float2 *>(a.ws + p.ml_at);
-    float top = -INFINITY, x[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.0f;
-    for (int i = tid; i < np; i += blockDim.x) {
-        s_f[i] = ml[place(i)].x;
-        top = fmaxf(top, s_f[i]);
-    }
-    top = wave_max(top);
-    if (lane == 0) s_top[wave] = top;
-    __syncthreads();
-    for (int w = 0; w < waves; ++w) top = fmaxf(top, s_top[w]);
-    for (int i = tid; i < np; i += blockDim.x) {
-        const float f = s_f[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_f[i] - top);
-        l += ml[place(i)].y * f;
-        s_f[i] = f;
-    }
-    l = wave_sum(l);
-    __syncthreads();
-    const float *o = a.ws + p.o_at;
-#pragma unroll 4
-    for (int i = wave; i < np; i += waves) {
-        const float f = s_f[i], *oi = o + place(i) * D;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (lane + 64 * e < D) x[e] = fmaf(oi[lane + 64 * e], f, x[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (lane + 64 * e < D) s_o[wave][lane + 64 * e] = x[e];
-    if (lane == 0) s_l[wave] = l;
-    __syncthreads();
-    l = 0.0f;
-    for (int w = 0; w < waves; ++w) l += s_l[w];
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const size_t rh = (size_t)row * a.q_heads + hq;
-    for (int d = tid; d < D; d += blockDim.x) {
-        float sum = 0.0f;
-        for (int w = 0; w < waves; ++w) sum += s_o[w][d];
-        a.out[rh * D + d] = sum * inv;
-    }
-    if (tid == 0 && p.sums) reinterpret_cast<float2 *>(a.ws + p.row_ml_at)[rh] = make_float2(top, inv);
-}
-
 template <int DP, int NC>
 void launch(const Kv8Attention &a, const Kv8Split &p, unsigned grid, hipStream_t s) {
     switch (p.sums) {
@@ -560,7 +399,7 @@ void launch(const Kv8Attention &a, const Kv8Split &p, unsigned grid, hipStream_t
 int kv8_stream_residents(int dp, int tile) { return dp * tile > 128 * 16 ? 2 : 3; }
 
 void kv8_stream(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
-    const unsigned grid = p.grid + (a.c.rows + 3) / 4;
+    const unsigned grid = p.grid + kv8_zero_grid(a.c);
     if (p.tile == 16) {
         if (p.dp == 64) launch<64, 1>(a, p, grid, s);
         if (p.dp == 128) launch<128, 1>(a, p, grid, s);
@@ -568,11 +407,6 @@ void kv8_stream(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
     } else {
         if (p.dp == 64) launch<64, 2>(a, p, grid, s);
         if (p.dp == 128) launch<128, 2>(a, p, grid, s);
-    }
-    if (p.join) {
-        // one workgroup a row and head; many waves where few rows have many pieces
-        const unsigned n = (unsigned)a.c.rows * a.q_heads;
-        join_kernel<<<n, n <= 64 ? 1024 : n <= 1024 ? 256 : 64, 0, s>>>(a, p);
     }
 }
 

@@ -1,0 +1,534 @@
+// kv8_tile.hip -- attention of many query rows over the 8-bit paged cache:
+// prompts, chunks of prompts, and the weights of their blocks.
+//
+// A workgroup takes a tile of 64 * NR query rows of one kv head (a wave 16 * NR
+// of them) and walks the tokens they see in steps.  A step's codes are widened
+// to bf16 once for the whole tile, on their way to LDS: the keys as rows, the
+// values as columns of eight tokens; the next step's codes are on their way from
+// memory meanwhile.  The products are those of kv8_stream.hip (S^T = K Q^T with
+// q, O^T = V^T P^T with P, as three bf16 pieces each), and an operand read from
+// LDS feeds 3 * NR MFMAs.
+#include "bf16x3.h"
+#include "kv8.h"
+#include "wave.h"
+
+namespace clove {
+namespace k {
+
+namespace {
+
+constexpr int kChunk = 4096;  // tokens whose rows a workgroup's table holds
+
+__device__ __forceinline__ cl_f4 mfma(u4 a, u4 b, cl_f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a),
+                                                   __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+}
+
+// Eight dims of a query row times `scale`, in pieces.
+__device__ __forceinline__ void split_q(const float *q, bool ok, float scale, u4 (&w)[3]) {
+    cl_f4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+    if (ok) {
+        lo = reinterpret_cast<const cl_f4 *>(q)[0] * scale;
+        hi = reinterpret_cast<const cl_f4 *>(q)[1] * scale;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        unsigned w1, w2, w3;
+        split_pair<false>(e < 2 ? lo[2 * e] : hi[2 * e - 4], e < 2 ? lo[2 * e + 1] : hi[2 * e - 3],
+                          &w1, &w2, &w3);
+        w[0][e] = w1;
+        w[1][e] = w2;
+        w[2][e] = w3;
+    }
+}
+
+// The table of tokens [c0, c1), rounded up to whole steps: the row of each four
+// tokens' first and the scales of its key and value tile as bf16, 0 outside the
+// pool.  Tokens behind the end take the first place.  True: some are outside.
+__device__ __forceinline__ int fill_table(const Kv8Args &c, int b, int h, int c0, int c1,
+                                          int step, uint2 *table) {
+    int bad = 0;
+    for (int i = threadIdx.x; i < (c1 - c0 + step - 1) / step * (step / 4); i += 256) {
+        const int t = c0 + 4 * i < c1 ? c0 + 4 * i : c0;
+        const int64_t id = kv8_block(c, b, t / c.block_size, h == 0);
+        uint2 e = {0, 0};
+        if (id >= 0) {
+            e.x = (unsigned)((id * c.num_heads + h) * c.block_size + t % c.block_size);
+            e.y = __float_as_uint(kv8_scale(c.exps[kv8_tile(c, 0, id, h)])) |
+                  __float_as_uint(kv8_scale(c.exps[kv8_tile(c, 1, id, h)])) >> 16;
+        }
+        bad |= id < 0;
+        table[i] = e;
+    }
+    return bad;
+}
+
+template <int DP, int NR>
+__global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p) {
+    constexpr int KI = DP / 32;               // MFMA steps of q . k
+    constexpr int KB = DP > 128 ? 32 : 64;    // tokens of a step
+    constexpr int JB = DP / 16;               // 16-dim blocks of O^T
+    constexpr int PK = 2 * DP + 16, PV = 2 * KB + 16;  // LDS pitches: no bank conflicts
+    constexpr int NK = KB * DP / 16 / 256;    // 16-byte pieces of keys a thread stages
+    constexpr int JV = DP * KB / 4 / 256;     // dims of four tokens' values a thread stages
+    static_assert(NK >= 1 && (JV == 4 || JV == 8), "256 threads stage a step");
+    const Kv8Args &c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = lane & 15, q = lane >> 4;
+    const int H = c.num_heads, G = a.q_heads / H, D = c.head_dim, bs = c.block_size;
+    __shared__ uint2 table[kChunk / 4];
+    __shared__ __attribute__((aligned(16))) uint8_t sK[2][KB * PK], sV[2][DP * PV];
+    __shared__ int64_t s_wave[4];
+    __shared__ Kv8Place s_place;
+
+    if ((int)blockIdx.x >= p.grid) {
+        kv8_zero_rows(a, blockIdx.x - p.grid);
+        return;
+    }
+    Kv8Place at;
+    int64_t left, run = 0;
+    if (p.join) {
+        at = kv8_find_place(c, G, p.tile, p.step, p.grid, blockIdx.x, s_wave, &s_place);
+        run = min(at.share, at.total - at.share * blockIdx.x);
+        left = run;
+        if (blockIdx.x == 0 && tid == 0)
+            reinterpret_cast<int64_t *>(a.ws + p.start_at)[0] = at.share;
+    } else {
+        // a tile to a workgroup; a sequence's last tiles, the longest, first
+        at.h = blockIdx.x % H;
+        at.b = kv8_slot(c, p.grid / H - 1 - blockIdx.x / H, p.tile, G, 1, &at.item);
+        at.step = 0;
+        at.share = 0;
+        left = 1;
+    }
+    bool front = true;
+
+    while (left > 0) {
+        Kv8Tile T;
+        if (p.join) {
+            if (!kv8_next_tile(c, G, p.tile, &at, &T)) return;
+        } else if (!kv8_tile_of(c, G, at.b, at.item, p.tile, &T) || T.high <= 0) {
+            return;
+        }
+        const int h = at.h, all = kv8_steps(T.high, KB);
+        const int s0 = at.step, s1 = p.join ? (int)min((int64_t)all, s0 + left) : all;
+        const int t_end = min(s1 * KB, T.high);
+        if (p.join && s0 == 0 && tid == 0)
+            reinterpret_cast<int64_t *>(a.ws + p.start_at)
+                [1 + (size_t)(kv8_first_slot(c, at.b, p.tile, G, 1) + at.item) * H + h] =
+                    at.share * blockIdx.x + (run - left);
+
+        // this wave's rows: q in pieces, and the tokens each row sees
+        u4 qf[NR][KI][3];
+        int lim[NR];
+        size_t rowhead[NR];
+#pragma unroll
+        for (int cc = 0; cc < NR; ++cc) {
+            const int u = 16 * (NR * wave + cc) + r;
+            const bool ok = u < T.rows;
+            const int tok = (T.r0 + (ok ? u : 0)) / G, g = (T.r0 + (ok ? u : 0)) % G;
+            lim[cc] = ok ? min(t_end, T.ctx - T.n + tok + 1) : 0;
+            rowhead[cc] = (size_t)(T.first + tok) * a.q_heads + h * G + g;
+#pragma unroll
+            for (int i = 0; i < KI; ++i)
+                split_q(a.q + rowhead[cc] * D + 32 * i + 8 * q, ok && 32 * i + 8 * q < D,
+                        a.scale * kLog2e, qf[cc][i]);
+        }
+        const int u0 = 16 * NR * wave;  // tokens that all the wave's rows see, and that any does
+        const int low = u0 < T.rows ? T.ctx - T.n + (T.r0 + u0) / G + 1 : 0;
+        const int high =
+            u0 < T.rows ? min(t_end, T.ctx - T.n + (T.r0 + min(u0 + 16 * NR, T.rows) - 1) / G + 1) : 0;
+
+        float m[NR], l[NR];
+        cl_f4 o[NR][JB];
+#pragma unroll
+        for (int cc = 0; cc < NR; ++cc) {
+            m[cc] = -INFINITY;
+            l[cc] = 0.0f;
+#pragma unroll
+            for (int jb = 0; jb < JB; ++jb) o[cc][jb] = (cl_f4){0.f, 0.f, 0.f, 0.f};
+        }
+
+        // what this thread stages: NK pieces of keys, JV dims of a quad's values
+        const int vquad = tid % (KB / 4), vdim = tid / (KB / 4) * JV;
+        const uint8_t *vbase =
+            c.codes + (size_t)c.num_blocks * H * bs * D + (vdim < D ? vdim : 0);
+        // tokens 4 * (vquad % 4) + i of half (vquad / 4) % 2 of 32 tokens: the
+        // order of S^T's elements in a lane, twice four of them
+        const int vpos = vquad / 8 * 32 + vquad % 4 * 8 + vquad / 4 % 2 * 4;
+
+        for (int c0 = s0 * KB; c0 < t_end; c0 += kChunk) {
+            const int c1 = min(c0 + kChunk, t_end);
+            __syncthreads();  // the table and tiles before are done with
+            const int bad = __syncthreads_or(fill_table(c, at.b, h, c0, c1, KB, table));
+
+            u4 rk[NK];
+            unsigned rv[4][JV / 4];
+            float ksc[NK], vsc;
+            auto load = [&](int kb) {
+#pragma unroll
+                for (int i = 0; i < NK; ++i) {
+                    const int x = tid + 256 * i, key = x / (DP / 16), d = x % (DP / 16) * 16;
+                    const uint2 e = table[(kb - c0 + key) >> 2];
+                    ksc[i] = __uint_as_float(e.y & 0xffff0000u);
+                    // (past D, where q is 0, the row's first dims stand in)
+                    rk[i] = *reinterpret_cast<const u4 *>(
+                        c.codes + (size_t)(e.x + (key & 3)) * D + (d < D ? d : 0));
+                }
+                const uint2 e = table[((kb - c0) >> 2) + vquad];
+                vsc = __uint_as_float(e.y << 16);
+                const uint8_t *row = vbase + (size_t)e.x * D;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (JV == 8) {
+                        const uint2 w = *reinterpret_cast<const uint2 *>(row + i * D);
+                        rv[i][0] = w.x;
+                        rv[i][1] = w.y;
+                    } else {
+                        rv[i][0] = *reinterpret_cast<const unsigned *>(row + i * D);
+                    }
+                }
+            };
+            auto store = [&](int kb, int buf) {
+#pragma unroll
+                for (int i = 0; i < NK; ++i) {
+                    const int x = tid + 256 * i, key = x / (DP / 16), d = x % (DP / 16) * 16;
+                    u4 w[2];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        w[e / 2][2 * (e & 1)] = kv8_widen<false>(rk[i][e], ksc[i]);
+                        w[e / 2][2 * (e & 1) + 1] = kv8_widen<true>(rk[i][e], ksc[i]);
+                    }
+                    u4 *to = reinterpret_cast<u4 *>(&sK[buf][key * PK + 2 * d]);
+                    to[0] = w[0];
+                    to[1] = w[1];
+                }
+                if (bad || kb + KB > c1) {
+                    // codes that nothing wrote may be NaN: 0 * NaN would stay
+                    asm volatile("");
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (vsc == 0.0f || kb + 4 * vquad + i >= c1)
+#pragma unroll
+                            for (int e = 0; e < JV / 4; ++e) rv[i][e] = 0;
+                }
+#pragma unroll
+                for (int e = 0; e < JV / 4; ++e)
+#pragma unroll
+                    for (int hi = 0; hi < 2; ++hi) {
+                        unsigned w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            w[i] = hi ? kv8_widen<true>(rv[i][e], vsc) : kv8_widen<false>(rv[i][e], vsc);
+                        uint8_t *to = &sV[buf][(vdim + 4 * e + 2 * hi) * PV + 2 * vpos];
+                        *reinterpret_cast<uint2 *>(to) =
+                            make_uint2(__builtin_amdgcn_perm(w[1], w[0], 0x05040100u),
+                                       __builtin_amdgcn_perm(w[3], w[2], 0x05040100u));
+                        *reinterpret_cast<uint2 *>(to + PV) =
+                            make_uint2(__builtin_amdgcn_perm(w[1], w[0], 0x07060302u),
+                                       __builtin_amdgcn_perm(w[3], w[2], 0x07060302u));
+                    }
+            };
+
+            load(c0);
+            store(c0, 0);
+            __syncthreads();
+            int buf = 0;
+            for (int kb = c0; kb < c1; kb += KB, buf ^= 1) {
+                const bool more = kb + KB < c1;
+                if (more) load(kb + KB);
+#pragma unroll
+                for (int sub = 0; sub < KB / 32; ++sub) {
+                    const int t0 = kb + 32 * sub;
+                    if (t0 >= high) break;
+                    cl_f4 s[NR][2];
+#pragma unroll
+                    for (int cc = 0; cc < NR; ++cc)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) s[cc][u] = (cl_f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < KI; ++i) {
+                        u4 kf[2];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            kf[u] = *reinterpret_cast<const u4 *>(
+                                &sK[buf][(32 * sub + 16 * u + r) * PK + 64 * i + 16 * q]);
+#pragma unroll
+                        for (int x = 2; x >= 0; --x)
+#pragma unroll
+                            for (int cc = 0; cc < NR; ++cc)
+#pragma unroll
+                                for (int u = 0; u < 2; ++u)
+                                    s[cc][u] = mfma(kf[u], qf[cc][i][x], s[cc][u]);
+                    }
+                    if (bad || t0 + 32 > min(low, c1)) {
+                        asm volatile("");  // (a branch, not selects that every step pays for)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const bool in = table[((t0 - c0) >> 2) + 4 * u + q].y != 0;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                for (int cc = 0; cc < NR; ++cc)
+                                    if (!in || t0 + 16 * u + 4 * q + i >= lim[cc])
+                                        s[cc][u][i] = -INFINITY;
+                        }
+                    }
+                    u4 pf[NR][3];
+#pragma unroll
+                    for (int cc = 0; cc < NR; ++cc) {
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[cc][u][i]);
+                        if (__any(top > m[cc] + kKv8Slack)) {
+                            // a row moves its maximum by its own scores alone, so
+                            // that its bits do not depend on the rows beside it
+                            top = fmaxf(top, __shfl_xor(top, 16, 64));
+                            top = fmaxf(top, __shfl_xor(top, 32, 64));
+                            const float m_new = top > m[cc] + kKv8Slack ? top : m[cc];
+                            const float f0 =
+                                m_new == m[cc] ? 1.0f : __builtin_amdgcn_exp2f(m[cc] - m_new);
+                            l[cc] *= f0;
+#pragma unroll
+                            for (int jb = 0; jb < JB; ++jb) o[cc][jb] *= f0;
+                            m[cc] = m_new;
+                        }
+                        const float mz = m[cc] == -INFINITY ? 0.0f : m[cc];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                s[cc][u][i] = __builtin_amdgcn_exp2f(s[cc][u][i] - mz);
+                            l[cc] += hsum4(s[cc][u]);
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                unsigned w1, w2, w3;
+                                split_pair<false>(s[cc][u][2 * e], s[cc][u][2 * e + 1], &w1, &w2,
+                                                  &w3);
+                                pf[cc][0][2 * u + e] = w1;
+                                pf[cc][1][2 * u + e] = w2;
+                                pf[cc][2][2 * u + e] = w3;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int jb = 0; jb < JB; jb += 4) {
+                        u4 v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            v[i] = *reinterpret_cast<const u4 *>(
+                                &sV[buf][(16 * (jb + i) + r) * PV + 64 * sub + 16 * q]);
+#pragma unroll
+                        for (int x = 2; x >= 0; --x)
+#pragma unroll
+                            for (int cc = 0; cc < NR; ++cc)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    o[cc][jb + i] = mfma(v[i], pf[cc][x], o[cc][jb + i]);
+                    }
+                }
+                if (more) store(kb + KB, buf ^ 1);
+                __syncthreads();
+            }
+        }
+
+        const bool whole = s0 == 0 && s1 == all;
+        const size_t piece = (size_t)(2 * blockIdx.x + (front ? 0 : 1)) * p.stored;
+#pragma unroll
+        for (int cc = 0; cc < NR; ++cc) {
+            float ls = l[cc];
+            ls += __shfl_xor(ls, 16, 64);
+            ls += __shfl_xor(ls, 32, 64);
+            const int u = 16 * (NR * wave + cc) + r;
+            if (u >= T.rows) continue;
+            const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+            float *to = whole ? a.out + rowhead[cc] * D : a.ws + p.o_at + (piece + u) * D;
+            const float f = whole ? inv : 1.0f;
+#pragma unroll
+            for (int jb = 0; jb < JB; ++jb)
+                if (DP == 64 ? 16 * jb < D : 16 * jb + 4 * q < D)
+                    *reinterpret_cast<cl_f4 *>(to + 16 * jb + 4 * q) = o[cc][jb] * f;
+            if (q == 0) {
+                if (!whole)
+                    reinterpret_cast<float2 *>(a.ws + p.ml_at)[piece + u] = make_float2(m[cc], ls);
+                else if (a.w_out)
+                    reinterpret_cast<float2 *>(a.ws + p.row_ml_at)[rowhead[cc]] =
+                        make_float2(m[cc], inv);
+            }
+        }
+        left -= p.join ? s1 - s0 : 1;
+        front = false;
+        at.step = 0;
+        ++at.h;
+    }
+}
+
+// The attention weight of every four tokens, summed over the rows and the heads
+// of a group: a workgroup takes 256 tokens of one kv head, a wave 64 of them as
+// MFMA operands in registers, and walks the rows that see them, 32 at a time, in
+// pieces through LDS.  A row's weights are 2^(s - m) / sum.
+template <int DP>
+__global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
+    tile_weights_kernel(Kv8Attention a, Kv8Split p) {
+    constexpr int KI = DP / 32;
+    const Kv8Args &c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = lane & 15, q = lane >> 4;
+    const int H = c.num_heads, G = a.q_heads / H, D = c.head_dim;
+    const int h = blockIdx.y, b = blockIdx.z, c0 = blockIdx.x * 256;
+    __shared__ uint2 table[64];
+    __shared__ u4 sq[2 * KI * 3 * 64];
+    __shared__ float2 s_ml[32];
+    __shared__ int s_lim[32];
+    int first, n;
+    kv8_rows(c, b, &first, &n);
+    const int ctx = kv8_context(c, b), c1 = min(c0 + 256, ctx);
+    if (c0 >= c1) return;
+    const int bad = __syncthreads_or(fill_table(c, b, 0, c0, c1, 256, table) | 0);
+    (void)bad;
+    // the keys: token 16u + r of the wave's, dims 32i + 8q .. + 7
+    u4 kf[4][KI];
+    bool in[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int t = 64 * wave + 16 * u + r;
+        const uint2 e0 = table[t >> 2];
+        // (the table is head 0's)
+        const uint8_t *row =
+            c.codes + ((size_t)e0.x + (size_t)h * c.block_size + (t & 3)) * D;
+        const int tt = c0 + t < c1 ? c0 + t : c0;
+        const int64_t id = kv8_block(c, b, tt / c.block_size, false);
+        const float sc = id >= 0 ? kv8_scale(c.exps[kv8_tile(c, 0, id, h)]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < KI; ++i) {
+            const int d = 32 * i + 8 * q;
+            const uint2 w = *reinterpret_cast<const uint2 *>((id >= 0 ? row : c.codes) + (d < D ? d : 0));
+            kf[u][i] = (u4){kv8_widen<false>(w.x, sc), kv8_widen<true>(w.x, sc),
+                            kv8_widen<false>(w.y, sc), kv8_widen<true>(w.y, sc)};
+        }
+        in[u] = table[(64 * wave + 16 * u + 4 * q) >> 2].y != 0;
+    }
+    cl_f4 sum[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) sum[u] = (cl_f4){0.f, 0.f, 0.f, 0.f};
+    // the first row that sees the tokens' first
+    const int i0 = max(c0 - (ctx - n), 0);
+    for (int u0 = i0 * G; u0 < n * G; u0 += 32) {
+        __syncthreads();
+        for (int x = tid; x < 2 * KI * 64; x += 256) {
+            const int lr = x & 15, lq = x >> 4 & 3, i = (x >> 6) % KI, cc = x / (64 * KI);
+            const int u = u0 + 16 * cc + lr, d = 32 * i + 8 * lq;
+            const bool ok = u < n * G && d < D;
+            const int tok = ok ? u / G : 0, g = ok ? u % G : 0;
+            u4 w[3];
+            split_q(a.q + ((size_t)(first + tok) * a.q_heads + h * G + g) * D + d, ok,
+                    a.scale * kLog2e, w);
+#pragma unroll
+            for (int y = 0; y < 3; ++y) sq[((cc * KI + i) * 3 + y) * 64 + (x & 63)] = w[y];
+        }
+        if (tid < 32) {
+            const int u = u0 + tid;
+            const bool ok = u < n * G;
+            s_lim[tid] = ok ? min(c1, ctx - n + u / G + 1) : 0;
+            s_ml[tid] = make_float2(0.f, 0.f);
+            if (ok && s_lim[tid] > 0)
+                s_ml[tid] = reinterpret_cast<const float2 *>(
+                    a.ws + p.row_ml_at)[(size_t)(first + u / G) * a.q_heads + h * G + u % G];
+        }
+        __syncthreads();
+        cl_f4 s[2][4];
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s[cc][u] = (cl_f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < KI; ++i)
+#pragma unroll
+            for (int x = 2; x >= 0; --x)
+#pragma unroll
+                for (int cc = 0; cc < 2; ++cc) {
+                    const u4 qf = sq[((cc * KI + i) * 3 + x) * 64 + lane];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) s[cc][u] = mfma(kf[u][i], qf, s[cc][u]);
+                }
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+            const float2 ml = s_ml[16 * cc + r];
+            const float mz = ml.x == -INFINITY ? 0.0f : ml.x;
+            const int lim = s_lim[16 * cc + r];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int t = c0 + 64 * wave + 16 * u + 4 * q + i;
+                    const float w = __builtin_amdgcn_exp2f(s[cc][u][i] - mz) * ml.y;
+                    sum[u][i] += in[u] && t < lim ? w : 0.0f;
+                }
+        }
+    }
+    float *out = a.ws + p.sums_at + ((size_t)b * H + h) * p.groups;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        float x = hsum4(sum[u]);
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) x += __shfl_xor(x, o, 64);
+        const int t = c0 + 64 * wave + 16 * u + 4 * q;
+        if (r == 0 && t < c1) out[t >> 2] = x;
+    }
+}
+
+// The quads' sums of all heads into the blocks' weights; lanes take 64 blocks,
+// the four waves the heads in turn.
+__global__ void __launch_bounds__(256) block_weights_kernel(Kv8Attention a, Kv8Split p) {
+    const Kv8Args &c = a.c;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int j = blockIdx.x * 64 + lane, b = blockIdx.y, per = c.block_size / 4;
+    __shared__ float part[4][64];
+    const int ctx = kv8_context(c, b);
+    int first, n;
+    kv8_rows(c, b, &first, &n);
+    float w = 0.0f;
+    if (n > 0 && j < c.max_blocks && j * c.block_size < ctx) {
+        const int quads = min(per, (ctx - j * c.block_size + 3) / 4);
+        for (int h = wave; h < c.num_heads; h += 4) {
+            const float *x = a.ws + p.sums_at + ((size_t)b * c.num_heads + h) * p.groups + (size_t)j * per;
+            for (int i = 0; i < quads; ++i) w += x[i];
+        }
+    }
+    part[wave][lane] = w;
+    __syncthreads();
+    if (wave == 0 && j < c.max_blocks) {
+        const size_t at = (size_t)b * c.max_blocks + j;
+        a.w_out[at] = a.w_in[at] + ((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]));
+    }
+}
+
+}  // namespace
+
+void kv8_tiles(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
+    const unsigned grid = p.grid + kv8_zero_grid(a.c);
+    if (p.dp == 256)
+        tile_kernel<256, 1><<<grid, 256, 0, s>>>(a, p);
+    else if (p.dp == 128 && p.tile == 128)
+        tile_kernel<128, 2><<<grid, 256, 0, s>>>(a, p);
+    else if (p.dp == 128)
+        tile_kernel<128, 1><<<grid, 256, 0, s>>>(a, p);
+    else if (p.tile == 128)
+        tile_kernel<64, 2><<<grid, 256, 0, s>>>(a, p);
+    else
+        tile_kernel<64, 1><<<grid, 256, 0, s>>>(a, p);
+}
+
+void kv8_tile_weights(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
+    const Kv8Args &c = a.c;
+    const dim3 grid((c.max_blocks * c.block_size + 255) / 256, c.num_heads, c.num_seqs);
+    if (p.dp == 64) tile_weights_kernel<64><<<grid, 256, 0, s>>>(a, p);
+    if (p.dp == 128) tile_weights_kernel<128><<<grid, 256, 0, s>>>(a, p);
+    if (p.dp == 256) tile_weights_kernel<256><<<grid, 256, 0, s>>>(a, p);
+    block_weights_kernel<<<dim3((c.max_blocks + 63) / 64, c.num_seqs), 256, 0, s>>>(a, p);
+}
+
+}  // namespace k
+}  // namespace clove
