@@ -48,12 +48,27 @@ __device__ __forceinline__ void kv8_check(const Kv8Args &a) {
     if (bad) atomicOr(a.err_flag, bad);
 }
 
+// How many of n ascending things come first for which f is true; the lanes of a
+// wave look at 64 of them at a time (one round trip to memory for most batches,
+// where a binary search takes one for each halving).
+template <class F>
+__device__ __forceinline__ int kv8_count(int n, F f) {
+    const int lane = threadIdx.x & 63;
+    int count = 0;
+    for (int b = 0; b < n; b += 64) {
+        const int hits = __popcll(__ballot(b + lane < n && f(b + lane)));
+        count += hits;
+        if (hits < 64) break;
+    }
+    return count;
+}
+
 // Work items of `per` units, `mul` units a row (`extra` more items than
 // floor(units / per) at most).  Sequence b's items get the slots from
 // floor(mul * row_starts[b] / per) + extra * b on: never more than the next
 // sequence's first slot, so kv8_slots() slots serve any split of the rows
-// without the host knowing it.  Returns the sequence a slot belongs to and the
-// item's number within it.
+// without the host knowing it.  Returns the sequence that a slot (one for the
+// wave) belongs to and the item's number within it.
 __host__ __device__ __forceinline__ int64_t kv8_slots(const Kv8Args &a, int per, int mul,
                                                       int extra) {
     if (!a.row_starts) return (int64_t)a.num_seqs * ((mul + per - 1) / per);
@@ -66,34 +81,21 @@ __device__ __forceinline__ int kv8_slot(const Kv8Args &a, int slot, int per, int
         *item = slot % each;
         return slot / each;
     }
-    auto base = [&](int b) {
-        const int64_t s = min(max(a.row_starts[b], 0), a.rows);
-        return (int)(s * mul / per) + extra * b;
-    };
-    int lo = 0, hi = a.num_seqs;  // the last b with base(b) <= slot
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (base(mid) <= slot)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    *item = slot - base(lo);
+    // the last b whose first slot is not behind this one
+    const int lo = max(kv8_count(a.num_seqs, [&](int b) {
+                           const int64_t s = min(max(a.row_starts[b], 0), a.rows);
+                           return (int)(s * mul / per) + extra * b <= slot;
+                       }) - 1, 0);
+    const int64_t s = min(max(a.row_starts[lo], 0), a.rows);
+    *item = slot - ((int)(s * mul / per) + extra * lo);
     return lo;
 }
 
-// The sequence that row r belongs to, or -1.
+// The sequence that row r (one for the wave) belongs to, or -1.
 __device__ __forceinline__ int kv8_seq_of_row(const Kv8Args &a, int r) {
     if (a.num_seqs == 0) return -1;
     if (!a.row_starts) return r;
-    int lo = 0, hi = a.num_seqs;  // the last b with row_starts[b] <= r
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.row_starts[mid] <= r)
-            lo = mid;
-        else
-            hi = mid;
-    }
+    const int lo = max(kv8_count(a.num_seqs, [&](int b) { return a.row_starts[b] <= r; }) - 1, 0);
     int first, n;
     kv8_rows(a, lo, &first, &n);
     return r >= first && r < first + n ? lo : -1;
@@ -327,6 +329,7 @@ void kv8_stream(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
 void kv8_tiles(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
 // The weights of the blocks, the scores computed again (kv8_tiles has left every
 // row's maximum and sum).
+constexpr int kKv8WeightPart = 512;
 void kv8_tile_weights(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
 
 }  // namespace k

@@ -114,74 +114,87 @@ __global__ void __launch_bounds__(256) kv8_weights_any_kernel(Kv8Attention a, co
     if (threadIdx.x == 0) a.w_out[at] = a.w_in[at] + part[0];
 }
 
-// Joins the pieces of one row and query head, the workgroup's waves in turn, a
-// lane up to four dims.
-__global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split p) {
+// Joins the pieces of the tiles that were cut.  A workgroup takes `rows` rows of
+// a tile; rows = 1: its waves take the pieces in turn, else each wave takes
+// whole rows.  A lane holds up to four dims.
+__global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split p, int rows) {
     const Kv8Args &c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
-    const int hq = blockIdx.x % a.q_heads, row = blockIdx.x / a.q_heads;
-    const int D = c.head_dim, H = c.num_heads, G = a.q_heads / H, h = hq / G;
-    __shared__ float s_o[16][kKv8MaxHeadDim], s_f[kKv8MaxGrid], s_l[16], s_top[16];
-    const int b = kv8_seq_of_row(c, row);
-    if (b < 0) return;
-    int first, n;
-    kv8_rows(c, b, &first, &n);
-    const int u = (row - first) * G + hq % G;
+    const int D = c.head_dim, H = c.num_heads, G = a.q_heads / H;
+    const int groups = (p.stored + rows - 1) / rows;
+    const int h = blockIdx.x % H, slot = blockIdx.x / H / groups;
+    const int u0 = (int)(blockIdx.x / H % groups) * rows;
+    __shared__ float s_o[16][kKv8MaxHeadDim], s_l[16], s_top[16];
+    int item;
+    const int b = kv8_slot(c, slot, p.tile, G, 1, &item);
     Kv8Tile T;
-    if (!kv8_tile_of(c, G, b, u / p.tile, p.tile, &T) || T.high <= 0) return;
+    if (!kv8_tile_of(c, G, b, item, p.tile, &T) || T.high <= 0 || u0 >= T.rows) return;
     const int64_t *starts = reinterpret_cast<const int64_t *>(a.ws + p.start_at);
     const int64_t share = starts[0];
-    const size_t slot = kv8_first_slot(c, b, p.tile, G, 1) + u / p.tile;
-    const int64_t start = starts[1 + slot * H + h], end = start + kv8_steps(T.high, p.step);
-    const int64_t w0 = start / share;
+    const int64_t start = starts[1 + (size_t)slot * H + h];
+    const int64_t end = start + kv8_steps(T.high, p.step), w0 = start / share;
     const int np = (int)((end - 1) / share - w0) + 1;
     if (np == 1) return;  // written whole
     // the first piece ends its workgroup's run unless the run begins with it
-    auto place = [&](int i) {
-        const int64_t w = w0 + i;
-        return (size_t)(2 * w + (i == 0 && start != w * share ? 1 : 0)) * p.stored + u % p.tile;
-    };
+    const size_t first = (size_t)(2 * w0 + (start != w0 * share ? 1 : 0)) * p.stored;
+    auto place = [&](int i) { return i == 0 ? first : (size_t)(2 * (w0 + i)) * p.stored; };
     const float2 *ml = reinterpret_cast<const float2 *>(a.ws + p.ml_at);
-    float top = -INFINITY, x[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.0f;
-    for (int i = tid; i < np; i += blockDim.x) {
-        s_f[i] = ml[place(i)].x;
-        top = fmaxf(top, s_f[i]);
-    }
-    top = wave_max(top);
-    if (lane == 0) s_top[wave] = top;
-    __syncthreads();
-    for (int w = 0; w < waves; ++w) top = fmaxf(top, s_top[w]);
-    for (int i = tid; i < np; i += blockDim.x) {
-        const float f = s_f[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_f[i] - top);
-        l += ml[place(i)].y * f;
-        s_f[i] = f;
-    }
-    l = wave_sum(l);
-    __syncthreads();
     const float *o = a.ws + p.o_at;
+    const bool alone = rows == 1;  // one row for all waves
+    for (int u = alone ? u0 : u0 + wave; u < min(u0 + rows, T.rows); u += alone ? 1 : waves) {
+        float top = -INFINITY, l = 0.0f, x[4] = {0.f, 0.f, 0.f, 0.f};
+        // pieces wave, wave + waves, ... of a row all waves share, else all of them
+        const int p0 = alone ? wave : 0, dp = alone ? waves : 1;
+        for (int i = p0 + lane * dp; i < np; i += 64 * dp) top = fmaxf(top, ml[place(i) + u].x);
+        top = wave_max(top);
+        if (alone) {
+            if (lane == 0) s_top[wave] = top;
+            __syncthreads();
+            for (int w = 0; w < waves; ++w) top = fmaxf(top, s_top[w]);
+        }
+        for (int i0 = p0; i0 < np; i0 += 64 * dp) {
+            const int i = i0 + lane * dp;
+            float f = 0.0f;
+            if (i < np) {
+                const float2 v = ml[place(i) + u];
+                f = v.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v.x - top);
+                l += v.y * f;
+            }
+            const int k = min(64, (np - i0 + dp - 1) / dp);
 #pragma unroll 4
-    for (int i = wave; i < np; i += waves) {
-        const float f = s_f[i], *oi = o + place(i) * D;
+            for (int j = 0; j < k; ++j) {
+                const float fj = __shfl(f, j, 64);
+                const float *oj = o + (place(i0 + j * dp) + u) * D;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (lane + 64 * e < D) x[e] = fmaf(oj[lane + 64 * e], fj, x[e]);
+            }
+        }
+        l = wave_sum(l);
+        if (alone) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (lane + 64 * e < D) s_o[wave][lane + 64 * e] = x[e];
+            if (lane == 0) s_l[wave] = l;
+            __syncthreads();
+            if (wave) return;
+            l = 0.0f;
+            for (int w = 0; w < waves; ++w) l += s_l[w];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] = 0.0f;
+                if (lane + 64 * e < D)
+                    for (int w = 0; w < waves; ++w) x[e] += s_o[w][lane + 64 * e];
+            }
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const size_t rh = (size_t)(T.first + (T.r0 + u) / G) * a.q_heads + h * G + (T.r0 + u) % G;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (lane + 64 * e < D) x[e] = fmaf(oi[lane + 64 * e], f, x[e]);
+            if (lane + 64 * e < D) a.out[rh * D + lane + 64 * e] = x[e] * inv;
+        if (lane == 0 && a.w_out)
+            reinterpret_cast<float2 *>(a.ws + p.row_ml_at)[rh] = make_float2(top, inv);
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (lane + 64 * e < D) s_o[wave][lane + 64 * e] = x[e];
-    if (lane == 0) s_l[wave] = l;
-    __syncthreads();
-    l = 0.0f;
-    for (int w = 0; w < waves; ++w) l += s_l[w];
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const size_t rh = (size_t)row * a.q_heads + hq;
-    for (int d = tid; d < D; d += blockDim.x) {
-        float sum = 0.0f;
-        for (int w = 0; w < waves; ++w) sum += s_o[w][d];
-        a.out[rh * D + d] = sum * inv;
-    }
-    if (tid == 0 && a.w_out)
-        reinterpret_cast<float2 *>(a.ws + p.row_ml_at)[rh] = make_float2(top, inv);
 }
 
 // The weight of each block from the sums stored on the way: lanes take 64
@@ -234,10 +247,12 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
                       c.num_blocks > 0 && c.max_blocks > 0 && rh < (1 << 24) &&
                       c.num_blocks * c.num_heads * bs < (1ll << 32) &&
                       ((reinterpret_cast<uintptr_t>(c.codes) | reinterpret_cast<uintptr_t>(a.q)) & 15) == 0;
-    if (!fast) {
+    auto plain = [&] {
+        p = Kv8Split{};
         if (a.w_out) p.row_ml_at = take(2 * rh);
         return p;
-    }
+    };
+    if (!fast) return plain();
     p.dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
     // rows of one sequence and kv head, on the average
     const int64_t units = ((int64_t)c.rows * G + c.num_seqs - 1) / c.num_seqs;
@@ -256,6 +271,7 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
     }
     p.stored = !c.row_starts && G < p.tile ? G : p.tile;
     const int64_t tiles = kv8_slots(c, p.tile, G, 1) * c.num_heads;
+    if (tiles >= (1 << 20) || kv8_slots(c, kKv8WeightPart, G, 1) > 65535) return plain();
     const int64_t steps = (cap + p.step - 1) / p.step;
     const int64_t room = std::min(kKv8MaxGrid, cus * residents);
     p.join = steps > 1 && (p.kind == KV8_STREAM || tiles < 2 * room);
@@ -273,7 +289,7 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
             p.sums_at = take(2 * rh * p.groups);
         } else {
             p.groups = (int)((cap + 3) / 4);
-            p.sums_at = take((int64_t)c.num_seqs * c.num_heads * p.groups);
+            p.sums_at = take(kv8_slots(c, kKv8WeightPart, G, 1) * c.num_heads * p.groups);
         }
     }
     return p;
@@ -301,9 +317,13 @@ void kv8_attention(const Kv8Attention &a, int cus, hipStream_t s) {
     else
         kv8_tiles(a, p, s);
     if (p.join) {
-        // one workgroup a row and head; many waves where few rows have many pieces
-        const unsigned n = (unsigned)c.rows * a.q_heads;
-        kv8_join_kernel<<<n, n <= 64 ? 1024 : n <= 1024 ? 256 : 64, 0, s>>>(a, p);
+        // few rows: a workgroup each, with more waves the more pieces there are
+        // to a tile; many: four to a wave
+        const unsigned tiles = (unsigned)kv8_slots(c, p.tile, a.q_heads / c.num_heads, 1) * c.num_heads;
+        const bool few = p.kind == KV8_STREAM && (int64_t)tiles * p.stored <= 4096;
+        const int rows = few ? 1 : 16, pieces = p.grid / (int)tiles + 1;
+        const int threads = !few ? 256 : pieces <= 4 ? 64 : pieces <= 16 ? 256 : 1024;
+        kv8_join_kernel<<<tiles * ((p.stored + rows - 1) / rows), threads, 0, s>>>(a, p, rows);
     }
     if (weights && p.kind == KV8_TILE)
         kv8_tile_weights(a, p, s);

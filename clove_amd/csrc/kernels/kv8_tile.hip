@@ -25,12 +25,8 @@ __device__ __forceinline__ cl_f4 mfma(u4 a, u4 b, cl_f4 c) {
 }
 
 // Eight dims of a query row times `scale`, in pieces.
-__device__ __forceinline__ void split_q(const float *q, bool ok, float scale, u4 (&w)[3]) {
-    cl_f4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
-    if (ok) {
-        lo = reinterpret_cast<const cl_f4 *>(q)[0] * scale;
-        hi = reinterpret_cast<const cl_f4 *>(q)[1] * scale;
-    }
+__device__ __forceinline__ void split_q(const cl_f4 (&x)[2], float scale, u4 (&w)[3]) {
+    const cl_f4 lo = x[0] * scale, hi = x[1] * scale;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         unsigned w1, w2, w3;
@@ -130,9 +126,15 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
             lim[cc] = ok ? min(t_end, T.ctx - T.n + tok + 1) : 0;
             rowhead[cc] = (size_t)(T.first + tok) * a.q_heads + h * G + g;
 #pragma unroll
-            for (int i = 0; i < KI; ++i)
-                split_q(a.q + rowhead[cc] * D + 32 * i + 8 * q, ok && 32 * i + 8 * q < D,
-                        a.scale * kLog2e, qf[cc][i]);
+            for (int i = 0; i < KI; ++i) {
+                const int d = 32 * i + 8 * q;
+                cl_f4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+                if (ok && d < D) {
+                    x[0] = reinterpret_cast<const cl_f4 *>(a.q + rowhead[cc] * D + d)[0];
+                    x[1] = reinterpret_cast<const cl_f4 *>(a.q + rowhead[cc] * D + d)[1];
+                }
+                split_q(x, a.scale * kLog2e, qf[cc][i]);
+            }
         }
         const int u0 = 16 * NR * wave;  // tokens that all the wave's rows see, and that any does
         const int low = u0 < T.rows ? T.ctx - T.n + (T.r0 + u0) / G + 1 : 0;
@@ -368,7 +370,10 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
 // The attention weight of every four tokens, summed over the rows and the heads
 // of a group: a workgroup takes 256 tokens of one kv head, a wave 64 of them as
 // MFMA operands in registers, and walks the rows that see them, 32 at a time, in
-// pieces through LDS.  A row's weights are 2^(s - m) / sum.
+// pieces through LDS (the next 32 on their way meanwhile).  A row's weights are
+// 2^(s - m) / sum.  Long runs of rows are cut into parts of kPart pairs, each with
+// sums of its own.
+constexpr int kPart = kKv8WeightPart;
 template <int DP>
 __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
     tile_weights_kernel(Kv8Attention a, Kv8Split p) {
@@ -377,17 +382,20 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r = lane & 15, q = lane >> 4;
     const int H = c.num_heads, G = a.q_heads / H, D = c.head_dim;
-    const int h = blockIdx.y, b = blockIdx.z, c0 = blockIdx.x * 256;
+    const int h = blockIdx.y, slot = blockIdx.z, c0 = blockIdx.x * 256;
+    constexpr int NQ = (2 * KI * 64 + 255) / 256;  // eight dims of a row each
     __shared__ uint2 table[64];
-    __shared__ u4 sq[2 * KI * 3 * 64];
-    __shared__ float2 s_ml[32];
-    __shared__ int s_lim[32];
+    __shared__ u4 sq[2][2 * KI * 3 * 64];
+    __shared__ float2 s_ml[2][32];
+    __shared__ int s_lim[2][32];
+    int part;
+    const int b = kv8_slot(c, slot, kPart, G, 1, &part);
     int first, n;
     kv8_rows(c, b, &first, &n);
     const int ctx = kv8_context(c, b), c1 = min(c0 + 256, ctx);
-    if (c0 >= c1) return;
-    const int bad = __syncthreads_or(fill_table(c, b, 0, c0, c1, 256, table) | 0);
-    (void)bad;
+    if (part < 0 || part * kPart >= n * G || c0 >= c1) return;
+    fill_table(c, b, 0, c0, c1, 256, table);
+    __syncthreads();
     // the keys: token 16u + r of the wave's, dims 32i + 8q .. + 7
     u4 kf[4][KI];
     bool in[4];
@@ -413,31 +421,55 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
     cl_f4 sum[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) sum[u] = (cl_f4){0.f, 0.f, 0.f, 0.f};
-    // the first row that sees the tokens' first
-    const int i0 = max(c0 - (ctx - n), 0);
-    for (int u0 = i0 * G; u0 < n * G; u0 += 32) {
-        __syncthreads();
-        for (int x = tid; x < 2 * KI * 64; x += 256) {
+    // from the first row that sees the tokens' first
+    const int u_end = min((part + 1) * kPart, n * G);
+    int u0 = max(part * kPart, max(c0 - (ctx - n), 0) * G);
+    cl_f4 raw[NQ][2];
+    float2 ml_next;
+    int lim_next;
+    auto load = [&](int u0) {
+#pragma unroll
+        for (int y = 0; y < NQ; ++y) {
+            const int x = tid + 256 * y;
             const int lr = x & 15, lq = x >> 4 & 3, i = (x >> 6) % KI, cc = x / (64 * KI);
             const int u = u0 + 16 * cc + lr, d = 32 * i + 8 * lq;
-            const bool ok = u < n * G && d < D;
-            const int tok = ok ? u / G : 0, g = ok ? u % G : 0;
-            u4 w[3];
-            split_q(a.q + ((size_t)(first + tok) * a.q_heads + h * G + g) * D + d, ok,
-                    a.scale * kLog2e, w);
+            raw[y][0] = raw[y][1] = (cl_f4){0.f, 0.f, 0.f, 0.f};
+            if (x < 2 * KI * 64 && u < u_end && d < D) {
+                const cl_f4 *qr = reinterpret_cast<const cl_f4 *>(
+                    a.q + ((size_t)(first + u / G) * a.q_heads + h * G + u % G) * D + d);
+                raw[y][0] = qr[0];
+                raw[y][1] = qr[1];
+            }
+        }
+        const int u = u0 + tid;
+        lim_next = tid < 32 && u < u_end ? min(c1, ctx - n + u / G + 1) : 0;
+        ml_next = make_float2(0.f, 0.f);
+        if (lim_next > 0)
+            ml_next = reinterpret_cast<const float2 *>(
+                a.ws + p.row_ml_at)[(size_t)(first + u / G) * a.q_heads + h * G + u % G];
+    };
+    auto store = [&](int buf) {
 #pragma unroll
-            for (int y = 0; y < 3; ++y) sq[((cc * KI + i) * 3 + y) * 64 + (x & 63)] = w[y];
+        for (int y = 0; y < NQ; ++y) {
+            const int x = tid + 256 * y;
+            if (x >= 2 * KI * 64) continue;
+            u4 w[3];
+            split_q(raw[y], a.scale * kLog2e, w);
+#pragma unroll
+            for (int z = 0; z < 3; ++z) sq[buf][((x >> 6) * 3 + z) * 64 + (x & 63)] = w[z];
         }
         if (tid < 32) {
-            const int u = u0 + tid;
-            const bool ok = u < n * G;
-            s_lim[tid] = ok ? min(c1, ctx - n + u / G + 1) : 0;
-            s_ml[tid] = make_float2(0.f, 0.f);
-            if (ok && s_lim[tid] > 0)
-                s_ml[tid] = reinterpret_cast<const float2 *>(
-                    a.ws + p.row_ml_at)[(size_t)(first + u / G) * a.q_heads + h * G + u % G];
+            s_lim[buf][tid] = lim_next;
+            s_ml[buf][tid] = ml_next;
         }
-        __syncthreads();
+    };
+    if (u0 < u_end) {
+        load(u0);
+        store(0);
+    }
+    __syncthreads();
+    for (int buf = 0; u0 < u_end; u0 += 32, buf ^= 1) {
+        if (u0 + 32 < u_end) load(u0 + 32);
         cl_f4 s[2][4];
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc)
@@ -449,15 +481,15 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
             for (int x = 2; x >= 0; --x)
 #pragma unroll
                 for (int cc = 0; cc < 2; ++cc) {
-                    const u4 qf = sq[((cc * KI + i) * 3 + x) * 64 + lane];
+                    const u4 qf = sq[buf][((cc * KI + i) * 3 + x) * 64 + lane];
 #pragma unroll
                     for (int u = 0; u < 4; ++u) s[cc][u] = mfma(kf[u][i], qf, s[cc][u]);
                 }
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
-            const float2 ml = s_ml[16 * cc + r];
+            const float2 ml = s_ml[buf][16 * cc + r];
             const float mz = ml.x == -INFINITY ? 0.0f : ml.x;
-            const int lim = s_lim[16 * cc + r];
+            const int lim = s_lim[buf][16 * cc + r];
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -467,8 +499,10 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
                     sum[u][i] += in[u] && t < lim ? w : 0.0f;
                 }
         }
+        if (u0 + 32 < u_end) store(buf ^ 1);
+        __syncthreads();
     }
-    float *out = a.ws + p.sums_at + ((size_t)b * H + h) * p.groups;
+    float *out = a.ws + p.sums_at + ((size_t)slot * H + h) * p.groups;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
         float x = hsum4(sum[u]);
@@ -479,8 +513,8 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
     }
 }
 
-// The quads' sums of all heads into the blocks' weights; lanes take 64 blocks,
-// the four waves the heads in turn.
+// The quads' sums of all parts and heads into the blocks' weights; lanes take 64
+// blocks, the four waves the parts and heads in turn.
 __global__ void __launch_bounds__(256) block_weights_kernel(Kv8Attention a, Kv8Split p) {
     const Kv8Args &c = a.c;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -491,10 +525,12 @@ __global__ void __launch_bounds__(256) block_weights_kernel(Kv8Attention a, Kv8S
     kv8_rows(c, b, &first, &n);
     float w = 0.0f;
     if (n > 0 && j < c.max_blocks && j * c.block_size < ctx) {
-        const int quads = min(per, (ctx - j * c.block_size + 3) / 4);
-        for (int h = wave; h < c.num_heads; h += 4) {
-            const float *x = a.ws + p.sums_at + ((size_t)b * c.num_heads + h) * p.groups + (size_t)j * per;
-            for (int i = 0; i < quads; ++i) w += x[i];
+        const int G = a.q_heads / c.num_heads, quads = min(per, (ctx - j * c.block_size + 3) / 4);
+        const int parts = (n * G + kPart - 1) / kPart;
+        const size_t slot = kv8_first_slot(c, b, kPart, G, 1);
+        for (int x = wave; x < parts * c.num_heads; x += 4) {
+            const float *y = a.ws + p.sums_at + (slot * c.num_heads + x) * p.groups + (size_t)j * per;
+            for (int i = 0; i < quads; ++i) w += y[i];
         }
     }
     part[wave][lane] = w;
@@ -523,7 +559,8 @@ void kv8_tiles(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
 
 void kv8_tile_weights(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
     const Kv8Args &c = a.c;
-    const dim3 grid((c.max_blocks * c.block_size + 255) / 256, c.num_heads, c.num_seqs);
+    const dim3 grid((c.max_blocks * c.block_size + 255) / 256, c.num_heads,
+                    (unsigned)kv8_slots(c, kPart, a.q_heads / c.num_heads, 1));
     if (p.dp == 64) tile_weights_kernel<64><<<grid, 256, 0, s>>>(a, p);
     if (p.dp == 128) tile_weights_kernel<128><<<grid, 256, 0, s>>>(a, p);
     if (p.dp == 256) tile_weights_kernel<256><<<grid, 256, 0, s>>>(a, p);
