@@ -179,7 +179,7 @@ struct Kv8Split {
     // in the workspace, in floats
     size_t o_at, ml_at;      // piece 2w (+ 1: at the end of the run) of workgroup w:
                              // `stored` sums over V [D], and (maximum, sum) pairs
-    size_t start_at;         // [slot, head] first step of the tile (int64), then share
+    size_t start_at;         // share, then [slot, head] first step of the tile
     size_t row_ml_at;        // (maximum, 1 / sum) of every row and query head
     size_t sums_at;          // [row, query head][groups] (sum, maximum) pairs
     size_t floats;
@@ -220,49 +220,49 @@ __device__ __forceinline__ int kv8_steps(int high, int step) { return (max(high,
 // Where a workgroup's run of steps begins.
 struct Kv8Place {
     int b, item, h, step;
-    int64_t share, total;
+    int share, total;
 };
 
 // All 256 threads: the steps before each sequence are summed up (in one order
 // everywhere), and step `share * w` is looked up in them.
 __device__ __forceinline__ Kv8Place kv8_find_place(const Kv8Args &c, int G, int tile, int step,
-                                                    int grid, int w, int64_t *s_wave,
+                                                    int grid, int w, int *s_wave,
                                                     Kv8Place *s_place) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, H = c.num_heads;
     const int per = (c.num_seqs + 255) / 256;
     auto steps = [&](int b) {
-        int64_t sum = 0;
+        int sum = 0;
         Kv8Tile t;
         for (int item = 0; kv8_tile_of(c, G, b, item, tile, &t); ++item) sum += kv8_steps(t.high, step);
         return sum * H;
     };
-    int64_t mine = 0;
+    int mine = 0;
     for (int b = tid * per; b < min((tid + 1) * per, c.num_seqs); ++b) mine += steps(b);
-    int64_t inc = mine;
+    int inc = mine;
     for (int o = 1; o < 64; o <<= 1) {
-        const int64_t up = __shfl_up(inc, o, 64);
+        const int up = __shfl_up(inc, o, 64);
         if (lane >= o) inc += up;
     }
     if (lane == 63) s_wave[wave] = inc;
     if (tid == 0) s_place->b = -1;
     __syncthreads();
-    const int64_t total = s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
-    int64_t at = inc - mine;
+    const int total = s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
+    int at = inc - mine;
     for (int i = 0; i < wave; ++i) at += s_wave[i];
-    const int64_t share = max((total + grid - 1) / grid, (int64_t)1);
-    const int64_t want = share * w;
+    const int share = max((total + grid - 1) / grid, 1);
+    const int want = share * w;  // (the host keeps (tiles + grid) * steps below 2^31)
     if (want >= at && want < at + mine) {
         for (int b = tid * per; b < min((tid + 1) * per, c.num_seqs); ++b) {
             Kv8Tile t;
             for (int item = 0; kv8_tile_of(c, G, b, item, tile, &t); ++item) {
                 const int n = kv8_steps(t.high, step);
-                if (want >= at && want < at + (int64_t)n * H) {
+                if (want >= at && want < at + n * H) {
                     s_place->b = b;
                     s_place->item = item;
-                    s_place->h = (int)((want - at) / n);
-                    s_place->step = (int)((want - at) % n);
+                    s_place->h = (want - at) / n;
+                    s_place->step = (want - at) % n;
                 }
-                at += (int64_t)n * H;
+                at += n * H;
             }
         }
     }
@@ -280,7 +280,7 @@ __device__ __forceinline__ bool kv8_next_tile(const Kv8Args &c, int G, int tile,
         at->h = 0;
         ++at->item;
     }
-    while (at->b < c.num_seqs) {
+    while (at->b >= 0 && at->b < c.num_seqs) {
         if (!kv8_tile_of(c, G, at->b, at->item, tile, T)) {
             ++at->b;
             at->item = 0;

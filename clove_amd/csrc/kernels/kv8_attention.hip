@@ -114,97 +114,102 @@ __global__ void __launch_bounds__(256) kv8_weights_any_kernel(Kv8Attention a, co
     if (threadIdx.x == 0) a.w_out[at] = a.w_in[at] + part[0];
 }
 
-// Joins the pieces of the tiles that were cut.  A workgroup takes `rows` rows of
-// a tile; rows = 1: its waves take the pieces in turn, else each wave takes
-// whole rows.  A lane holds up to four dims.
-__global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split p, int rows) {
+// Joins the pieces of the tiles that were cut: `per` waves take the pieces of a
+// row in turn, eight on their way at a time, and a lane holds up to four dims.
+__global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split p, int per) {
     const Kv8Args &c = a.c;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rows = (blockDim.x >> 6) / per;
     const int D = c.head_dim, H = c.num_heads, G = a.q_heads / H;
     const int groups = (p.stored + rows - 1) / rows;
     const int h = blockIdx.x % H, slot = blockIdx.x / H / groups;
-    const int u0 = (int)(blockIdx.x / H % groups) * rows;
+    const int u = (int)(blockIdx.x / H % groups) * rows + wave / per;
     __shared__ float s_o[16][kKv8MaxHeadDim], s_l[16], s_top[16];
+    const int *starts = reinterpret_cast<const int *>(a.ws + p.start_at);
+    const int share = starts[0], start = starts[1 + (size_t)slot * H + h];
     int item;
     const int b = kv8_slot(c, slot, p.tile, G, 1, &item);
     Kv8Tile T;
-    if (!kv8_tile_of(c, G, b, item, p.tile, &T) || T.high <= 0 || u0 >= T.rows) return;
-    const int64_t *starts = reinterpret_cast<const int64_t *>(a.ws + p.start_at);
-    const int64_t share = starts[0];
-    const int64_t start = starts[1 + (size_t)slot * H + h];
-    const int64_t end = start + kv8_steps(T.high, p.step), w0 = start / share;
-    const int np = (int)((end - 1) / share - w0) + 1;
+    if (!kv8_tile_of(c, G, b, item, p.tile, &T) || T.high <= 0) return;
+    const int end = start + kv8_steps(T.high, p.step), w0 = start / share;
+    const int np = (end - 1) / share - w0 + 1;
     if (np == 1) return;  // written whole
-    // the first piece ends its workgroup's run unless the run begins with it
-    const size_t first = (size_t)(2 * w0 + (start != w0 * share ? 1 : 0)) * p.stored;
-    auto place = [&](int i) { return i == 0 ? first : (size_t)(2 * (w0 + i)) * p.stored; };
-    const float2 *ml = reinterpret_cast<const float2 *>(a.ws + p.ml_at);
-    const float *o = a.ws + p.o_at;
-    const bool alone = rows == 1;  // one row for all waves
-    for (int u = alone ? u0 : u0 + wave; u < min(u0 + rows, T.rows); u += alone ? 1 : waves) {
-        float top = -INFINITY, l = 0.0f, x[4] = {0.f, 0.f, 0.f, 0.f};
-        // pieces wave, wave + waves, ... of a row all waves share, else all of them
-        const int p0 = alone ? wave : 0, dp = alone ? waves : 1;
-        for (int i = p0 + lane * dp; i < np; i += 64 * dp) top = fmaxf(top, ml[place(i) + u].x);
-        top = wave_max(top);
-        if (alone) {
-            if (lane == 0) s_top[wave] = top;
-            __syncthreads();
-            for (int w = 0; w < waves; ++w) top = fmaxf(top, s_top[w]);
-        }
-        for (int i0 = p0; i0 < np; i0 += 64 * dp) {
-            const int i = i0 + lane * dp;
-            float f = 0.0f;
-            if (i < np) {
-                const float2 v = ml[place(i) + u];
-                f = v.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v.x - top);
-                l += v.y * f;
-            }
-            const int k = min(64, (np - i0 + dp - 1) / dp);
-#pragma unroll 4
-            for (int j = 0; j < k; ++j) {
-                const float fj = __shfl(f, j, 64);
-                const float *oj = o + (place(i0 + j * dp) + u) * D;
+    float top = -INFINITY, l = 0.0f, x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (u < T.rows) {
+        // the first piece ends its workgroup's run unless the run begins with it
+        const size_t first = (size_t)(2 * w0 + (start != w0 * share ? 1 : 0)) * p.stored + u;
+        const float2 *ml = reinterpret_cast<const float2 *>(a.ws + p.ml_at);
+        const float *o = a.ws + p.o_at;
+        for (int i0 = wave % per; i0 < np; i0 += 8 * per) {
+            float2 v[8];
+            float y[8][4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (lane + 64 * e < D) x[e] = fmaf(oj[lane + 64 * e], fj, x[e]);
-            }
-        }
-        l = wave_sum(l);
-        if (alone) {
+            for (int j = 0; j < 8; ++j) {
+                const int i = i0 + j * per;
+                v[j] = make_float2(-INFINITY, 0.0f);
+                if (i < np) {
+                    const size_t at = i == 0 ? first : (size_t)(2 * (w0 + i)) * p.stored + u;
+                    v[j] = ml[at];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (lane + 64 * e < D) s_o[wave][lane + 64 * e] = x[e];
-            if (lane == 0) s_l[wave] = l;
-            __syncthreads();
-            if (wave) return;
-            l = 0.0f;
-            for (int w = 0; w < waves; ++w) l += s_l[w];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = 0.0f;
-                if (lane + 64 * e < D)
-                    for (int w = 0; w < waves; ++w) x[e] += s_o[w][lane + 64 * e];
+                    for (int e = 0; e < 4; ++e)
+                        y[j][e] = lane + 64 * e < D ? o[at * D + lane + 64 * e] : 0.0f;
+                }
             }
+            float t = top;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t = fmaxf(t, v[j].x);
+            const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - t);
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] *= f;
+            top = t;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (v[j].x != -INFINITY) {
+                    const float fj = __builtin_amdgcn_exp2f(v[j].x - t);
+                    l = fmaf(v[j].y, fj, l);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = fmaf(y[j][e], fj, x[e]);
+                }
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const size_t rh = (size_t)(T.first + (T.r0 + u) / G) * a.q_heads + h * G + (T.r0 + u) % G;
+    }
+    if (per > 1) {  // (one row to the workgroup)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (lane + 64 * e < D) a.out[rh * D + lane + 64 * e] = x[e] * inv;
-        if (lane == 0 && a.w_out)
-            reinterpret_cast<float2 *>(a.ws + p.row_ml_at)[rh] = make_float2(top, inv);
+            if (lane + 64 * e < D) s_o[wave][lane + 64 * e] = x[e];
+        if (lane == 0) {
+            s_l[wave] = l;
+            s_top[wave] = top;
+        }
+        __syncthreads();
+        if (wave) return;
+        for (int w = 1; w < per; ++w) top = fmaxf(top, s_top[w]);
+        l = x[0] = x[1] = x[2] = x[3] = 0.0f;
+        for (int w = 0; w < per; ++w) {
+            const float f = s_top[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_top[w] - top);
+            l = fmaf(s_l[w], f, l);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (lane + 64 * e < D) x[e] = fmaf(s_o[w][lane + 64 * e], f, x[e]);
+        }
     }
+    if (u >= T.rows) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const size_t rh = (size_t)(T.first + (T.r0 + u) / G) * a.q_heads + h * G + (T.r0 + u) % G;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (lane + 64 * e < D) a.out[rh * D + lane + 64 * e] = x[e] * inv;
+    if (lane == 0 && a.w_out)
+        reinterpret_cast<float2 *>(a.ws + p.row_ml_at)[rh] = make_float2(top, inv);
 }
 
 // The weight of each block from the sums stored on the way: lanes take 64
-// blocks, the four waves a sequence's rows and heads in turn.
-__global__ void __launch_bounds__(256) kv8_weights_kernel(Kv8Attention a, Kv8Split p) {
+// blocks, the waves a sequence's rows and heads in turn.
+__global__ void __launch_bounds__(1024) kv8_weights_kernel(Kv8Attention a, Kv8Split p) {
     const Kv8Args &c = a.c;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const int j = blockIdx.x * 64 + lane, b = blockIdx.y;
     const int per = c.block_size / p.sums;
-    __shared__ float part[4][64];
+    __shared__ float part[16][64];
     int first, n;
     kv8_rows(c, b, &first, &n);
     const int ctx = kv8_context(c, b);
@@ -212,7 +217,8 @@ __global__ void __launch_bounds__(256) kv8_weights_kernel(Kv8Attention a, Kv8Spl
     const float2 *sums = reinterpret_cast<const float2 *>(a.ws + p.sums_at);
     float w = 0.0f;
     if (j < c.max_blocks && (int64_t)j * c.block_size < ctx) {
-        for (int x = wave; x < n * a.q_heads; x += 4) {
+        #pragma unroll 4
+        for (int x = wave; x < n * a.q_heads; x += waves) {
             const size_t rh = (size_t)first * a.q_heads + x;
             const int see = ctx - n + x / a.q_heads + 1 - j * c.block_size;
             const float2 ml = row_ml[rh];
@@ -227,7 +233,8 @@ __global__ void __launch_bounds__(256) kv8_weights_kernel(Kv8Attention a, Kv8Spl
     __syncthreads();
     if (wave == 0 && j < c.max_blocks) {
         const size_t at = (size_t)b * c.max_blocks + j;
-        a.w_out[at] = a.w_in[at] + ((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]));
+        for (int x = 1; x < waves; ++x) w += part[x][lane];
+        a.w_out[at] = a.w_in[at] + w;
     }
 }
 
@@ -274,12 +281,13 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
     if (tiles >= (1 << 20) || kv8_slots(c, kKv8WeightPart, G, 1) > 65535) return plain();
     const int64_t steps = (cap + p.step - 1) / p.step;
     const int64_t room = std::min(kKv8MaxGrid, cus * residents);
+    if (tiles * steps >= (1ll << 30)) return plain();
     p.join = steps > 1 && (p.kind == KV8_STREAM || tiles < 2 * room);
     p.grid = (int)(p.join || p.kind == KV8_STREAM ? std::min<int64_t>(room, tiles * steps) : tiles);
     if (p.join) {
         p.o_at = take((int64_t)2 * p.grid * p.stored * D);
         p.ml_at = take((int64_t)2 * p.grid * p.stored * 2);
-        p.start_at = take(2 * (1 + tiles));
+        p.start_at = take(1 + tiles);
     }
     if (a.w_out) {
         p.row_ml_at = take(2 * rh);
@@ -317,18 +325,18 @@ void kv8_attention(const Kv8Attention &a, int cus, hipStream_t s) {
     else
         kv8_tiles(a, p, s);
     if (p.join) {
-        // few rows: a workgroup each, with more waves the more pieces there are
-        // to a tile; many: four to a wave
         const unsigned tiles = (unsigned)kv8_slots(c, p.tile, a.q_heads / c.num_heads, 1) * c.num_heads;
-        const bool few = p.kind == KV8_STREAM && (int64_t)tiles * p.stored <= 4096;
-        const int rows = few ? 1 : 16, pieces = p.grid / (int)tiles + 1;
-        const int threads = !few ? 256 : pieces <= 4 ? 64 : pieces <= 16 ? 256 : 1024;
-        kv8_join_kernel<<<tiles * ((p.stored + rows - 1) / rows), threads, 0, s>>>(a, p, rows);
+        // pieces to a tile: 2 on the average where there are as many tiles as runs
+        const int pieces = p.grid / (int)tiles + 1;
+        const int per = pieces <= 8 ? 1 : pieces <= 32 ? 4 : 16;
+        const int waves = std::max(per, std::min(4, p.stored)), rows = waves / per;
+        kv8_join_kernel<<<tiles * ((p.stored + rows - 1) / rows), 64 * waves, 0, s>>>(a, p, per);
     }
     if (weights && p.kind == KV8_TILE)
         kv8_tile_weights(a, p, s);
     else if (weights)
-        kv8_weights_kernel<<<dim3((c.max_blocks + 63) / 64, c.num_seqs), 256, 0, s>>>(a, p);
+        kv8_weights_kernel<<<dim3((c.max_blocks + 63) / 64, c.num_seqs), a.q_heads > 8 ? 1024 : 256, 0,
+                             s>>>(a, p);
 }
 
 }  // namespace k

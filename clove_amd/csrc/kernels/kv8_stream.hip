@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(256, DP * NC > 128 ? 2 : 3)
         float o[4][16][kPitch];
     } sh;
     __shared__ float s_m[4][16], s_l[4][16];
-    __shared__ int64_t s_wave[4];
+    __shared__ int s_wave[4];
     __shared__ Kv8Place s_place;
 
     if ((int)blockIdx.x >= p.grid) {
@@ -81,18 +81,18 @@ __global__ void __launch_bounds__(256, DP * NC > 128 ? 2 : 3)
     }
     Kv8Place at =
         kv8_find_place(c, G, p.tile, p.step, p.grid, blockIdx.x, s_wave, &s_place);
-    int64_t *starts = reinterpret_cast<int64_t *>(a.ws + p.start_at);
+    int *starts = reinterpret_cast<int *>(a.ws + p.start_at);
     if (p.join && blockIdx.x == 0 && tid == 0) starts[0] = at.share;
-    int64_t left = min(at.share, at.total - at.share * blockIdx.x);
+    int left = min(at.share, at.total - at.share * (int)blockIdx.x);
     bool front = true;
 
     while (left > 0) {
         Kv8Tile T;
         if (!kv8_next_tile(c, G, p.tile, &at, &T)) return;
         const int h = at.h, all = kv8_steps(T.high, kStep);
-        const int s0 = at.step, s1 = (int)min((int64_t)all, s0 + left);
+        const int s0 = at.step, s1 = min(all, s0 + left);
         const int t_end = min(s1 * kStep, T.high);
-        const int64_t run0 = at.share * blockIdx.x + (min(at.share, at.total - at.share * blockIdx.x) - left);
+        const int run0 = at.share * (int)blockIdx.x + (min(at.share, at.total - at.share * (int)blockIdx.x) - left);
         if (p.join && s0 == 0 && tid == 0)
             starts[1 + (size_t)(kv8_first_slot(c, at.b, p.tile, G, 1) + at.item) * H + h] = run0;
 

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
     const int H = c.num_heads, G = a.q_heads / H, D = c.head_dim, bs = c.block_size;
     __shared__ uint2 table[kChunk / 4];
     __shared__ __attribute__((aligned(16))) uint8_t sK[2][KB * PK], sV[2][DP * PV];
-    __shared__ int64_t s_wave[4];
+    __shared__ int s_wave[4];
     __shared__ Kv8Place s_place;
 
     if ((int)blockIdx.x >= p.grid) {
@@ -82,13 +82,13 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
         return;
     }
     Kv8Place at;
-    int64_t left, run = 0;
+    int left, run = 0;
     if (p.join) {
         at = kv8_find_place(c, G, p.tile, p.step, p.grid, blockIdx.x, s_wave, &s_place);
-        run = min(at.share, at.total - at.share * blockIdx.x);
+        run = min(at.share, at.total - at.share * (int)blockIdx.x);
         left = run;
         if (blockIdx.x == 0 && tid == 0)
-            reinterpret_cast<int64_t *>(a.ws + p.start_at)[0] = at.share;
+            reinterpret_cast<int *>(a.ws + p.start_at)[0] = at.share;
     } else {
         // a tile to a workgroup; a sequence's last tiles, the longest, first
         at.h = blockIdx.x % H;
@@ -107,12 +107,12 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
             return;
         }
         const int h = at.h, all = kv8_steps(T.high, KB);
-        const int s0 = at.step, s1 = p.join ? (int)min((int64_t)all, s0 + left) : all;
+        const int s0 = at.step, s1 = p.join ? min(all, s0 + left) : all;
         const int t_end = min(s1 * KB, T.high);
         if (p.join && s0 == 0 && tid == 0)
-            reinterpret_cast<int64_t *>(a.ws + p.start_at)
+            reinterpret_cast<int *>(a.ws + p.start_at)
                 [1 + (size_t)(kv8_first_slot(c, at.b, p.tile, G, 1) + at.item) * H + h] =
-                    at.share * blockIdx.x + (run - left);
+                    at.share * (int)blockIdx.x + (run - left);
 
         // this wave's rows: q in pieces, and the tokens each row sees
         u4 qf[NR][KI][3];
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
             for (int kb = c0; kb < c1; kb += KB, buf ^= 1) {
                 const bool more = kb + KB < c1;
                 if (more) load(kb + KB);
-#pragma unroll
+#pragma unroll 1
                 for (int sub = 0; sub < KB / 32; ++sub) {
                     const int t0 = kb + 32 * sub;
                     if (t0 >= high) break;
@@ -514,12 +514,12 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
 }
 
 // The quads' sums of all parts and heads into the blocks' weights; lanes take 64
-// blocks, the four waves the parts and heads in turn.
-__global__ void __launch_bounds__(256) block_weights_kernel(Kv8Attention a, Kv8Split p) {
+// blocks, the sixteen waves the parts and heads in turn.
+__global__ void __launch_bounds__(1024) block_weights_kernel(Kv8Attention a, Kv8Split p) {
     const Kv8Args &c = a.c;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int j = blockIdx.x * 64 + lane, b = blockIdx.y, per = c.block_size / 4;
-    __shared__ float part[4][64];
+    __shared__ float part[16][64];
     const int ctx = kv8_context(c, b);
     int first, n;
     kv8_rows(c, b, &first, &n);
@@ -528,8 +528,9 @@ __global__ void __launch_bounds__(256) block_weights_kernel(Kv8Attention a, Kv8S
         const int G = a.q_heads / c.num_heads, quads = min(per, (ctx - j * c.block_size + 3) / 4);
         const int parts = (n * G + kPart - 1) / kPart;
         const size_t slot = kv8_first_slot(c, b, kPart, G, 1);
-        for (int x = wave; x < parts * c.num_heads; x += 4) {
+        for (int x = wave; x < parts * c.num_heads; x += 16) {
             const float *y = a.ws + p.sums_at + (slot * c.num_heads + x) * p.groups + (size_t)j * per;
+#pragma unroll 4
             for (int i = 0; i < quads; ++i) w += y[i];
         }
     }
@@ -537,7 +538,8 @@ __global__ void __launch_bounds__(256) block_weights_kernel(Kv8Attention a, Kv8S
     __syncthreads();
     if (wave == 0 && j < c.max_blocks) {
         const size_t at = (size_t)b * c.max_blocks + j;
-        a.w_out[at] = a.w_in[at] + ((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]));
+        for (int x = 1; x < 16; ++x) w += part[x][lane];
+        a.w_out[at] = a.w_in[at] + w;
     }
 }
 
@@ -564,7 +566,7 @@ void kv8_tile_weights(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
     if (p.dp == 64) tile_weights_kernel<64><<<grid, 256, 0, s>>>(a, p);
     if (p.dp == 128) tile_weights_kernel<128><<<grid, 256, 0, s>>>(a, p);
     if (p.dp == 256) tile_weights_kernel<256><<<grid, 256, 0, s>>>(a, p);
-    block_weights_kernel<<<dim3((c.max_blocks + 63) / 64, c.num_seqs), 256, 0, s>>>(a, p);
+    block_weights_kernel<<<dim3((c.max_blocks + 63) / 64, c.num_seqs), 1024, 0, s>>>(a, p);
 }
 
 }  // namespace k
