@@ -171,21 +171,25 @@ struct Kv8Split {
     int dp;            // head_dim the kernel is laid out for
     int tile;
     int step;
+    int hw;            // heads that a workgroup takes together
     int grid;          // workgroups that share the steps, at most kKv8MaxGrid
     bool join;         // whether a tile may be cut
     int stored;        // rows of a piece
     int sums;          // tokens to a stored sum of weights, 0: none stored
     int groups;        // such sums a row
     // in the workspace, in floats
-    size_t o_at, ml_at;      // piece 2w (+ 1: at the end of the run) of workgroup w:
-                             // `stored` sums over V [D], and (maximum, sum) pairs
-    size_t start_at;         // share, then [slot, head] first step of the tile
+    size_t o_at, ml_at;      // piece 2w (+ 1: at the end of the run) of workgroup w: of hw
+                             // heads `stored` sums over V [D], and (maximum, sum) pairs
+    size_t start_at;         // share, then [slot, head / hw] first step of the tile
     size_t row_ml_at;        // (maximum, 1 / sum) of every row and query head
     size_t sums_at;          // [row, query head][groups] (sum, maximum) pairs
     size_t floats;
 };
 enum { KV8_ANY = 0, KV8_STREAM = 1, KV8_TILE = 2 };
-constexpr int kKv8StreamStep = 128, kKv8TileStep = 64, kKv8MaxGrid = 1024;
+constexpr int kKv8MaxGrid = 1024;
+// Heads that a workgroup of the stream kernel takes together, where there are
+// whole groups of them.
+constexpr int kv8_stream_heads(int dp, int tile) { return dp * tile <= 128 * 16 ? 4 : 2; }
 
 // The rows of a tile and the tokens they see.
 struct Kv8Tile {
@@ -225,10 +229,10 @@ struct Kv8Place {
 
 // All 256 threads: the steps before each sequence are summed up (in one order
 // everywhere), and step `share * w` is looked up in them.
-__device__ __forceinline__ Kv8Place kv8_find_place(const Kv8Args &c, int G, int tile, int step,
+__device__ __forceinline__ Kv8Place kv8_find_place(const Kv8Args &c, int G, int H, int tile, int step,
                                                     int grid, int w, int *s_wave,
                                                     Kv8Place *s_place) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, H = c.num_heads;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int per = (c.num_seqs + 255) / 256;
     auto steps = [&](int b) {
         int sum = 0;
@@ -274,9 +278,9 @@ __device__ __forceinline__ Kv8Place kv8_find_place(const Kv8Args &c, int G, int 
 }
 
 // Moves `at` on to the next tile with steps; false behind the last.
-__device__ __forceinline__ bool kv8_next_tile(const Kv8Args &c, int G, int tile, Kv8Place *at,
+__device__ __forceinline__ bool kv8_next_tile(const Kv8Args &c, int G, int H, int tile, Kv8Place *at,
                                               Kv8Tile *T) {
-    if (at->h >= c.num_heads) {
+    if (at->h >= H) {
         at->h = 0;
         ++at->item;
     }
@@ -324,7 +328,7 @@ __device__ __forceinline__ unsigned kv8_widen(unsigned codes, float scale) {
 }
 
 // Workgroups of the stream kernel that a CU holds.
-int kv8_stream_residents(int dp, int tile);
+int kv8_stream_residents();
 void kv8_stream(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
 void kv8_tiles(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
 // The weights of the blocks, the scores computed again (kv8_tiles has left every

@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split
     const int u = (int)(blockIdx.x / H % groups) * rows + wave / per;
     __shared__ float s_o[16][kKv8MaxHeadDim], s_l[16], s_top[16];
     const int *starts = reinterpret_cast<const int *>(a.ws + p.start_at);
-    const int share = starts[0], start = starts[1 + (size_t)slot * H + h];
+    const int share = starts[0], start = starts[1 + (size_t)slot * (H / p.hw) + h / p.hw];
     int item;
     const int b = kv8_slot(c, slot, p.tile, G, 1, &item);
     Kv8Tile T;
@@ -136,7 +136,8 @@ __global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split
     float top = -INFINITY, l = 0.0f, x[4] = {0.f, 0.f, 0.f, 0.f};
     if (u < T.rows) {
         // the first piece ends its workgroup's run unless the run begins with it
-        const size_t first = (size_t)(2 * w0 + (start != w0 * share ? 1 : 0)) * p.stored + u;
+        const size_t row = (size_t)(h % p.hw) * p.stored + u, per_piece = (size_t)p.hw * p.stored;
+        const size_t first = (2 * w0 + (start != w0 * share ? 1 : 0)) * per_piece + row;
         const float2 *ml = reinterpret_cast<const float2 *>(a.ws + p.ml_at);
         const float *o = a.ws + p.o_at;
         for (int i0 = wave % per; i0 < np; i0 += 8 * per) {
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split
                 const int i = i0 + j * per;
                 v[j] = make_float2(-INFINITY, 0.0f);
                 if (i < np) {
-                    const size_t at = i == 0 ? first : (size_t)(2 * (w0 + i)) * p.stored + u;
+                    const size_t at = i == 0 ? first : 2 * (w0 + i) * per_piece + row;
                     v[j] = ml[at];
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
@@ -268,16 +269,26 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
     if (units <= (p.dp == 256 ? 16 : 32)) {
         p.kind = KV8_STREAM;
         p.tile = units <= 16 || p.dp == 256 ? 16 : 32;
-        p.step = kKv8StreamStep;
-        residents = kv8_stream_residents(p.dp, p.tile);
+        // Four heads of the same tokens side by side are 8 KB in a row to the memory
+        // (32 x 4096 tokens, 32 heads of 128: 98 against 109 us) but cut a tile
+        // into four times the pieces: where the heads' tiles are few, that costs
+        // more than it gives (one context of 131001 tokens: 57 against 47 us;
+        // speculated tokens: 59 against 50).
+        p.hw = kv8_stream_heads(p.dp, p.tile);
+        if (c.num_heads % p.hw ||
+            2 * kv8_slots(c, p.tile, G, 1) * c.num_heads / p.hw < cus * kv8_stream_residents())
+            p.hw = 1;
+        p.step = 32 * 4 / p.hw;
+        residents = kv8_stream_residents();
     } else {
         p.kind = KV8_TILE;
         p.tile = units <= 64 || p.dp == 256 ? 64 : 128;
-        p.step = p.dp == 256 ? 32 : kKv8TileStep;
+        p.hw = 1;
+        p.step = p.dp == 256 ? 32 : 64;
         residents = 2;
     }
     p.stored = !c.row_starts && G < p.tile ? G : p.tile;
-    const int64_t tiles = kv8_slots(c, p.tile, G, 1) * c.num_heads;
+    const int64_t tiles = kv8_slots(c, p.tile, G, 1) * c.num_heads / p.hw;
     if (tiles >= (1 << 20) || kv8_slots(c, kKv8WeightPart, G, 1) > 65535) return plain();
     const int64_t steps = (cap + p.step - 1) / p.step;
     const int64_t room = std::min(kKv8MaxGrid, cus * residents);
@@ -285,8 +296,8 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
     p.join = steps > 1 && (p.kind == KV8_STREAM || tiles < 2 * room);
     p.grid = (int)(p.join || p.kind == KV8_STREAM ? std::min<int64_t>(room, tiles * steps) : tiles);
     if (p.join) {
-        p.o_at = take((int64_t)2 * p.grid * p.stored * D);
-        p.ml_at = take((int64_t)2 * p.grid * p.stored * 2);
+        p.o_at = take((int64_t)2 * p.grid * p.hw * p.stored * D);
+        p.ml_at = take((int64_t)2 * p.grid * p.hw * p.stored * 2);
         p.start_at = take(1 + tiles);
     }
     if (a.w_out) {
@@ -327,7 +338,7 @@ void kv8_attention(const Kv8Attention &a, int cus, hipStream_t s) {
     if (p.join) {
         const unsigned tiles = (unsigned)kv8_slots(c, p.tile, a.q_heads / c.num_heads, 1) * c.num_heads;
         // pieces to a tile: 2 on the average where there are as many tiles as runs
-        const int pieces = p.grid / (int)tiles + 1;
+        const int pieces = p.grid * p.hw / (int)tiles + 1;
         const int per = pieces <= 8 ? 1 : pieces <= 32 ? 4 : 16;
         const int waves = std::max(per, std::min(4, p.stored)), rows = waves / per;
         kv8_join_kernel<<<tiles * ((p.stored + rows - 1) / rows), 64 * waves, 0, s>>>(a, p, per);

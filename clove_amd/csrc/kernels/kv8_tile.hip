@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
     Kv8Place at;
     int left, run = 0;
     if (p.join) {
-        at = kv8_find_place(c, G, p.tile, p.step, p.grid, blockIdx.x, s_wave, &s_place);
+        at = kv8_find_place(c, G, H, p.tile, p.step, p.grid, blockIdx.x, s_wave, &s_place);
         run = min(at.share, at.total - at.share * (int)blockIdx.x);
         left = run;
         if (blockIdx.x == 0 && tid == 0)
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
     while (left > 0) {
         Kv8Tile T;
         if (p.join) {
-            if (!kv8_next_tile(c, G, p.tile, &at, &T)) return;
+            if (!kv8_next_tile(c, G, H, p.tile, &at, &T)) return;
         } else if (!kv8_tile_of(c, G, at.b, at.item, p.tile, &T) || T.high <= 0) {
             return;
         }
