@@ -64,6 +64,9 @@ k::Kv8Args cache_args(const Tensor &codes, const Tensor &exps, const Tensor &bt,
     // grids count threads in 32 bits, up to 256 a row
     CLOVE_REQUIRE(rows < (1ull << 24), CLOVE_HIP_ERR_SHAPE,
                   "the rows of a call must be fewer than 2^24");
+    // (the append and the read cut the rows into tiles of a block and head)
+    CLOVE_REQUIRE((rows / bs + 2 * cl.numel) * ((H + 3) / 4) * 2 + rows < (1ull << 32),
+                  CLOVE_HIP_ERR_SHAPE, "too many rows and heads");
     k::Kv8Args a{};
     a.codes = codes.u8();
     a.exps = exps.i32();
@@ -104,7 +107,7 @@ void HipBackend::paged_kv8_append(const Tensor &codes, const Tensor &exps, const
     CLOVE_REQUIRE(rows_of(v, row ? row : 1, "v") == rows, CLOVE_HIP_ERR_SHAPE,
                   "k and v must have the same number of elements");
     const k::Kv8Args a = cache_args(codes, exps, bt, cl, rs, rows);
-    if (a.num_seqs == 0 || a.rows == 0 || a.num_blocks == 0) return;
+    if (a.num_seqs == 0 || a.rows == 0) return;
     k::kv8_append(a, k.f32(), v.f32(), ctx().stream);
 }
 
