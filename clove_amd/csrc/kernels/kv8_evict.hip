@@ -1,19 +1,19 @@
 // kv8_evict.hip -- eviction of the lightest blocks of long sequences.
 //
 // One workgroup a sequence.  Of its n = ceil(ctx / block_size) blocks the first
-// and last ones stay; of the m between them the (budget - first - last) heaviest
-// do.  The weight of the last one that stays is found by radix selection, a byte
-// of the order-preserving key a pass (four histograms of 256 bins), then one
-// ordered pass writes kept and evicted blocks: among equal weights the earlier
-// blocks stay.  Only integers are counted, so results do not depend on timing.
+// and last ones stay; of those between them the (budget - first - last) heaviest
+// do.  Weights are read once, as unsigned keys of the same order, into registers
+// (K a thread).  The least key that stays is
+// found bit by bit from the top: the largest x with at least `left` keys >= x,
+// counted by ballots, which ends early once exactly `left` are.  One scan then
+// gives every block its place: among equal weights the earlier blocks stay.
+// Only integers are counted, so results do not depend on timing.
 #include "kv8.h"
 
 namespace clove {
 namespace k {
 
 namespace {
-
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
 
 // Unsigned keys in the order of the weights; NaN lowest, -0 as 0.
 __device__ __forceinline__ unsigned order_key(float w) {
@@ -22,32 +22,24 @@ __device__ __forceinline__ unsigned order_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Exclusive sum over the workgroup in thread order; *total gets the whole sum.
-__device__ __forceinline__ int block_scan(int v, int *s_wave, int *total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int inc = v;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int up = __shfl_up(inc, o, 64);
-        if (lane >= o) inc += up;
-    }
-    __syncthreads();
-    if (lane == 63) s_wave[wave] = inc;
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int w = 0; w < kWaves; ++w) {
-        const int x = s_wave[w];
-        if (w < wave) before += x;
-        all += x;
-    }
-    *total = all;
-    return before + inc - v;
-}
-
-__global__ void __launch_bounds__(kThreads) evict_kernel(EvictArgs a) {
-    const int b = blockIdx.x, tid = threadIdx.x;
+// Block tid + THREADS * i is thread tid's i-th.  K = 0: more blocks than registers
+// hold; they are read again for every bit.
+template <int THREADS, int K>
+__global__ void __launch_bounds__(THREADS) evict_kernel(EvictArgs a) {
+    constexpr int kWaves = THREADS / 64;
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const size_t at = (size_t)b * a.max_blocks;
     const int32_t *table = a.tables + at;
-    const float *w = a.weights + at;
+    const float *weights = a.weights + at;
+    const int rounds = K ? K : (a.max_blocks + THREADS - 1) / THREADS;
+    float w[K ? K : 1];
+    int id[K ? K : 1];
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        const int j = tid + THREADS * i;
+        w[i] = j < a.max_blocks ? weights[j] : 0.0f;
+        id[i] = j < a.max_blocks ? table[j] : 0;
+    }
     const int cap = a.max_blocks * a.block_size;
     int ctx = a.lens[b];
     if (ctx < 0 || ctx > cap) {
@@ -55,78 +47,153 @@ __global__ void __launch_bounds__(kThreads) evict_kernel(EvictArgs a) {
         ctx = ctx < 0 ? 0 : cap;
     }
     const int n = ctx / a.block_size + (ctx % a.block_size != 0);
-    const int gone_all = max(n - a.budget, 0);
-    __shared__ int hist[256], s_wave[kWaves], s_byte, s_left;
+    const int gone = max(n - a.budget, 0), mid_end = n - a.last;
+    const int left = a.budget - a.first - a.last;  // places for blocks [first, mid_end)
+    __shared__ int s_count[2][kWaves];
 
-    // blocks [first, n - last) compete for `left` places
-    const int mid_end = n - a.last;
-    unsigned prefix = 0, mask = 0;
-    int left = a.budget - a.first - a.last;
-    if (gone_all > 0 && left > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += kThreads) hist[i] = 0;
-            __syncthreads();
-            for (int i = a.first + tid; i < mid_end; i += kThreads) {
-                const unsigned key = order_key(w[i]);
-                if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
-            }
-            __syncthreads();
-            if (tid == 0) {
-                int byte = 255, need = left;
-                while (byte > 0 && hist[byte] < need) need -= hist[byte--];
-                s_byte = byte;
-                s_left = need;
-            }
-            __syncthreads();
-            prefix |= (unsigned)s_byte << shift;
-            mask |= 255u << shift;
-            left = s_left;
-            __syncthreads();
-        }
-    }
-    // kept: key above prefix, or equal to it and among the first `left` of those
-    const bool some = a.budget - a.first - a.last > 0;
-    const int per = (n + kThreads - 1) / kThreads;
-    const int i0 = min(tid * per, n), i1 = min(i0 + per, n);
-    int ties = 0;
-    if (gone_all > 0 && some)
-        for (int i = max(i0, a.first); i < min(i1, mid_end); ++i)
-            ties += order_key(w[i]) == prefix;
-    int total;
-    int tie_at = block_scan(ties, s_wave, &total);
-    auto keeps = [&](int i) {
-        if (gone_all == 0 || i < a.first || i >= mid_end) return true;
-        if (!some) return false;
-        const unsigned key = order_key(w[i]);
-        return key > prefix || (key == prefix && tie_at++ < left);
+    // (a block that does not compete has the key 0, which no bit counts)
+    auto mid = [&](int j) { return j >= a.first && j < mid_end; };
+    unsigned keys[K ? K : 1];
+#pragma unroll
+    for (int i = 0; i < K; ++i) keys[i] = mid(tid + THREADS * i) ? order_key(w[i]) : 0;
+    auto key = [&](int i) {
+        const int j = tid + THREADS * i;
+        return K ? keys[K ? i : 0] : mid(j) ? order_key(weights[j]) : 0u;
     };
-    const int tie0 = tie_at;
-    int kept = 0;
-    for (int i = i0; i < i1; ++i) kept += keeps(i);
-    const int kept_at = block_scan(kept, s_wave, &total);
-    tie_at = tie0;
-    int to = kept_at, out = i0 - kept_at;
-    for (int i = i0; i < i1; ++i) {
-        if (keeps(i)) {
-            a.tables_out[at + to] = table[i];
-            a.weights_out[at + to] = w[i];
-            ++to;
-        } else {
-            a.evicted[at + out++] = table[i];
+    unsigned least = ~0u;  // kept: keys above it, and the first ones equal to it
+    if (gone > 0 && left > 0) {
+        least = 0;
+        for (int bit = 31; bit >= 0; --bit) {
+            const unsigned x = least | 1u << bit;
+            int count = 0;
+            if constexpr (K > 0) {
+#pragma unroll
+                for (int i = 0; i < K; ++i) count += __popcll(__ballot(keys[i] >= x));
+            } else {
+                for (int i = 0; i < rounds; ++i) count += __popcll(__ballot(key(i) >= x));
+            }
+            if (lane == 0) s_count[bit & 1][wave] = count;
+            __syncthreads();
+            count = 0;
+#pragma unroll
+            for (int v = 0; v < kWaves; ++v) count += s_count[bit & 1][v];
+            if (count >= left) least = x;
+            if (count == left) break;
         }
     }
-    for (int i = n - gone_all + tid; i < a.max_blocks; i += kThreads) {
+    auto sure = [&](int i) {  // stays whatever the ties
+        const int j = tid + THREADS * i;
+        return j < n && (gone == 0 || !mid(j) || key(i) > least);
+    };
+    auto tied = [&](int i) {
+        return gone > 0 && left > 0 && mid(tid + THREADS * i) && key(i) == least;
+    };
+    // before a block: `x` that surely stay and `y` ties, of which the first stay
+    auto put = [&](int i, int2 before, int ties, uint64_t bs, uint64_t bt) {
+        const int j = tid + THREADS * i;
+        if (j >= n) return;
+        const uint64_t below = (1ull << lane) - 1;
+        before.x += __popcll(bs & below);
+        before.y += __popcll(bt & below);
+        const int to = before.x + min(before.y, ties);
+        const int block = K ? id[K ? i : 0] : table[j];
+        if ((bs >> lane & 1) || ((bt >> lane & 1) && before.y < ties)) {
+            a.tables_out[at + to] = block;
+            a.weights_out[at + to] = K ? w[K ? i : 0] : weights[j];
+        } else {
+            a.evicted[at + j - to] = block;
+        }
+    };
+    if constexpr (K > 0) {
+        // one scan over what every wave counts in every round, in block order
+        constexpr int E = K * kWaves, PER = (E + 63) / 64;
+        __shared__ int2 s_before[PER * 64];
+        __shared__ int s_sure;
+        uint64_t bs[K], bt[K];
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            bs[i] = __ballot(sure(i));
+            bt[i] = __ballot(tied(i));
+            if (lane == 0) s_before[i * kWaves + wave] = make_int2(__popcll(bs[i]), __popcll(bt[i]));
+        }
+        __syncthreads();
+        if (wave == 0) {
+            int2 mine = {0, 0}, each[PER];
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                each[i] = lane * PER + i < E ? s_before[lane * PER + i] : make_int2(0, 0);
+                mine.x += each[i].x;
+                mine.y += each[i].y;
+            }
+            int2 inc = mine;
+            for (int o = 1; o < 64; o <<= 1) {
+                const int x = __shfl_up(inc.x, o, 64), y = __shfl_up(inc.y, o, 64);
+                if (lane >= o) {
+                    inc.x += x;
+                    inc.y += y;
+                }
+            }
+            if (lane == 63) s_sure = inc.x;
+            inc.x -= mine.x;
+            inc.y -= mine.y;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                s_before[lane * PER + i] = inc;
+                inc.x += each[i].x;
+                inc.y += each[i].y;
+            }
+        }
+        __syncthreads();
+        const int ties = gone > 0 ? a.budget - s_sure : 0;
+#pragma unroll
+        for (int i = 0; i < K; ++i) put(i, s_before[i * kWaves + wave], ties, bs[i], bt[i]);
+    } else {
+        __shared__ int2 s_wave[2][kWaves];
+        int all = 0;
+        for (int i = 0; i < rounds; ++i) all += __popcll(__ballot(sure(i)));
+        __syncthreads();  // (s_count is done with)
+        if (lane == 0) s_count[0][wave] = all;
+        __syncthreads();
+        all = 0;
+        for (int v = 0; v < kWaves; ++v) all += s_count[0][v];
+        const int ties = gone > 0 ? a.budget - all : 0;
+        int2 base = {0, 0};
+        for (int i = 0; i < rounds; ++i) {
+            const uint64_t bs = __ballot(sure(i)), bt = __ballot(tied(i));
+            if (lane == 0) s_wave[i & 1][wave] = make_int2(__popcll(bs), __popcll(bt));
+            __syncthreads();
+            int2 before = base;
+            for (int v = 0; v < kWaves; ++v) {
+                const int2 x = s_wave[i & 1][v];
+                if (v < wave) {
+                    before.x += x.x;
+                    before.y += x.y;
+                }
+                base.x += x.x;
+                base.y += x.y;
+            }
+            put(i, before, ties, bs, bt);
+        }
+    }
+    for (int i = n - gone + tid; i < a.max_blocks; i += THREADS) {
         a.tables_out[at + i] = -1;
         a.weights_out[at + i] = 0.0f;
     }
-    for (int i = gone_all + tid; i < a.max_blocks; i += kThreads) a.evicted[at + i] = -1;
-    if (tid == 0) a.lens_out[b] = ctx - gone_all * a.block_size;
+    for (int i = gone + tid; i < a.max_blocks; i += THREADS) a.evicted[at + i] = -1;
+    if (tid == 0) a.lens_out[b] = ctx - gone * a.block_size;
 }
 
 }  // namespace
 
 void paged_evict(const EvictArgs &a, hipStream_t s) {
-    evict_kernel<<<a.num_seqs, kThreads, 0, s>>>(a);
+    if (a.max_blocks <= 256 * 4)
+        evict_kernel<256, 4><<<a.num_seqs, 256, 0, s>>>(a);
+    else if (a.max_blocks <= 256 * 16)
+        evict_kernel<512, 8><<<a.num_seqs, 512, 0, s>>>(a);
+    else if (a.max_blocks <= 1024 * 16)
+        evict_kernel<1024, 16><<<a.num_seqs, 1024, 0, s>>>(a);
+    else
+        evict_kernel<1024, 0><<<a.num_seqs, 1024, 0, s>>>(a);
 }
 
 }  // namespace k

@@ -50,7 +50,7 @@ def check_append(hip, g, codes, exps, k, v, tables, lens, starts):
 
 @pytest.mark.parametrize("D,bs,H", [(64, 16, 3), (128, 16, 2), (80, 8, 2), (256, 32, 1), (96, 64, 2),
                                     (1, 1, 1), (7, 5, 3), (33, 16, 2), (130, 3, 1), (16, 128, 2),
-                                    (4, 16, 5), (255, 33, 1)])
+                                    (4, 16, 5), (255, 33, 1), (128, 128, 1)])
 @pytest.mark.parametrize("rows_hi,past_hi", [(1, 70), (40, 0), (90, 50)])
 def test_append_and_read(hip, D, bs, H, rows_hi, past_hi):
     g = rng(1000 + D * 31 + bs + rows_hi)
@@ -361,7 +361,8 @@ def test_no_rows_and_no_sequences(hip):
 
 @pytest.mark.parametrize("width,bs,budget,first,last", [
     (1, 16, 1, 0, 1), (5, 4, 3, 1, 1), (5, 4, 2, 1, 1), (40, 16, 16, 0, 1), (300, 16, 64, 4, 8),
-    (1500, 8, 700, 2, 3), (3000, 1, 31, 0, 31), (2048, 16, 2047, 0, 1), (70, 3, 200, 5, 5)])
+    (1500, 8, 700, 2, 3), (3000, 1, 31, 0, 31), (2048, 16, 2047, 0, 1), (70, 3, 200, 5, 5),
+    (9000, 2, 1000, 3, 2), (20000, 1, 15000, 1, 1)])
 def test_evict(hip, width, bs, budget, first, last):
     g = rng(width + budget)
     lens = np.concatenate([[0, 1, width * bs, width * bs - bs + 1],
