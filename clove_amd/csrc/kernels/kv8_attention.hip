@@ -203,6 +203,61 @@ __global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split
         reinterpret_cast<float2 *>(a.ws + p.row_ml_at)[rh] = make_float2(top, inv);
 }
 
+// The same for tiles of many rows with few pieces: a thread joins four dims of a
+// row, all the loads of a workgroup run along the rows.
+__global__ void __launch_bounds__(256) kv8_join_rows_kernel(Kv8Attention a, Kv8Split p) {
+    const Kv8Args &c = a.c;
+    const int D = c.head_dim, H = c.num_heads, G = a.q_heads / H, D4 = D / 4;
+    const int groups = (p.stored * D4 + blockDim.x - 1) / blockDim.x;
+    const int h = blockIdx.x % H, slot = blockIdx.x / H / groups;
+    const int x = (int)(blockIdx.x / H % groups) * blockDim.x + threadIdx.x;
+    const int *starts = reinterpret_cast<const int *>(a.ws + p.start_at);
+    const int share = starts[0], start = starts[1 + (size_t)slot * (H / p.hw) + h / p.hw];
+    int item;
+    const int b = kv8_slot(c, slot, p.tile, G, 1, &item);
+    Kv8Tile T;
+    if (!kv8_tile_of(c, G, b, item, p.tile, &T) || T.high <= 0) return;
+    const int end = start + kv8_steps(T.high, p.step), w0 = start / share;
+    const int np = (end - 1) / share - w0 + 1;
+    const int u = x / D4, d4 = x - u * D4;
+    if (np == 1 || u >= T.rows) return;  // written whole, or no row
+    const size_t row = (size_t)(h % p.hw) * p.stored + u, per_piece = (size_t)p.hw * p.stored;
+    const size_t first = (2 * w0 + (start != w0 * share ? 1 : 0)) * per_piece + row;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.ws + p.ml_at);
+    const cl_f4 *o = reinterpret_cast<const cl_f4 *>(a.ws + p.o_at);
+    float top = -INFINITY, l = 0.0f;
+    cl_f4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < np; i0 += 2) {
+        float2 v[2];
+        cl_f4 y[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = min(i0 + j, np - 1);
+            const size_t at = i == 0 ? first : 2 * (w0 + i) * per_piece + row;
+            v[j] = ml[at];
+            y[j] = o[at * D4 + d4];
+        }
+        if (i0 + 1 >= np) v[1].x = -INFINITY;
+        const float t = fmaxf(top, fmaxf(v[0].x, v[1].x));
+        const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - t);
+        l *= f;
+        sum *= f;
+        top = t;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (v[j].x != -INFINITY) {
+                const float fj = __builtin_amdgcn_exp2f(v[j].x - t);
+                l = fmaf(v[j].y, fj, l);
+                sum += y[j] * fj;
+            }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const size_t rh = (size_t)(T.first + (T.r0 + u) / G) * a.q_heads + h * G + (T.r0 + u) % G;
+    reinterpret_cast<cl_f4 *>(a.out)[rh * D4 + d4] = sum * inv;
+    if (d4 == 0 && a.w_out)
+        reinterpret_cast<float2 *>(a.ws + p.row_ml_at)[rh] = make_float2(top, inv);
+}
+
 // The weight of each block from the sums stored on the way: lanes take 64
 // blocks, the waves a sequence's rows and heads in turn.
 __global__ void __launch_bounds__(1024) kv8_weights_kernel(Kv8Attention a, Kv8Split p) {
@@ -339,9 +394,13 @@ void kv8_attention(const Kv8Attention &a, int cus, hipStream_t s) {
         const unsigned tiles = (unsigned)kv8_slots(c, p.tile, a.q_heads / c.num_heads, 1) * c.num_heads;
         // pieces to a tile: 2 on the average where there are as many tiles as runs
         const int pieces = p.grid * p.hw / (int)tiles + 1;
-        const int per = pieces <= 8 ? 1 : pieces <= 32 ? 4 : 16;
-        const int waves = std::max(per, std::min(4, p.stored)), rows = waves / per;
-        kv8_join_kernel<<<tiles * ((p.stored + rows - 1) / rows), 64 * waves, 0, s>>>(a, p, per);
+        if (pieces <= 8) {
+            const int n = p.stored * c.head_dim / 4, threads = std::min(256, (n + 63) / 64 * 64);
+            kv8_join_rows_kernel<<<tiles * ((n + threads - 1) / threads), threads, 0, s>>>(a, p);
+        } else {
+            const int per = pieces <= 32 ? 4 : 16, rows = 4 / per > 0 ? 4 / per : 1;
+            kv8_join_kernel<<<tiles * ((p.stored + rows - 1) / rows), 64 * per * rows, 0, s>>>(a, p, per);
+        }
     }
     if (weights && p.kind == KV8_TILE)
         kv8_tile_weights(a, p, s);

@@ -8,6 +8,8 @@
 // memory meanwhile.  The products are those of kv8_stream.hip (S^T = K Q^T with
 // q, O^T = V^T P^T with P, as three bf16 pieces each), and an operand read from
 // LDS feeds 3 * NR MFMAs.
+#include <type_traits>
+
 #include "bf16x3.h"
 #include "kv8.h"
 #include "wave.h"
@@ -59,11 +61,13 @@ __device__ __forceinline__ int fill_table(const Kv8Args &c, int b, int h, int c0
     return bad;
 }
 
-template <int DP, int NR>
+// FULL: head_dim = DP; else MFMA steps and blocks past it are left out.
+template <int DP, int NR, bool FULL>
 __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p) {
     constexpr int KI = DP / 32;               // MFMA steps of q . k
     constexpr int KB = DP > 128 ? 32 : 64;    // tokens of a step
     constexpr int JB = DP / 16;               // 16-dim blocks of O^T
+    constexpr int JG = FULL ? 4 : 2;          // of them at a time
     constexpr int PK = 2 * DP + 16, PV = 2 * KB + 16;  // LDS pitches: no bank conflicts
     constexpr int NK = KB * DP / 16 / 256;    // 16-byte pieces of keys a thread stages
     constexpr int JV = DP * KB / 4 / 256;     // dims of four tokens' values a thread stages
@@ -250,6 +254,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                         for (int u = 0; u < 2; ++u) s[cc][u] = (cl_f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int i = 0; i < KI; ++i) {
+                        if (!FULL && 32 * i >= D) break;
                         u4 kf[2];
 #pragma unroll
                         for (int u = 0; u < 2; ++u)
@@ -316,10 +321,11 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                         }
                     }
 #pragma unroll
-                    for (int jb = 0; jb < JB; jb += 4) {
-                        u4 v[4];
+                    for (int jb = 0; jb < JB; jb += JG) {
+                        if (!FULL && 16 * jb >= D) break;
+                        u4 v[JG];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
+                        for (int i = 0; i < JG; ++i)
                             v[i] = *reinterpret_cast<const u4 *>(
                                 &sV[buf][(16 * (jb + i) + r) * PV + 64 * sub + 16 * q]);
 #pragma unroll
@@ -327,7 +333,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
 #pragma unroll
                             for (int cc = 0; cc < NR; ++cc)
 #pragma unroll
-                                for (int i = 0; i < 4; ++i)
+                                for (int i = 0; i < JG; ++i)
                                     o[cc][jb + i] = mfma(v[i], pf[cc][x], o[cc][jb + i]);
                     }
                 }
@@ -476,7 +482,8 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
 #pragma unroll
             for (int u = 0; u < 4; ++u) s[cc][u] = (cl_f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < KI; ++i)
+        for (int i = 0; i < KI; ++i) {
+            if (32 * i >= D) break;
 #pragma unroll
             for (int x = 2; x >= 0; --x)
 #pragma unroll
@@ -485,6 +492,7 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
 #pragma unroll
                     for (int u = 0; u < 4; ++u) s[cc][u] = mfma(kf[u][i], qf, s[cc][u]);
                 }
+        }
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
             const float2 ml = s_ml[buf][16 * cc + r];
@@ -547,16 +555,23 @@ __global__ void __launch_bounds__(1024) block_weights_kernel(Kv8Attention a, Kv8
 
 void kv8_tiles(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
     const unsigned grid = p.grid + kv8_zero_grid(a.c);
-    if (p.dp == 256)
-        tile_kernel<256, 1><<<grid, 256, 0, s>>>(a, p);
-    else if (p.dp == 128 && p.tile == 128)
-        tile_kernel<128, 2><<<grid, 256, 0, s>>>(a, p);
-    else if (p.dp == 128)
-        tile_kernel<128, 1><<<grid, 256, 0, s>>>(a, p);
-    else if (p.tile == 128)
-        tile_kernel<64, 2><<<grid, 256, 0, s>>>(a, p);
+    auto go = [&](auto full) {
+        constexpr bool F = decltype(full)::value;
+        if (p.dp == 256)
+            tile_kernel<256, 1, F><<<grid, 256, 0, s>>>(a, p);
+        else if (p.dp == 128 && p.tile == 128)
+            tile_kernel<128, 2, F><<<grid, 256, 0, s>>>(a, p);
+        else if (p.dp == 128)
+            tile_kernel<128, 1, F><<<grid, 256, 0, s>>>(a, p);
+        else if (p.tile == 128)
+            tile_kernel<64, 2, F><<<grid, 256, 0, s>>>(a, p);
+        else
+            tile_kernel<64, 1, F><<<grid, 256, 0, s>>>(a, p);
+    };
+    if (a.c.head_dim == p.dp)
+        go(std::true_type{});
     else
-        tile_kernel<64, 1><<<grid, 256, 0, s>>>(a, p);
+        go(std::false_type{});
 }
 
 void kv8_tile_weights(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
