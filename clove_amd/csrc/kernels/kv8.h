@@ -234,14 +234,17 @@ __device__ __forceinline__ Kv8Place kv8_find_place(const Kv8Args &c, int G, int 
                                                     Kv8Place *s_place) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int per = (c.num_seqs + 255) / 256;
-    auto steps = [&](int b) {
-        int sum = 0;
-        Kv8Tile t;
-        for (int item = 0; kv8_tile_of(c, G, b, item, tile, &t); ++item) sum += kv8_steps(t.high, step);
-        return sum * H;
+    // f(item, steps) for the tiles of sequence b
+    auto tiles = [&](int b, auto f) {
+        int first, n;
+        kv8_rows(c, b, &first, &n);
+        const int ctx = kv8_context(c, b);
+        for (int item = 0; item * tile < n * G; ++item)
+            f(item, kv8_steps(ctx - n + (min((item + 1) * tile, n * G) - 1) / G + 1, step) * H);
     };
     int mine = 0;
-    for (int b = tid * per; b < min((tid + 1) * per, c.num_seqs); ++b) mine += steps(b);
+    for (int b = tid * per; b < min((tid + 1) * per, c.num_seqs); ++b)
+        tiles(b, [&](int, int n) { mine += n; });
     int inc = mine;
     for (int o = 1; o < 64; o <<= 1) {
         const int up = __shfl_up(inc, o, 64);
@@ -256,19 +259,16 @@ __device__ __forceinline__ Kv8Place kv8_find_place(const Kv8Args &c, int G, int 
     const int share = max((total + grid - 1) / grid, 1);
     const int want = share * w;  // (the host keeps (tiles + grid) * steps below 2^31)
     if (want >= at && want < at + mine) {
-        for (int b = tid * per; b < min((tid + 1) * per, c.num_seqs); ++b) {
-            Kv8Tile t;
-            for (int item = 0; kv8_tile_of(c, G, b, item, tile, &t); ++item) {
-                const int n = kv8_steps(t.high, step);
-                if (want >= at && want < at + n * H) {
+        for (int b = tid * per; b < min((tid + 1) * per, c.num_seqs); ++b)
+            tiles(b, [&](int item, int n) {
+                if (want >= at && want < at + n) {
                     s_place->b = b;
                     s_place->item = item;
-                    s_place->h = (want - at) / n;
-                    s_place->step = (want - at) % n;
+                    s_place->h = (want - at) / (n / H);
+                    s_place->step = (want - at) % (n / H);
                 }
-                at += n * H;
-            }
-        }
+                at += n;
+            });
     }
     __syncthreads();
     Kv8Place p = *s_place;

@@ -252,6 +252,9 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                     for (int cc = 0; cc < NR; ++cc)
 #pragma unroll
                         for (int u = 0; u < 2; ++u) s[cc][u] = (cl_f4){0.f, 0.f, 0.f, 0.f};
+                    // raised priority over the MFMAs: the other wave of the SIMD does
+                    // its softmax, conversions and loads in the gaps
+                    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                     for (int i = 0; i < KI; ++i) {
                         if (!FULL && 32 * i >= D) break;
@@ -268,6 +271,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                                 for (int u = 0; u < 2; ++u)
                                     s[cc][u] = mfma(kf[u], qf[cc][i][x], s[cc][u]);
                     }
+                    __builtin_amdgcn_s_setprio(0);
                     if (bad || t0 + 32 > min(low, c1)) {
                         asm volatile("");  // (a branch, not selects that every step pays for)
 #pragma unroll
@@ -320,6 +324,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                             }
                         }
                     }
+                    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                     for (int jb = 0; jb < JB; jb += JG) {
                         if (!FULL && 16 * jb >= D) break;
@@ -337,6 +342,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                                     o[cc][jb + i] = mfma(v[i], pf[cc][x], o[cc][jb + i]);
                     }
                 }
+                __builtin_amdgcn_s_setprio(0);
                 if (more) store(kb + KB, buf ^ 1);
                 __syncthreads();
             }
