@@ -181,6 +181,7 @@ struct Kv8Split {
     size_t o_at, ml_at;      // piece 2w (+ 1: at the end of the run) of workgroup w: of hw
                              // heads `stored` sums over V [D], and (maximum, sum) pairs
     size_t start_at;         // share, then [slot, head / hw] first step of the tile
+    size_t declined_at;      // KV8_TILE: whether a workgroup leaves its run to the bf16 form
     size_t row_ml_at;        // (maximum, 1 / sum) of every row and query head
     size_t sums_at;          // [row, query head][groups] (sum, maximum) pairs
     size_t floats;

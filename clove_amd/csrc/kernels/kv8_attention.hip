@@ -355,6 +355,7 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
         p.ml_at = take((int64_t)2 * p.grid * p.hw * p.stored * 2);
         p.start_at = take(1 + tiles);
     }
+    if (p.kind == KV8_TILE) p.declined_at = take(p.grid);
     if (a.w_out) {
         p.row_ml_at = take(2 * rh);
         if (p.kind == KV8_STREAM) {

@@ -7,7 +7,10 @@
 // values as columns of eight tokens; the next step's codes are on their way from
 // memory meanwhile.  The products are those of kv8_stream.hip (S^T = K Q^T with
 // q, O^T = V^T P^T with P, as three bf16 pieces each), and an operand read from
-// LDS feeds 3 * NR MFMAs.
+// LDS feeds 3 * NR MFMAs.  Where the exponents of the tiles and the magnitudes
+// within each row of q lie close enough together, which is nearly always, f16
+// takes the place of bf16: two pieces of 11 bits do for q and P what three of 8
+// bits do, two thirds of the MFMAs.
 #include <type_traits>
 
 #include "bf16x3.h"
@@ -20,6 +23,9 @@ namespace k {
 namespace {
 
 constexpr int kChunk = 4096;  // tokens whose rows a workgroup's table holds
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ cl_f4 mfma(u4 a, u4 b, cl_f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a),
@@ -40,12 +46,47 @@ __device__ __forceinline__ void split_q(const cl_f4 (&x)[2], float scale, u4 (&w
     }
 }
 
+__device__ __forceinline__ cl_f4 mfma_half(u4 a, u4 b, cl_f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a),
+                                                  __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+template <bool HALF>
+__device__ __forceinline__ cl_f4 product(u4 a, u4 b, cl_f4 c) {
+    return HALF ? mfma_half(a, b, c) : mfma(a, b, c);
+}
+
+// Two codes times a power of two: as two bf16, or as two f16 (exact where the
+// result's bits are 2^-24 or more).
+template <bool HALF, bool HIGH>
+__device__ __forceinline__ unsigned widen(unsigned codes, float scale) {
+    if constexpr (HALF)
+        return __builtin_bit_cast(unsigned,
+                                  __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, HIGH));
+    else
+        return kv8_widen<HIGH>(codes, scale);
+}
+
+// Two floats as f16 and the rest of each as f16: off by at most 2^-23 of it, and
+// by 2^-25 where that is more.
+__device__ __forceinline__ void split_half(float a, float b, unsigned *w1, unsigned *w2) {
+    const unsigned h = __builtin_bit_cast(unsigned, __builtin_convertvector((f2){a, b}, h2));
+    float ra, rb;  // a - the low half of h, b - the high half
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(h), "v"(a));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+        : "=v"(rb)
+        : "v"(h), "v"(b));
+    *w1 = h;
+    *w2 = __builtin_bit_cast(unsigned, __builtin_convertvector((f2){ra, rb}, h2));
+}
+
 // The table of tokens [c0, c1), rounded up to whole steps: the row of each four
 // tokens' first and the scales of its key and value tile as bf16, 0 outside the
 // pool.  Tokens behind the end take the first place.  True: some are outside.
+// range (-1000s before): the keys' largest exponent and their least one's
+// negative, then the values'.
 __device__ __forceinline__ int fill_table(const Kv8Args &c, int b, int h, int c0, int c1,
-                                          int step, uint2 *table) {
-    int bad = 0;
+                                          int step, uint2 *table, int *range = nullptr) {
+    int bad = 0, ends[4] = {-1000, -1000, -1000, -1000};
     for (int i = threadIdx.x; i < (c1 - c0 + step - 1) / step * (step / 4); i += 256) {
         const int t = c0 + 4 * i < c1 ? c0 + 4 * i : c0;
         const int64_t id = kv8_block(c, b, t / c.block_size, h == 0);
@@ -54,15 +95,30 @@ __device__ __forceinline__ int fill_table(const Kv8Args &c, int b, int h, int c0
             e.x = (unsigned)((id * c.num_heads + h) * c.block_size + t % c.block_size);
             e.y = __float_as_uint(kv8_scale(c.exps[kv8_tile(c, 0, id, h)])) |
                   __float_as_uint(kv8_scale(c.exps[kv8_tile(c, 1, id, h)])) >> 16;
+            const int ke = (int)(e.y >> 23) - 127, ve = (int)(e.y >> 7 & 255) - 127;
+            ends[0] = max(ends[0], ke);
+            ends[1] = max(ends[1], -ke);
+            ends[2] = max(ends[2], ve);
+            ends[3] = max(ends[3], -ve);
         }
         bad |= id < 0;
         table[i] = e;
+    }
+    if (range) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) ends[j] = max(ends[j], __shfl_xor(ends[j], o, 64));
+            if ((threadIdx.x & 63) == 0) atomicMax(&range[j], ends[j]);
+        }
     }
     return bad;
 }
 
 // FULL: head_dim = DP; else MFMA steps and blocks past it are left out.
-template <int DP, int NR, bool FULL>
+// HALF: f16 pieces, two of each; a workgroup whose tiles or rows do not let it
+// leaves its run to the bf16 form (p.declined), which otherwise finds nothing to do.
+template <int DP, int NR, bool FULL, bool HALF>
 __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p) {
     constexpr int KI = DP / 32;               // MFMA steps of q . k
     constexpr int KB = DP > 128 ? 32 : 64;    // tokens of a step
@@ -78,11 +134,17 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
     const int H = c.num_heads, G = a.q_heads / H, D = c.head_dim, bs = c.block_size;
     __shared__ uint2 table[kChunk / 4];
     __shared__ __attribute__((aligned(16))) uint8_t sK[2][KB * PK], sV[2][DP * PV];
-    __shared__ int s_wave[4];
+    __shared__ int s_wave[4], s_range[6];  // (the last two: bad, wide)
     __shared__ Kv8Place s_place;
 
     if ((int)blockIdx.x >= p.grid) {
         kv8_zero_rows(a, blockIdx.x - p.grid);
+        return;
+    }
+    int *declined = reinterpret_cast<int *>(a.ws + p.declined_at) + blockIdx.x;
+    if (HALF) {
+        if (tid == 0) *declined = 0;
+    } else if (*declined == 0) {
         return;
     }
     Kv8Place at;
@@ -118,10 +180,19 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                 [1 + (size_t)(kv8_first_slot(c, at.b, p.tile, G, 1) + at.item) * H + h] =
                     at.share * (int)blockIdx.x + (run - left);
 
-        // this wave's rows: q in pieces, and the tokens each row sees
-        u4 qf[NR][KI][3];
-        int lim[NR];
+        // this wave's rows, and the tokens each sees
+        int lim[NR], lift[NR];
+        bool wide = false;
         size_t rowhead[NR];
+        auto q_of = [&](int cc, int i, cl_f4 (&x)[2]) {
+            const int d = 32 * i + 8 * q;
+            x[0] = x[1] = (cl_f4){0.f, 0.f, 0.f, 0.f};
+            if (16 * (NR * wave + cc) + r < T.rows && d < D) {
+                const cl_f4 *from = reinterpret_cast<const cl_f4 *>(a.q + rowhead[cc] * D + d);
+                x[0] = from[0] * (a.scale * kLog2e);  // (weights are powers of two)
+                x[1] = from[1] * (a.scale * kLog2e);
+            }
+        };
 #pragma unroll
         for (int cc = 0; cc < NR; ++cc) {
             const int u = 16 * (NR * wave + cc) + r;
@@ -129,16 +200,6 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
             const int tok = (T.r0 + (ok ? u : 0)) / G, g = (T.r0 + (ok ? u : 0)) % G;
             lim[cc] = ok ? min(t_end, T.ctx - T.n + tok + 1) : 0;
             rowhead[cc] = (size_t)(T.first + tok) * a.q_heads + h * G + g;
-#pragma unroll
-            for (int i = 0; i < KI; ++i) {
-                const int d = 32 * i + 8 * q;
-                cl_f4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-                if (ok && d < D) {
-                    x[0] = reinterpret_cast<const cl_f4 *>(a.q + rowhead[cc] * D + d)[0];
-                    x[1] = reinterpret_cast<const cl_f4 *>(a.q + rowhead[cc] * D + d)[1];
-                }
-                split_q(x, a.scale * kLog2e, qf[cc][i]);
-            }
         }
         const int u0 = 16 * NR * wave;  // tokens that all the wave's rows see, and that any does
         const int low = u0 < T.rows ? T.ctx - T.n + (T.r0 + u0) / G + 1 : 0;
@@ -165,9 +226,91 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
 
         for (int c0 = s0 * KB; c0 < t_end; c0 += kChunk) {
             const int c1 = min(c0 + kChunk, t_end);
+            if (tid < 6) s_range[tid] = tid < 4 ? -1000 : 0;
             __syncthreads();  // the table and tiles before are done with
-            const int bad = __syncthreads_or(fill_table(c, at.b, h, c0, c1, KB, table));
-
+            if (__any(fill_table(c, at.b, h, c0, c1, KB, table, s_range)) && lane == 0)
+                s_range[4] = 1;
+            if (HALF && c0 == s0 * KB) {
+                // A row is lifted to 2^14 .. 2^15.  Elements below 2^-17 of its largest
+                // then lose bits; a few are chance and far below what the row's
+                // scores round by, but where they are a quarter of the row, its
+                // largest may meet keys of 0 and they be all that counts.
+#pragma unroll
+                for (int cc = 0; cc < NR; ++cc) {
+                    cl_f4 x[KI][2];
+                    float most = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < KI; ++i) {
+                        q_of(cc, i, x[i]);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float y = fabsf(x[i][e / 4][e & 3]);
+                            if (kv8_finite(y)) most = fmaxf(most, y);
+                        }
+                    }
+                    most = fmaxf(most, __shfl_xor(most, 16, 64));
+                    most = fmaxf(most, __shfl_xor(most, 32, 64));
+                    int small = 0;
+#pragma unroll
+                    for (int i = 0; i < KI; ++i)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float y = fabsf(x[i][e / 4][e & 3]);
+                            small += y > 0.0f && y < most * 0x1p-17f;
+                        }
+                    small += __shfl_xor(small, 16, 64);
+                    small += __shfl_xor(small, 32, 64);
+                    lift[cc] = min(14 + 127 - (int)(__float_as_uint(most) >> 23), 100);
+                    if (lift[cc] < -60 || 4 * small >= D) s_range[5] = 1;
+                }
+            }
+            __syncthreads();
+            const bool bad = s_range[4];
+            if (HALF && c0 == s0 * KB) wide = s_range[5];
+            // f16 holds codes times 2^(exponent - the largest + 7) exactly over 22
+            // octaves of the tiles' exponents; with rows and weights lifted likewise,
+            // two pieces of each do what three bf16 ones do.
+            const int ke = s_range[0], ve = s_range[2];
+            if (HALF && (wide || ke > 60 || ke + s_range[1] > 22 || ve > 60 ||
+                         ve + s_range[3] > 22 || ke == -1000)) {
+                if (tid == 0) *declined = 1;
+                return;
+            }
+            u4 qf[NR][KI][HALF ? 2 : 3];
+#pragma unroll
+            for (int cc = 0; cc < NR; ++cc)
+#pragma unroll
+                for (int i = 0; i < KI; ++i) {
+                    cl_f4 x[2];
+                    q_of(cc, i, x);
+                    if constexpr (HALF) {
+                        const float up = kv8_pow2(lift[cc]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            unsigned w1, w2;
+                            split_half(x[e / 2][2 * (e & 1)] * up,
+                                       x[e / 2][2 * (e & 1) + 1] * up, &w1, &w2);
+                            qf[cc][i][0][e] = w1;
+                            qf[cc][i][1][e] = w2;
+                        }
+                    } else {
+                        split_q(x, 1.0f, qf[cc][i]);
+                    }
+                }
+            const float k_down = HALF ? kv8_pow2(7 - ke) : 1.0f;
+            const float v_down = HALF ? kv8_pow2(7 - ve) : 1.0f;
+            float down[NR];  // a score's factor
+#pragma unroll
+            for (int cc = 0; cc < NR; ++cc)
+                down[cc] = HALF ? kv8_pow2(ke - 7) * kv8_pow2(-lift[cc]) : 1.0f;
+            auto rescale = [&](float f) {
+                if (HALF)
+#pragma unroll
+                    for (int cc = 0; cc < NR; ++cc)
+#pragma unroll
+                        for (int jb = 0; jb < JB; ++jb) o[cc][jb] *= f;
+            };
+            rescale(v_down);
             u4 rk[NK];
             unsigned rv[4][JV / 4];
             float ksc[NK], vsc;
@@ -177,12 +320,14 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                     const int x = tid + 256 * i, key = x / (DP / 16), d = x % (DP / 16) * 16;
                     const uint2 e = table[(kb - c0 + key) >> 2];
                     ksc[i] = __uint_as_float(e.y & 0xffff0000u);
+                    if (HALF) ksc[i] *= k_down;
                     // (past D, where q is 0, the row's first dims stand in)
                     rk[i] = *reinterpret_cast<const u4 *>(
                         c.codes + (size_t)(e.x + (key & 3)) * D + (d < D ? d : 0));
                 }
                 const uint2 e = table[((kb - c0) >> 2) + vquad];
                 vsc = __uint_as_float(e.y << 16);
+                if (HALF) vsc *= v_down;
                 const uint8_t *row = vbase + (size_t)e.x * D;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -202,8 +347,8 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                     u4 w[2];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        w[e / 2][2 * (e & 1)] = kv8_widen<false>(rk[i][e], ksc[i]);
-                        w[e / 2][2 * (e & 1) + 1] = kv8_widen<true>(rk[i][e], ksc[i]);
+                        w[e / 2][2 * (e & 1)] = widen<HALF, false>(rk[i][e], ksc[i]);
+                        w[e / 2][2 * (e & 1) + 1] = widen<HALF, true>(rk[i][e], ksc[i]);
                     }
                     u4 *to = reinterpret_cast<u4 *>(&sK[buf][key * PK + 2 * d]);
                     to[0] = w[0];
@@ -225,7 +370,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                         unsigned w[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            w[i] = hi ? kv8_widen<true>(rv[i][e], vsc) : kv8_widen<false>(rv[i][e], vsc);
+                            w[i] = hi ? widen<HALF, true>(rv[i][e], vsc) : widen<HALF, false>(rv[i][e], vsc);
                         uint8_t *to = &sV[buf][(vdim + 4 * e + 2 * hi) * PV + 2 * vpos];
                         *reinterpret_cast<uint2 *>(to) =
                             make_uint2(__builtin_amdgcn_perm(w[1], w[0], 0x05040100u),
@@ -264,12 +409,12 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                             kf[u] = *reinterpret_cast<const u4 *>(
                                 &sK[buf][(32 * sub + 16 * u + r) * PK + 64 * i + 16 * q]);
 #pragma unroll
-                        for (int x = 2; x >= 0; --x)
+                        for (int x = HALF ? 1 : 2; x >= 0; --x)
 #pragma unroll
                             for (int cc = 0; cc < NR; ++cc)
 #pragma unroll
                                 for (int u = 0; u < 2; ++u)
-                                    s[cc][u] = mfma(kf[u], qf[cc][i][x], s[cc][u]);
+                                    s[cc][u] = product<HALF>(kf[u], qf[cc][i][x], s[cc][u]);
                     }
                     __builtin_amdgcn_s_setprio(0);
                     if (bad || t0 + 32 > min(low, c1)) {
@@ -293,12 +438,16 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                         for (int u = 0; u < 2; ++u)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) top = fmaxf(top, s[cc][u][i]);
-                        if (__any(top > m[cc] + kKv8Slack)) {
+                        // weights are up to 2^8 with bf16 pieces, and with f16 ones, which
+                        // hold them down to 2^-40 of that, up to 2^15
+                        constexpr float kMost = HALF ? 15.0f : kKv8Slack, kAim = HALF ? 7.0f : 0.0f;
+                        if (HALF) top *= down[cc];
+                        if (__any(top > m[cc] + kMost)) {
                             // a row moves its maximum by its own scores alone, so
                             // that its bits do not depend on the rows beside it
                             top = fmaxf(top, __shfl_xor(top, 16, 64));
                             top = fmaxf(top, __shfl_xor(top, 32, 64));
-                            const float m_new = top > m[cc] + kKv8Slack ? top : m[cc];
+                            const float m_new = top > m[cc] + kMost ? top - kAim : m[cc];
                             const float f0 =
                                 m_new == m[cc] ? 1.0f : __builtin_amdgcn_exp2f(m[cc] - m_new);
                             l[cc] *= f0;
@@ -311,13 +460,17 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                         for (int u = 0; u < 2; ++u) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                s[cc][u][i] = __builtin_amdgcn_exp2f(s[cc][u][i] - mz);
+                                s[cc][u][i] = __builtin_amdgcn_exp2f(
+                                    HALF ? fmaf(s[cc][u][i], down[cc], -mz) : s[cc][u][i] - mz);
                             l[cc] += hsum4(s[cc][u]);
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                unsigned w1, w2, w3;
-                                split_pair<false>(s[cc][u][2 * e], s[cc][u][2 * e + 1], &w1, &w2,
-                                                  &w3);
+                                unsigned w1, w2, w3 = 0;
+                                if constexpr (HALF)
+                                    split_half(s[cc][u][2 * e], s[cc][u][2 * e + 1], &w1, &w2);
+                                else
+                                    split_pair<false>(s[cc][u][2 * e], s[cc][u][2 * e + 1], &w1,
+                                                      &w2, &w3);
                                 pf[cc][0][2 * u + e] = w1;
                                 pf[cc][1][2 * u + e] = w2;
                                 pf[cc][2][2 * u + e] = w3;
@@ -334,18 +487,20 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                             v[i] = *reinterpret_cast<const u4 *>(
                                 &sV[buf][(16 * (jb + i) + r) * PV + 64 * sub + 16 * q]);
 #pragma unroll
-                        for (int x = 2; x >= 0; --x)
+                        for (int x = HALF ? 1 : 2; x >= 0; --x)
 #pragma unroll
                             for (int cc = 0; cc < NR; ++cc)
 #pragma unroll
                                 for (int i = 0; i < JG; ++i)
-                                    o[cc][jb + i] = mfma(v[i], pf[cc][x], o[cc][jb + i]);
+                                    o[cc][jb + i] = product<HALF>(v[i], pf[cc][x], o[cc][jb + i]);
                     }
                 }
                 __builtin_amdgcn_s_setprio(0);
                 if (more) store(kb + KB, buf ^ 1);
                 __syncthreads();
             }
+            if (HALF) rescale(kv8_pow2(ve - 7));
+            // (bf16: a group at a time, which its third pieces leave registers for)
         }
 
         const bool whole = s0 == 0 && s1 == all;
@@ -560,24 +715,27 @@ __global__ void __launch_bounds__(1024) block_weights_kernel(Kv8Attention a, Kv8
 }  // namespace
 
 void kv8_tiles(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
-    const unsigned grid = p.grid + kv8_zero_grid(a.c);
-    auto go = [&](auto full) {
-        constexpr bool F = decltype(full)::value;
+    auto go = [&](auto full, auto half) {
+        constexpr bool F = decltype(full)::value, HALF = decltype(half)::value;
+        const unsigned grid = p.grid + (HALF ? kv8_zero_grid(a.c) : 0);
         if (p.dp == 256)
-            tile_kernel<256, 1, F><<<grid, 256, 0, s>>>(a, p);
+            tile_kernel<256, 1, F, HALF><<<grid, 256, 0, s>>>(a, p);
         else if (p.dp == 128 && p.tile == 128)
-            tile_kernel<128, 2, F><<<grid, 256, 0, s>>>(a, p);
+            tile_kernel<128, 2, F, HALF><<<grid, 256, 0, s>>>(a, p);
         else if (p.dp == 128)
-            tile_kernel<128, 1, F><<<grid, 256, 0, s>>>(a, p);
+            tile_kernel<128, 1, F, HALF><<<grid, 256, 0, s>>>(a, p);
         else if (p.tile == 128)
-            tile_kernel<64, 2, F><<<grid, 256, 0, s>>>(a, p);
+            tile_kernel<64, 2, F, HALF><<<grid, 256, 0, s>>>(a, p);
         else
-            tile_kernel<64, 1, F><<<grid, 256, 0, s>>>(a, p);
+            tile_kernel<64, 1, F, HALF><<<grid, 256, 0, s>>>(a, p);
     };
-    if (a.c.head_dim == p.dp)
-        go(std::true_type{});
-    else
-        go(std::false_type{});
+    if (a.c.head_dim == p.dp) {
+        go(std::true_type{}, std::true_type{});
+        go(std::true_type{}, std::false_type{});
+    } else {
+        go(std::false_type{}, std::true_type{});
+        go(std::false_type{}, std::false_type{});
+    }
 }
 
 void kv8_tile_weights(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
