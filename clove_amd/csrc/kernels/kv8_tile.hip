@@ -561,8 +561,7 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
     kv8_rows(c, b, &first, &n);
     const int ctx = kv8_context(c, b), c1 = min(c0 + 256, ctx);
     if (part < 0 || part * kPart >= n * G || c0 >= c1) return;
-    fill_table(c, b, 0, c0, c1, 256, table);
-    __syncthreads();
+    const int bad = __syncthreads_or(fill_table(c, b, 0, c0, c1, 256, table));
     // the keys: token 16u + r of the wave's, dims 32i + 8q .. + 7
     u4 kf[4][KI];
     bool in[4];
@@ -659,14 +658,21 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
             const float2 ml = s_ml[buf][16 * cc + r];
             const float mz = ml.x == -INFINITY ? 0.0f : ml.x;
             const int lim = s_lim[buf][16 * cc + r];
+            // (rows that no query is count nothing by their 0)
+            if (bad || c0 + 64 * wave + 64 > min(c1, ctx - n + u0 / G + 1)) {
+                asm volatile("");  // (a branch, not selects that every step pays for)
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!in[u] || c0 + 64 * wave + 16 * u + 4 * q + i >= lim)
+                            s[cc][u][i] = -INFINITY;
+            }
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int t = c0 + 64 * wave + 16 * u + 4 * q + i;
-                    const float w = __builtin_amdgcn_exp2f(s[cc][u][i] - mz) * ml.y;
-                    sum[u][i] += in[u] && t < lim ? w : 0.0f;
-                }
+                for (int i = 0; i < 4; ++i)
+                    sum[u][i] = fmaf(__builtin_amdgcn_exp2f(s[cc][u][i] - mz), ml.y, sum[u][i]);
         }
         if (u0 + 32 < u_end) store(buf ^ 1);
         __syncthreads();
