@@ -114,6 +114,14 @@ __global__ void __launch_bounds__(256) kv8_weights_any_kernel(Kv8Attention a, co
     if (threadIdx.x == 0) a.w_out[at] = a.w_in[at] + part[0];
 }
 
+// The pieces of a tile and the first workgroup that has one.  Where row_starts
+// decrease, tiles may share a slot and its start: the pieces stay those there are.
+__device__ __forceinline__ int kv8_pieces(const Kv8Split &p, int share, int start, int steps,
+                                          int *w0) {
+    *w0 = min(max(start / share, 0), p.grid - 1);
+    return min((int)(((unsigned)start + steps - 1) / (unsigned)share), p.grid - 1) - *w0 + 1;
+}
+
 // Joins the pieces of the tiles that were cut: `per` waves take the pieces of a
 // row in turn, eight on their way at a time, and a lane holds up to four dims.
 __global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split p, int per) {
@@ -130,9 +138,9 @@ __global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split
     const int b = kv8_slot(c, slot, p.tile, G, 1, &item);
     Kv8Tile T;
     if (!kv8_tile_of(c, G, b, item, p.tile, &T) || T.high <= 0) return;
-    const int end = start + kv8_steps(T.high, p.step), w0 = start / share;
-    const int np = (end - 1) / share - w0 + 1;
-    if (np == 1) return;  // written whole
+    int w0;
+    const int np = kv8_pieces(p, share, start, kv8_steps(T.high, p.step), &w0);
+    if (np <= 1) return;  // written whole
     float top = -INFINITY, l = 0.0f, x[4] = {0.f, 0.f, 0.f, 0.f};
     if (u < T.rows) {
         // the first piece ends its workgroup's run unless the run begins with it
@@ -217,10 +225,10 @@ __global__ void __launch_bounds__(256) kv8_join_rows_kernel(Kv8Attention a, Kv8S
     const int b = kv8_slot(c, slot, p.tile, G, 1, &item);
     Kv8Tile T;
     if (!kv8_tile_of(c, G, b, item, p.tile, &T) || T.high <= 0) return;
-    const int end = start + kv8_steps(T.high, p.step), w0 = start / share;
-    const int np = (end - 1) / share - w0 + 1;
+    int w0;
+    const int np = kv8_pieces(p, share, start, kv8_steps(T.high, p.step), &w0);
     const int u = x / D4, d4 = x - u * D4;
-    if (np == 1 || u >= T.rows) return;  // written whole, or no row
+    if (np <= 1 || u >= T.rows) return;  // written whole, or no row
     const size_t row = (size_t)(h % p.hw) * p.stored + u, per_piece = (size_t)p.hw * p.stored;
     const size_t first = (2 * w0 + (start != w0 * share ? 1 : 0)) * per_piece + row;
     const float2 *ml = reinterpret_cast<const float2 *>(a.ws + p.ml_at);

@@ -22,8 +22,6 @@ namespace k {
 
 namespace {
 
-constexpr int kChunk = 4096;  // tokens whose rows a workgroup's table holds
-
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
@@ -127,6 +125,8 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
     constexpr int PK = 2 * DP + 16, PV = 2 * KB + 16;  // LDS pitches: no bank conflicts
     constexpr int NK = KB * DP / 16 / 256;    // 16-byte pieces of keys a thread stages
     constexpr int JV = DP * KB / 4 / 256;     // dims of four tokens' values a thread stages
+    // tokens whose rows the table holds (two workgroups to a CU in any case)
+    constexpr int kChunk = DP > 128 ? 2048 : 4096;
     static_assert(NK >= 1 && (JV == 4 || JV == 8), "256 threads stage a step");
     const Kv8Args &c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
     const int H = c.num_heads, G = a.q_heads / H, D = c.head_dim, bs = c.block_size;
     __shared__ uint2 table[kChunk / 4];
     __shared__ __attribute__((aligned(16))) uint8_t sK[2][KB * PK], sV[2][DP * PV];
-    __shared__ int s_wave[4], s_range[6];  // (the last two: bad, wide)
+    __shared__ int s_wave[4], s_range[6];  // (the last two: bad; lost, as a float's bits)
     __shared__ Kv8Place s_place;
 
     if ((int)blockIdx.x >= p.grid) {
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
 
         // this wave's rows, and the tokens each sees
         int lim[NR], lift[NR];
-        bool wide = false;
+        float lost = 0.0f;
         size_t rowhead[NR];
         auto q_of = [&](int cc, int i, cl_f4 (&x)[2]) {
             const int d = 32 * i + 8 * q;
@@ -232,9 +232,8 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                 s_range[4] = 1;
             if (HALF && c0 == s0 * KB) {
                 // A row is lifted to 2^14 .. 2^15.  Elements below 2^-17 of its largest
-                // then lose bits; a few are chance and far below what the row's
-                // scores round by, but where they are a quarter of the row, its
-                // largest may meet keys of 0 and they be all that counts.
+                // then lose bits: each is off by up to 2^-39 of the largest, `lost`
+                // times 2^-39 together.
 #pragma unroll
                 for (int cc = 0; cc < NR; ++cc) {
                     cl_f4 x[KI][2];
@@ -261,18 +260,22 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                     small += __shfl_xor(small, 16, 64);
                     small += __shfl_xor(small, 32, 64);
                     lift[cc] = min(14 + 127 - (int)(__float_as_uint(most) >> 23), 100);
-                    if (lift[cc] < -60 || 4 * small >= D) s_range[5] = 1;
+                    if (q == 0)
+                        atomicMax(&s_range[5],
+                                  __float_as_int(lift[cc] < -60 ? INFINITY : small * most));
                 }
             }
             __syncthreads();
             const bool bad = s_range[4];
-            if (HALF && c0 == s0 * KB) wide = s_range[5];
+            if (HALF && c0 == s0 * KB) lost = __int_as_float(s_range[5]);
             // f16 holds codes times 2^(exponent - the largest + 7) exactly over 22
             // octaves of the tiles' exponents; with rows and weights lifted likewise,
-            // two pieces of each do what three bf16 ones do.
+            // two pieces of each do what three bf16 ones do, if what the rows lost
+            // moves no score (base 2) by more than 2^-22, a quarter of a weight's ulp.
             const int ke = s_range[0], ve = s_range[2];
-            if (HALF && (wide || ke > 60 || ke + s_range[1] > 22 || ve > 60 ||
-                         ve + s_range[3] > 22 || ke == -1000)) {
+            if (HALF && (ke == -1000 || ke > 60 || ke + s_range[1] > 22 || ve > 60 ||
+                         ve + s_range[3] > 22 ||
+                         lost * (0x1p-17f * kE4m3Max) * kv8_pow2(ke) > 1.0f)) {
                 if (tid == 0) *declined = 1;
                 return;
             }
@@ -438,9 +441,9 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                         for (int u = 0; u < 2; ++u)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) top = fmaxf(top, s[cc][u][i]);
-                        // weights are up to 2^8 with bf16 pieces, and with f16 ones, which
-                        // hold them down to 2^-40 of that, up to 2^15
-                        constexpr float kMost = HALF ? 15.0f : kKv8Slack, kAim = HALF ? 7.0f : 0.0f;
+                        // weights are up to 2^8 with bf16 pieces; with f16 ones, which are
+                        // off by 2^-25 or less, the largest is 2^10 .. 2^15
+                        constexpr float kMost = HALF ? 15.0f : kKv8Slack, kAim = HALF ? 10.0f : 0.0f;
                         if (HALF) top *= down[cc];
                         if (__any(top > m[cc] + kMost)) {
                             // a row moves its maximum by its own scores alone, so
@@ -500,7 +503,6 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                 __syncthreads();
             }
             if (HALF) rescale(kv8_pow2(ve - 7));
-            // (bf16: a group at a time, which its third pieces leave registers for)
         }
 
         const bool whole = s0 == 0 && s1 == all;

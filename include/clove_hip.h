@@ -253,9 +253,11 @@ CTensor clove_hip_paged_gather_indices(CTensor block_tables, CTensor context_len
  * row for each sequence (rows == B).  block_tables is int32 [B, max_blocks].
  *
  * Errors that only the device sees (a block id outside the pool, a context
- * past its table, row_starts that decrease or leave [0, rows]) skip the tokens
+ * past its table, row_starts that leave [0, rows] or decrease) skip the tokens
  * or rows concerned and are reported as CLOVE_HIP_ERR_RANGE by the next
- * synchronising call, as for the f32 cache. */
+ * synchronising call, as for the f32 cache.  Where row_starts decrease, rows may
+ * belong to two sequences or be missed: what any row of that call is given is
+ * then not specified. */
 
 /* Stores the rows' keys and values (f32 [rows, H*D]).  A tile's exponent is the
  * smallest e in [-60, 119] with |x| <= 448 * 2^e for what it holds; codes are

@@ -6,6 +6,8 @@ Codes and exponents are bit-determined (scaling by powers of two is exact and
 each element is rounded once), so they are compared exactly; attention within
 the bounds that kv8_ref.attention derives from its 32-bit arithmetic.
 """
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -332,6 +334,205 @@ def test_shared_blocks_and_repeats(hip):
         want, ww, tol, wtol = ref.attention(q, codes, exps, tables, lens, starts, weights=w)
         within(first[0], want, tol, "out")
         within(first[1], ww, wtol, "weights")
+
+
+@pytest.mark.parametrize("weighed", [False, True])
+@pytest.mark.parametrize("D,bs,H,Hq,rows_hi", [
+    # four heads to a workgroup
+    (64, 16, 16, 16, 1), (128, 8, 16, 32, 1), (112, 4, 16, 16, 1), (128, 16, 16, 16, 12),
+    (64, 16, 16, 16, 30),
+    # two
+    (256, 16, 8, 16, 1), (144, 16, 8, 8, 8), (128, 16, 8, 8, 40), (80, 32, 8, 16, 20)])
+def test_many_sequences_and_heads(hip, D, bs, H, Hq, rows_hi, weighed):
+    """Enough tiles that heads are taken together; one context in many pieces,
+    whose table of tokens is filled twice."""
+    g = rng(4000 + D + bs + Hq + rows_hi)
+    B = 70
+    rows = np.ones(B, np.int64) if rows_hi == 1 else g.integers(0, rows_hi + 1, B)
+    if rows_hi > 1:
+        rows[7] = rows_hi
+    lens = (rows + g.integers(0, 70, B)).astype(np.int32)
+    lens[3], lens[9] = 0, 2100 + bs
+    rows[3] = min(rows[3], 1)
+    tables, nb = ref.pool(g, lens, bs, -(-int(lens.max()) // bs))
+    codes, exps = ref.cache(g, nb, H, bs, D)
+    q = g.standard_normal((int(rows.sum()), Hq * D)).astype(np.float32)
+    check_attention(hip, q, codes, exps, tables, lens, None if rows_hi == 1 else ref.starts_of(rows),
+                    weights=g.random(tables.shape).astype(np.float32) if weighed else None)
+
+
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+def test_long_prompt_chunks(hip, D):
+    """Chunks far into contexts: several tables of tokens to a tile, tiles cut
+    over workgroups and joined."""
+    g = rng(D)
+    rows, past = np.array([70, 3, 41]), np.array([5000, 4096, 2040])
+    lens = (rows + past).astype(np.int32)
+    tables, nb = ref.pool(g, lens, 16, -(-5070 // 16))
+    codes, exps = ref.cache(g, nb, 1, 16, D)
+    q = g.standard_normal((int(rows.sum()), 2 * D)).astype(np.float32)
+    check_attention(hip, q, codes, exps, tables, lens, ref.starts_of(rows),
+                    weights=g.random(tables.shape).astype(np.float32))
+
+
+@pytest.mark.parametrize("kspan,vspan,top", [(22, 22, -5), (23, 0, -5), (0, 23, -5), (3, 3, 60),
+                                             (3, 3, 61), (3, 3, -57), (3, 3, 70)])
+@pytest.mark.parametrize("small,gap,every", [(0, 0, 2), (1, 20, 2), (40, 20, 2), (63, 20, 2),
+                                             (1, 24, 1), (1, 40, 1), (40, 40, 1)])
+def test_sizes_of_tiles_and_query_elements(hip, kspan, vspan, top, small, gap, every):
+    """Tiles whose exponents lie as far apart as 16-bit pieces hold and farther,
+    the largest and smallest exponents, and rows of which `small` elements are
+    2^gap below the others, with keys of zero at the large ones (in every other
+    token, or in all of them, where the small ones alone make the scores)."""
+    g = rng(100 * kspan + vspan + top + small + gap)
+    H, D, bs, n = 2, 64, 16, 150
+    lens = np.array([n], np.int32)
+    tables, nb = ref.pool(g, lens, bs, 10)
+    codes, exps = ref.cache(g, nb, H, bs, D)
+    exps[0] = top - g.integers(0, kspan + 1, exps[0].shape)
+    exps[1] = min(top, 100) - g.integers(0, vspan + 1, exps[1].shape)
+    exps[0, tables[0, :2]] = np.array([[top], [max(top - kspan, -60)]])
+    q = g.standard_normal((n, H * D)) * 2.0 ** (-9 - top + (gap if every == 1 else 0))
+    at = g.permutation(D)[:small]
+    q.reshape(n, H, D)[:, :, at] *= 2.0 ** -gap
+    codes[0][:, :, ::every][..., np.setdiff1d(np.arange(D), at)] = 0
+    check_attention(hip, q.astype(np.float32), codes, exps, tables, lens,
+                    np.array([0, n], np.int32), weights=np.zeros(tables.shape, np.float32))
+
+
+@pytest.mark.parametrize("rows", [1, 8, 60, 130])
+def test_a_token_that_takes_all_the_weight(hip, rows):
+    """A token 2^20 ahead of the others whose value is 0: what is left is the
+    small weights' sum."""
+    g = rng(43)
+    H, D, bs, n = 2, 64, 16, 200
+    lens = np.array([n], np.int32)
+    tables, nb = ref.pool(g, lens, bs, 13)
+    codes, exps = ref.cache(g, nb, H, bs, D)
+    exps[0] = -10
+    q = g.standard_normal((rows, H * D)).astype(np.float32)
+    q.reshape(rows, H, D)[:, :, 0] = 5.0
+    codes[0, :, :, :, 0] = 0
+    codes[0, tables[0, 2]] = 0
+    codes[1, tables[0, 2], :, 5] = 0
+    codes[0, tables[0, 2], :, 5, 0] = ref.encode(np.array(20 * np.log(2) / 5 * 64))
+    exps[0, tables[0, 2]] = -6
+    out = check_attention(hip, q, codes, exps, tables, lens, np.array([0, rows], np.int32),
+                          scale=1.0)
+    assert np.abs(out).max() < 1e-2
+
+
+@pytest.mark.parametrize("off", [4, 8, 16])
+def test_wrapped_at_an_offset(hip, off):
+    """Codes, exponents and rows that begin inside other allocations."""
+    g = rng(off)
+    H, D, bs = 2, 64, 16
+    lens = np.array([40, 33, 90], np.int32)
+    tables, nb = ref.pool(g, lens, bs, 6)
+    codes, exps = ref.cache(g, nb, H, bs, D)
+    hold = []
+
+    def at(a, off=off):
+        raw = np.concatenate([np.full(off, 0x55, np.uint8), a.reshape(-1).view(np.uint8),
+                              np.full(32, 0x55, np.uint8)])
+        hold.append(hip.tensor(raw, np.uint8))
+        return hip.wrap(hold[-1].device_ptr + off, a.shape, a.dtype.type)
+
+    for rows in ([1, 1, 1], [9, 0, 50]):
+        starts = ref.starts_of(rows)
+        n = int(starts[-1])
+        k, v, q = (g.standard_normal((n, H * D)).astype(np.float32) for _ in range(3))
+        for where in ((off, off), (off, 0), (0, off)):
+            w = g.random(tables.shape).astype(np.float32)
+            tc, te, tk, tv = at(codes, where[0]), at(exps), at(k), at(v)
+            tt, tl, ts = at(tables), at(lens), at(starts)
+            hip.paged_kv8_append(tc, te, tk, tv, tt, tl, ts)
+            ref.append(codes, exps, k, v, tables, lens, starts)
+            np.testing.assert_array_equal(tc.numpy(), codes)
+            np.testing.assert_array_equal(te.numpy(), exps)
+            for x, y in zip(hip.paged_kv8_read(tc, te, tt, tl, ts, rows=n),
+                            ref.read(codes, exps, tables, lens, n, starts)):
+                np.testing.assert_array_equal(x.numpy(), y.astype(np.float32))
+            out, wo = hip.paged_kv8_attention(at(q, where[1]), tc, te, tt, tl, ts, weights=at(w))
+            want, ww, tol, wtol = ref.attention(q, codes, exps, tables, lens, starts, weights=w)
+            within(out.numpy(), want, tol, "out")
+            within(wo.numpy(), ww, wtol, "weights")
+            for x, y in zip(hip.paged_evict(tt, tl, at(w), bs, 3, 1, 1),
+                            ref.evict(tables, lens, w, bs, 3, 1, 1)):
+                np.testing.assert_array_equal(x.numpy(), y)
+    for t in hold:  # nothing before or behind the tensors was touched
+        raw = t.numpy()
+        assert (raw[-32:] == 0x55).all()
+
+
+@pytest.mark.parametrize("rows,D,Hq", [(25, 32, 2), (25, 128, 8), (400, 64, 2)])
+def test_bad_row_starts_and_blocks_in_attention(hip, rows, D, Hq):
+    """Starts that leave the rows: reported, and the other sequences get their
+    answers.  Starts that decrease: reported (what the rows receive is not
+    specified).  Then tables that leave the pool, in every kernel of the attention."""
+    g = rng(rows + D)
+    H, bs, ctx = 2, 16, 700
+    lens = np.array([ctx, ctx - 5, 90], np.int32)
+    tables, nb = ref.pool(g, lens, bs, 44)
+    codes, exps = ref.cache(g, nb, H, bs, D)
+    q = g.standard_normal((rows, Hq * D)).astype(np.float32)
+    w = g.random(tables.shape).astype(np.float32)
+    part = rows * 2 // 5
+    for starts, whole in (([0, rows + 1, part, rows], []), ([0, 2 * part, part, rows], []),
+                          ([-1, 3, 5, rows], [1, 2]), ([0, part, 2 * part, rows + 1], [0, 1]),
+                          ([2**31 - 1, -2**31, 0, rows], [])):
+        starts = np.array(starts, np.int32)
+        args = up(hip, q, codes, exps, tables, lens, starts)
+        out, wo = hip.paged_kv8_attention(*args, weights=hip.tensor(w))
+        with pytest.raises(hip.CloveError) as e:
+            hip.synchronize()
+        assert e.value.code == hip.ERR_RANGE and "row_starts" in str(e.value)
+        want, ww, tol, wtol = ref.attention(q, codes, exps, tables, lens, starts, weights=w)
+        got, gw = out.numpy(), wo.numpy()
+        for b in whole:
+            at = slice(starts[b], starts[b + 1])
+            within(got[at], want[at], tol[at], f"out of {b} of {starts}")
+            within(gw[b], ww[b], wtol[b] + 1e-37, f"weights of {b} of {starts}")
+    tables[0, [0, 3, 20]], tables[1, 43], tables[2, :] = [nb, -1, 2**31 - 1], -2**31, -7
+    starts = np.array([0, part, 2 * part, rows], np.int32)
+    out, wo = hip.paged_kv8_attention(*up(hip, q, codes, exps, tables, lens, starts),
+                                      weights=hip.tensor(w))
+    with pytest.raises(hip.CloveError) as e:
+        hip.synchronize()
+    assert e.value.code == hip.ERR_RANGE and "block-table" in str(e.value)
+    want, ww, tol, wtol = ref.attention(q, codes, exps, tables, lens, starts, weights=w)
+    within(out.numpy(), want, tol, "out")
+    within(wo.numpy(), ww, wtol + 1e-37, "weights")
+
+
+def test_on_another_stream(hip):
+    """A step on the backend's stream, the next on a caller's: each waits for
+    what it reads."""
+    rt = C.CDLL("libamdhip64.so")
+    g = rng(47)
+    H, D, bs, B = 2, 64, 16, 3
+    lens = np.array([40, 17, 64], np.int32)
+    tables, nb = ref.pool(g, lens + 2, bs, 5)
+    codes, exps = ref.cache(g, nb, H, bs, D)
+    tc, te, tt = up(hip, codes, exps, tables)
+    other = C.c_void_p()
+    assert rt.hipStreamCreate(C.byref(other)) == 0
+    try:
+        for stream in (None, other, None):
+            k, v, q = (g.standard_normal((B, H * D)).astype(np.float32) for _ in range(3))
+            tl, tq = up(hip, lens, q)
+            tk, tv = up(hip, k, v)
+            assert hip.lib().clove_hip_set_stream(stream) == 0
+            hip.paged_kv8_append(tc, te, tk, tv, tt, tl)
+            ref.append(codes, exps, k, v, tables, lens)
+            out = hip.paged_kv8_attention(tq, tc, te, tt, tl).numpy()
+            want, _, tol, _ = ref.attention(q, codes, exps, tables, lens)
+            within(out, want, tol, "out")
+            lens = lens + 1
+    finally:
+        hip.lib().clove_hip_set_stream(None)
+        rt.hipStreamDestroy(other)
+    hip.synchronize()
 
 
 def test_no_rows_and_no_sequences(hip):
