@@ -332,9 +332,10 @@ __device__ __forceinline__ unsigned kv8_widen(unsigned codes, float scale) {
 int kv8_stream_residents();
 void kv8_stream(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
 void kv8_tiles(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
-// The weights of the blocks, the scores computed again (kv8_tiles has left every
-// row's maximum and sum).
+// The weights of the blocks (kv8_tiles has left every row's maximum and sum): from
+// sums that it stored as well, or the scores computed again.
 constexpr int kKv8WeightPart = 512;
+constexpr int64_t kKv8MaxSums = 1ll << 30;  // bytes of such sums
 void kv8_tile_weights(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
 
 }  // namespace k

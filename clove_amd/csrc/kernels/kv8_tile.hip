@@ -11,6 +11,7 @@
 // within each row of q lie close enough together, which is nearly always, f16
 // takes the place of bf16: two pieces of 11 bits do for q and P what three of 8
 // bits do, two thirds of the MFMAs.
+#include <algorithm>
 #include <type_traits>
 
 #include "bf16x3.h"
@@ -116,7 +117,8 @@ __device__ __forceinline__ int fill_table(const Kv8Args &c, int b, int h, int c0
 // FULL: head_dim = DP; else MFMA steps and blocks past it are left out.
 // HALF: f16 pieces, two of each; a workgroup whose tiles or rows do not let it
 // leaves its run to the bf16 form (p.declined), which otherwise finds nothing to do.
-template <int DP, int NR, bool FULL, bool HALF>
+// SUMS: the weights of every 16 tokens go out, for kv8_tile_weights.
+template <int DP, int NR, bool FULL, bool HALF, bool SUMS>
 __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p) {
     constexpr int KI = DP / 32;               // MFMA steps of q . k
     constexpr int KB = DP > 128 ? 32 : 64;    // tokens of a step
@@ -206,6 +208,10 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
         const int high =
             u0 < T.rows ? min(t_end, T.ctx - T.n + (T.r0 + min(u0 + 16 * NR, T.rows) - 1) / G + 1) : 0;
 
+        // [kv head][16 tokens][(row, query head) pair of the call]
+        const size_t pairs = (size_t)c.rows * G;
+        float2 *sums = reinterpret_cast<float2 *>(a.ws + p.sums_at) +
+                       (size_t)h * p.groups * pairs + (size_t)T.first * G + T.r0 + u0 + r;
         float m[NR], l[NR];
         cl_f4 o[NR][JB];
 #pragma unroll
@@ -459,13 +465,15 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                             m[cc] = m_new;
                         }
                         const float mz = m[cc] == -INFINITY ? 0.0f : m[cc];
+                        float part_sum[2];
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
                                 s[cc][u][i] = __builtin_amdgcn_exp2f(
                                     HALF ? fmaf(s[cc][u][i], down[cc], -mz) : s[cc][u][i] - mz);
-                            l[cc] += hsum4(s[cc][u]);
+                            part_sum[u] = hsum4(s[cc][u]);
+                            l[cc] += part_sum[u];
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
                                 unsigned w1, w2, w3 = 0;
@@ -478,6 +486,16 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                                 pf[cc][1][2 * u + e] = w2;
                                 pf[cc][2][2 * u + e] = w3;
                             }
+                        }
+                        if constexpr (SUMS) {
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                part_sum[u] += __shfl_xor(part_sum[u], 16, 64);
+                                part_sum[u] += __shfl_xor(part_sum[u], 32, 64);
+                            }
+                            if (q < 2 && t0 + 16 * q < lim[cc])
+                                sums[(size_t)(t0 / 16 + q) * pairs + 16 * cc] =
+                                    make_float2(part_sum[q], m[cc]);
                         }
                     }
                     __builtin_amdgcn_s_setprio(1);
@@ -720,22 +738,93 @@ __global__ void __launch_bounds__(1024) block_weights_kernel(Kv8Attention a, Kv8
     }
 }
 
+// The weights of the blocks from the sums that the tiles stored: a workgroup takes
+// the blocks of about 64 tokens, four sums of 16 tokens at a time; the lanes take
+// pairs of rows and heads, the waves 64 pairs of one kv head in turn.
+__global__ void __launch_bounds__(1024) sums_weights_kernel(Kv8Attention a, Kv8Split p, int blocks) {
+    const Kv8Args &c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int H = c.num_heads, G = a.q_heads / H, per = c.block_size / 16;
+    const int b = blockIdx.y, j0 = blockIdx.x * blocks, g1 = min(j0 + blocks, c.max_blocks) * per;
+    __shared__ float part[16][4], total;
+    const int ctx = kv8_context(c, b);
+    int first, n;
+    kv8_rows(c, b, &first, &n);
+    const size_t pairs = (size_t)c.rows * G;
+    const float2 *row_ml = reinterpret_cast<const float2 *>(a.ws + p.row_ml_at);
+    const float2 *sums = reinterpret_cast<const float2 *>(a.ws + p.sums_at) + (size_t)first * G;
+    if (tid == 0) total = 0.0f;
+    for (int g0 = j0 * per; g0 < g1; g0 += 4) {
+        // from the first row that sees any of the tokens
+        const int past = ctx - n, R = n * G, low = max(16 * g0 - past, 0) * G / 64;
+        const int chunks = 16 * g0 < ctx ? (R + 63) / 64 - low : 0;
+        float w[4] = {};
+        for (int x0 = wave; x0 < chunks * H; x0 += 64) {  // four at a time on their way
+            float2 ml[4], v[4][4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const int x = x0 + 16 * y, h = x / chunks, u = 64 * (low + x % chunks) + lane;
+                const int see = x < chunks * H && u < R ? past + u / G + 1 : 0;
+                if (see > 16 * g0)
+                    ml[y] = row_ml[(size_t)(first + u / G) * a.q_heads + h * G + u % G];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[y][i] = make_float2(0.0f, -INFINITY);
+                    if (g0 + i < g1 && 16 * (g0 + i) < see)
+                        v[y][i] = sums[((size_t)h * p.groups + g0 + i) * pairs + u];
+                }
+            }
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (v[y][i].y != -INFINITY)
+                        w[i] = fmaf(v[y][i].x, __builtin_amdgcn_exp2f(v[y][i].y - ml[y].x) * ml[y].y,
+                                    w[i]);
+        }
+        __syncthreads();  // the four before are done with
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) w[i] += __shfl_xor(w[i], o, 64);
+            if (lane == 0) part[wave][i] = w[i];
+        }
+        __syncthreads();
+        if (tid == 0)
+            for (int i = 0; i < 4 && g0 + i < g1; ++i) {
+                for (int x = 0; x < 16; ++x) total += part[x][i];
+                if ((g0 + i + 1) % per == 0) {
+                    const size_t at = (size_t)b * c.max_blocks + (g0 + i) / per;
+                    a.w_out[at] = a.w_in[at] + total;
+                    total = 0.0f;
+                }
+            }
+    }
+}
+
 }  // namespace
 
 void kv8_tiles(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
-    auto go = [&](auto full, auto half) {
+    auto launch = [&](auto full, auto half, auto sums) {
         constexpr bool F = decltype(full)::value, HALF = decltype(half)::value;
+        constexpr bool S = decltype(sums)::value;
         const unsigned grid = p.grid + (HALF ? kv8_zero_grid(a.c) : 0);
         if (p.dp == 256)
-            tile_kernel<256, 1, F, HALF><<<grid, 256, 0, s>>>(a, p);
+            tile_kernel<256, 1, F, HALF, S><<<grid, 256, 0, s>>>(a, p);
         else if (p.dp == 128 && p.tile == 128)
-            tile_kernel<128, 2, F, HALF><<<grid, 256, 0, s>>>(a, p);
+            tile_kernel<128, 2, F, HALF, S><<<grid, 256, 0, s>>>(a, p);
         else if (p.dp == 128)
-            tile_kernel<128, 1, F, HALF><<<grid, 256, 0, s>>>(a, p);
+            tile_kernel<128, 1, F, HALF, S><<<grid, 256, 0, s>>>(a, p);
         else if (p.tile == 128)
-            tile_kernel<64, 2, F, HALF><<<grid, 256, 0, s>>>(a, p);
+            tile_kernel<64, 2, F, HALF, S><<<grid, 256, 0, s>>>(a, p);
         else
-            tile_kernel<64, 1, F, HALF><<<grid, 256, 0, s>>>(a, p);
+            tile_kernel<64, 1, F, HALF, S><<<grid, 256, 0, s>>>(a, p);
+    };
+    auto go = [&](auto full, auto half) {
+        if (p.sums)
+            launch(full, half, std::true_type{});
+        else
+            launch(full, half, std::false_type{});
     };
     if (a.c.head_dim == p.dp) {
         go(std::true_type{}, std::true_type{});
@@ -748,6 +837,12 @@ void kv8_tiles(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
 
 void kv8_tile_weights(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
     const Kv8Args &c = a.c;
+    if (p.sums) {
+        const int blocks = std::max(1, 64 / c.block_size);
+        sums_weights_kernel<<<dim3((c.max_blocks + blocks - 1) / blocks, c.num_seqs), 1024, 0, s>>>(
+            a, p, blocks);
+        return;
+    }
     const dim3 grid((c.max_blocks * c.block_size + 255) / 256, c.num_heads,
                     (unsigned)kv8_slots(c, kPart, a.q_heads / c.num_heads, 1));
     if (p.dp == 64) tile_weights_kernel<64><<<grid, 256, 0, s>>>(a, p);
