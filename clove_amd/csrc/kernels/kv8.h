@@ -298,6 +298,10 @@ __device__ __forceinline__ bool kv8_next_tile(const Kv8Args &c, int G, int H, in
     return false;
 }
 
+// A maximum and a sum of tokens that a row saw nothing of.  (Scores that are NaN
+// leave a sum that is.)
+__device__ __forceinline__ bool kv8_empty(float2 ml) { return ml.x == -INFINITY && ml.y == 0.0f; }
+
 // Workgroups behind the others, of 256 threads, a wave a row: zeros for the rows
 // of no sequence and those without a token to see.
 inline unsigned kv8_zero_grid(const Kv8Args &c) { return (c.rows + 3) / 4; }

@@ -122,15 +122,117 @@ __device__ __forceinline__ int kv8_pieces(const Kv8Split &p, int share, int star
     return min((int)(((unsigned)start + steps - 1) / (unsigned)share), p.grid - 1) - *w0 + 1;
 }
 
+// Blocks behind a join's others: the weights of 64 blocks of a sequence from the
+// sums that the stream kernel stored.  Lanes take blocks, the waves the sequence's
+// rows and heads in turn, 64 of them at a time, whose maxima and sums are put
+// together here once more, so that no launch has to wait for the join.
+__device__ void kv8_block_weights(const Kv8Attention &a, const Kv8Split &p, int block) {
+    const Kv8Args &c = a.c;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int across = (c.max_blocks + 63) / 64, b = block / across;
+    const int j = block % across * 64 + lane;
+    const int per = c.block_size / p.sums, G = a.q_heads / c.num_heads;
+    __shared__ float part[16][64];
+    __shared__ float2 s_ml[64];
+    int first, n;
+    kv8_rows(c, b, &first, &n);
+    const int ctx = kv8_context(c, b);
+    const int slot = kv8_first_slot(c, b, p.tile, G, 1);
+    const int *starts = reinterpret_cast<const int *>(a.ws + p.start_at);
+    const float2 *row_ml = reinterpret_cast<const float2 *>(a.ws + p.row_ml_at);
+    const float2 *piece_ml = reinterpret_cast<const float2 *>(a.ws + p.ml_at);
+    const float2 *sums = reinterpret_cast<const float2 *>(a.ws + p.sums_at);
+    float w = 0.0f;
+    if ((int64_t)(j - lane) * c.block_size >= ctx) n = 0;  // (none of the blocks holds a token)
+    for (int x0 = 0; x0 < n * a.q_heads; x0 += 64) {
+        const int xs = min(64, n * a.q_heads - x0);
+        __syncthreads();  // the rows before are done with
+        for (int x = 4 * wave + lane / 16; x < xs; x += 4 * waves) {  // 16 lanes to a row
+            const int i = (x0 + x) / a.q_heads, hq = (x0 + x) % a.q_heads, h = hq / G;
+            const int u = i * G + hq % G, item = u / p.tile;
+            Kv8Tile T;
+            int w0 = 0, np = 1;
+            bool cut = false;
+            if (p.join && kv8_tile_of(c, G, b, item, p.tile, &T) && T.high > 0) {
+                const int start = starts[1 + (size_t)(slot + item) * (c.num_heads / p.hw) + h / p.hw];
+                np = kv8_pieces(p, starts[0], start, kv8_steps(T.high, p.step), &w0);
+                cut = start != w0 * starts[0];
+            }
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (np <= 1) {
+                ml = row_ml[(size_t)first * a.q_heads + x0 + x];
+            } else {
+                const size_t row = (size_t)(h % p.hw) * p.stored + u - T.r0;
+                const size_t per_piece = (size_t)p.hw * p.stored;
+                for (int y0 = lane & 15; y0 < np; y0 += 64) {
+                    float2 v[4];
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) {
+                        const int y = y0 + 16 * z;
+                        v[z] = make_float2(-INFINITY, 0.0f);
+                        if (y < np)
+                            v[z] = piece_ml[(size_t)(2 * (w0 + y) + (y == 0 && cut ? 1 : 0)) * per_piece +
+                                            row];
+                    }
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) {
+                        if (kv8_empty(v[z])) continue;
+                        const float t = fmaxf(ml.x, v[z].x);
+                        ml.y = ml.y * __builtin_amdgcn_exp2f(ml.x - t) +
+                               v[z].y * __builtin_amdgcn_exp2f(v[z].x - t);
+                        ml.x = t;
+                    }
+                }
+                float top = ml.x;
+#pragma unroll
+                for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+                float l = kv8_empty(ml) ? 0.0f : ml.y * __builtin_amdgcn_exp2f(ml.x - top);
+#pragma unroll
+                for (int o = 1; o < 16; o <<= 1) l += __shfl_xor(l, o, 64);
+                ml = make_float2(top, l == 0.0f ? 0.0f : 1.0f / l);
+            }
+            if ((lane & 15) == 0) s_ml[x] = ml;
+        }
+        __syncthreads();
+        if (j < c.max_blocks && (int64_t)j * c.block_size < ctx) {
+#pragma unroll 4
+            for (int x = wave; x < xs; x += waves) {
+                const int see = ctx - n + (x0 + x) / a.q_heads + 1 - j * c.block_size;
+                const float2 ml = s_ml[x];
+                const float2 *from = sums + ((size_t)first * a.q_heads + x0 + x) * p.groups + (size_t)j * per;
+                for (int i = 0; i < per && i * p.sums < see; ++i) {
+                    const float2 v = from[i];
+                    const float f = v.y == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v.y - ml.x);
+                    w += v.x * f * ml.y;
+                }
+            }
+        }
+    }
+    part[wave][lane] = w;
+    __syncthreads();
+    if (wave == 0 && j < c.max_blocks) {
+        const size_t at = (size_t)b * c.max_blocks + j;
+        for (int x = 1; x < waves; ++x) w += part[x][lane];
+        a.w_out[at] = a.w_in[at] + w;
+    }
+}
+__global__ void __launch_bounds__(256) kv8_weights_kernel(Kv8Attention a, Kv8Split p) {
+    kv8_block_weights(a, p, blockIdx.x);
+}
+
 // Joins the pieces of the tiles that were cut: `per` waves take the pieces of a
 // row in turn, eight on their way at a time, and a lane holds up to four dims.
-__global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split p, int per) {
+__global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split p, int per,
+                                                        int grid) {
+    if ((int)blockIdx.x >= grid) {
+        kv8_block_weights(a, p, blockIdx.x - grid);
+        return;
+    }
     const Kv8Args &c = a.c;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rows = (blockDim.x >> 6) / per;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int D = c.head_dim, H = c.num_heads, G = a.q_heads / H;
-    const int groups = (p.stored + rows - 1) / rows;
-    const int h = blockIdx.x % H, slot = blockIdx.x / H / groups;
-    const int u = (int)(blockIdx.x / H % groups) * rows + wave / per;
+    const int h = blockIdx.x % H, slot = blockIdx.x / H / p.stored;
+    const int u = blockIdx.x / H % p.stored;
     __shared__ float s_o[16][kKv8MaxHeadDim], s_l[16], s_top[16];
     const int *starts = reinterpret_cast<const int *>(a.ws + p.start_at);
     const int share = starts[0], start = starts[1 + (size_t)slot * (H / p.hw) + h / p.hw];
@@ -141,79 +243,83 @@ __global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split
     int w0;
     const int np = kv8_pieces(p, share, start, kv8_steps(T.high, p.step), &w0);
     if (np <= 1) return;  // written whole
+    if (u >= T.rows) return;
     float top = -INFINITY, l = 0.0f, x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (u < T.rows) {
-        // the first piece ends its workgroup's run unless the run begins with it
-        const size_t row = (size_t)(h % p.hw) * p.stored + u, per_piece = (size_t)p.hw * p.stored;
-        const size_t first = (2 * w0 + (start != w0 * share ? 1 : 0)) * per_piece + row;
-        const float2 *ml = reinterpret_cast<const float2 *>(a.ws + p.ml_at);
-        const float *o = a.ws + p.o_at;
-        for (int i0 = wave % per; i0 < np; i0 += 8 * per) {
-            float2 v[8];
-            float y[8][4];
+    // the first piece ends its workgroup's run unless the run begins with it
+    const size_t row = (size_t)(h % p.hw) * p.stored + u, per_piece = (size_t)p.hw * p.stored;
+    const size_t first = (2 * w0 + (start != w0 * share ? 1 : 0)) * per_piece + row;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.ws + p.ml_at);
+    const float *o = a.ws + p.o_at;
+    for (int i0 = wave; i0 < np; i0 += 8 * per) {
+        float2 v[8];
+        float y[8][4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int i = i0 + j * per;
-                v[j] = make_float2(-INFINITY, 0.0f);
-                if (i < np) {
-                    const size_t at = i == 0 ? first : 2 * (w0 + i) * per_piece + row;
-                    v[j] = ml[at];
+        for (int j = 0; j < 8; ++j) {
+            const int i = i0 + j * per;
+            v[j] = make_float2(-INFINITY, 0.0f);
+            if (i < np) {
+                const size_t at = i == 0 ? first : 2 * (w0 + i) * per_piece + row;
+                v[j] = ml[at];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        y[j][e] = lane + 64 * e < D ? o[at * D + lane + 64 * e] : 0.0f;
-                }
+                for (int e = 0; e < 4; ++e)
+                    y[j][e] = lane + 64 * e < D ? o[at * D + lane + 64 * e] : 0.0f;
             }
-            float t = top;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) t = fmaxf(t, v[j].x);
-            const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - t);
-            l *= f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] *= f;
-            top = t;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (v[j].x != -INFINITY) {
-                    const float fj = __builtin_amdgcn_exp2f(v[j].x - t);
-                    l = fmaf(v[j].y, fj, l);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = fmaf(y[j][e], fj, x[e]);
-                }
         }
+        float t = top;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t = fmaxf(t, v[j].x);
+        const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - t);
+        l *= f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] *= f;
+        top = t;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (!kv8_empty(v[j])) {
+                const float fj = __builtin_amdgcn_exp2f(v[j].x - t);
+                l = fmaf(v[j].y, fj, l);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = fmaf(y[j][e], fj, x[e]);
+            }
     }
-    if (per > 1) {  // (one row to the workgroup)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (lane + 64 * e < D) s_o[wave][lane + 64 * e] = x[e];
+    if (lane == 0) {
+        s_l[wave] = l;
+        s_top[wave] = top;
+    }
+    __syncthreads();
+    if (wave) return;
+    const float mine = lane < per ? s_top[lane] : -INFINITY;
+    top = wave_max(mine);
+    const float f = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - top);
+    l = wave_sum(lane < per ? s_l[lane] * f : 0.0f);
+    x[0] = x[1] = x[2] = x[3] = 0.0f;
+#pragma unroll 4
+    for (int w = 0; w < per; ++w) {
+        const float fw = __shfl(f, w, 64);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (lane + 64 * e < D) s_o[wave][lane + 64 * e] = x[e];
-        if (lane == 0) {
-            s_l[wave] = l;
-            s_top[wave] = top;
-        }
-        __syncthreads();
-        if (wave) return;
-        for (int w = 1; w < per; ++w) top = fmaxf(top, s_top[w]);
-        l = x[0] = x[1] = x[2] = x[3] = 0.0f;
-        for (int w = 0; w < per; ++w) {
-            const float f = s_top[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_top[w] - top);
-            l = fmaf(s_l[w], f, l);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (lane + 64 * e < D) x[e] = fmaf(s_o[w][lane + 64 * e], f, x[e]);
-        }
+            if (lane + 64 * e < D) x[e] = fmaf(s_o[w][lane + 64 * e], fw, x[e]);
     }
-    if (u >= T.rows) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const size_t rh = (size_t)(T.first + (T.r0 + u) / G) * a.q_heads + h * G + (T.r0 + u) % G;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (lane + 64 * e < D) a.out[rh * D + lane + 64 * e] = x[e] * inv;
-    if (lane == 0 && a.w_out)
+    // (for the tiles' weights)
+    if (lane == 0 && a.w_out && p.kind == KV8_TILE)
         reinterpret_cast<float2 *>(a.ws + p.row_ml_at)[rh] = make_float2(top, inv);
 }
 
 // The same for tiles of many rows with few pieces: a thread joins four dims of a
 // row, all the loads of a workgroup run along the rows.
-__global__ void __launch_bounds__(256) kv8_join_rows_kernel(Kv8Attention a, Kv8Split p) {
+__global__ void __launch_bounds__(256) kv8_join_rows_kernel(Kv8Attention a, Kv8Split p, int grid) {
+    if ((int)blockIdx.x >= grid) {
+        kv8_block_weights(a, p, blockIdx.x - grid);
+        return;
+    }
     const Kv8Args &c = a.c;
     const int D = c.head_dim, H = c.num_heads, G = a.q_heads / H, D4 = D / 4;
     const int groups = (p.stored * D4 + blockDim.x - 1) / blockDim.x;
@@ -245,7 +351,7 @@ __global__ void __launch_bounds__(256) kv8_join_rows_kernel(Kv8Attention a, Kv8S
             v[j] = ml[at];
             y[j] = o[at * D4 + d4];
         }
-        if (i0 + 1 >= np) v[1].x = -INFINITY;
+        if (i0 + 1 >= np) v[1] = make_float2(-INFINITY, 0.0f);
         const float t = fmaxf(top, fmaxf(v[0].x, v[1].x));
         const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - t);
         l *= f;
@@ -253,7 +359,7 @@ __global__ void __launch_bounds__(256) kv8_join_rows_kernel(Kv8Attention a, Kv8S
         top = t;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-            if (v[j].x != -INFINITY) {
+            if (!kv8_empty(v[j])) {
                 const float fj = __builtin_amdgcn_exp2f(v[j].x - t);
                 l = fmaf(v[j].y, fj, l);
                 sum += y[j] * fj;
@@ -262,44 +368,8 @@ __global__ void __launch_bounds__(256) kv8_join_rows_kernel(Kv8Attention a, Kv8S
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const size_t rh = (size_t)(T.first + (T.r0 + u) / G) * a.q_heads + h * G + (T.r0 + u) % G;
     reinterpret_cast<cl_f4 *>(a.out)[rh * D4 + d4] = sum * inv;
-    if (d4 == 0 && a.w_out)
+    if (d4 == 0 && a.w_out && p.kind == KV8_TILE)
         reinterpret_cast<float2 *>(a.ws + p.row_ml_at)[rh] = make_float2(top, inv);
-}
-
-// The weight of each block from the sums stored on the way: lanes take 64
-// blocks, the waves a sequence's rows and heads in turn.
-__global__ void __launch_bounds__(1024) kv8_weights_kernel(Kv8Attention a, Kv8Split p) {
-    const Kv8Args &c = a.c;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int j = blockIdx.x * 64 + lane, b = blockIdx.y;
-    const int per = c.block_size / p.sums;
-    __shared__ float part[16][64];
-    int first, n;
-    kv8_rows(c, b, &first, &n);
-    const int ctx = kv8_context(c, b);
-    const float2 *row_ml = reinterpret_cast<const float2 *>(a.ws + p.row_ml_at);
-    const float2 *sums = reinterpret_cast<const float2 *>(a.ws + p.sums_at);
-    float w = 0.0f;
-    if (j < c.max_blocks && (int64_t)j * c.block_size < ctx) {
-        #pragma unroll 4
-        for (int x = wave; x < n * a.q_heads; x += waves) {
-            const size_t rh = (size_t)first * a.q_heads + x;
-            const int see = ctx - n + x / a.q_heads + 1 - j * c.block_size;
-            const float2 ml = row_ml[rh];
-            for (int i = 0; i < per && i * p.sums < see; ++i) {
-                const float2 v = sums[rh * p.groups + (size_t)j * per + i];
-                const float f = v.y == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v.y - ml.x);
-                w += v.x * f * ml.y;
-            }
-        }
-    }
-    part[wave][lane] = w;
-    __syncthreads();
-    if (wave == 0 && j < c.max_blocks) {
-        const size_t at = (size_t)b * c.max_blocks + j;
-        for (int x = 1; x < waves; ++x) w += part[x][lane];
-        a.w_out[at] = a.w_in[at] + w;
-    }
 }
 
 Kv8Split kv8_split(const Kv8Attention &a, int cus) {
@@ -407,23 +477,27 @@ void kv8_attention(const Kv8Attention &a, int cus, hipStream_t s) {
         kv8_stream(a, p, s);
     else
         kv8_tiles(a, p, s);
+    // the blocks' weights: with the join, or after the tiles' one
+    const unsigned blocks =
+        weights && p.kind == KV8_STREAM ? (unsigned)((c.max_blocks + 63) / 64) * c.num_seqs : 0;
     if (p.join) {
         const unsigned tiles = (unsigned)kv8_slots(c, p.tile, a.q_heads / c.num_heads, 1) * c.num_heads;
         // pieces to a tile: 2 on the average where there are as many tiles as runs
         const int pieces = p.grid * p.hw / (int)tiles + 1;
         if (pieces <= 8) {
-            const int n = p.stored * c.head_dim / 4, threads = std::min(256, (n + 63) / 64 * 64);
-            kv8_join_rows_kernel<<<tiles * ((n + threads - 1) / threads), threads, 0, s>>>(a, p);
+            const int n = p.stored * c.head_dim / 4;
+            const int threads = blocks ? 256 : std::min(256, (n + 63) / 64 * 64);
+            const unsigned grid = tiles * ((n + threads - 1) / threads);
+            kv8_join_rows_kernel<<<grid + blocks, threads, 0, s>>>(a, p, (int)grid);
         } else {
-            const int per = pieces <= 32 ? 4 : 16, rows = 4 / per > 0 ? 4 / per : 1;
-            kv8_join_kernel<<<tiles * ((p.stored + rows - 1) / rows), 64 * per * rows, 0, s>>>(a, p, per);
+            const int per = pieces <= 32 ? 4 : 16;
+            const unsigned grid = tiles * p.stored;
+            kv8_join_kernel<<<grid + blocks, 64 * per, 0, s>>>(a, p, per, (int)grid);
         }
+    } else if (blocks) {
+        kv8_weights_kernel<<<blocks, 256, 0, s>>>(a, p);
     }
-    if (weights && p.kind == KV8_TILE)
-        kv8_tile_weights(a, p, s);
-    else if (weights)
-        kv8_weights_kernel<<<dim3((c.max_blocks + 63) / 64, c.num_seqs), a.q_heads > 8 ? 1024 : 256, 0,
-                             s>>>(a, p);
+    if (weights && p.kind == KV8_TILE) kv8_tile_weights(a, p, s);
 }
 
 }  // namespace k

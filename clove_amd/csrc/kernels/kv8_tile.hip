@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(1024) sums_weights_kernel(Kv8Attention a, Kv8S
             for (int y = 0; y < 4; ++y)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (v[y][i].y != -INFINITY)
+                    if (!kv8_empty(make_float2(v[y][i].y, v[y][i].x)))
                         w[i] = fmaf(v[y][i].x, __builtin_amdgcn_exp2f(v[y][i].y - ml[y].x) * ml[y].y,
                                     w[i]);
         }

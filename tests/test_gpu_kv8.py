@@ -312,6 +312,27 @@ def test_not_finite_queries_stay_in_their_rows(hip):
     np.testing.assert_array_equal(heads[~dirty], clean.reshape(40, 2 * H, D)[~dirty])
 
 
+@pytest.mark.parametrize("rows,Hq", [(1, 4), (6, 4), (200, 2)])
+def test_not_finite_queries_over_cut_contexts(hip, rows, Hq):
+    """The same where a context is cut over workgroups and joined."""
+    g = rng(rows)
+    H, D, bs, n = 2, 64, 16, 6000
+    lens = np.array([n], np.int32)
+    tables, nb = ref.pool(g, lens, bs, n // bs)
+    codes, exps = ref.cache(g, nb, H, bs, D)
+    q = g.standard_normal((rows, Hq * D)).astype(np.float32)
+    starts, w = np.array([0, rows], np.int32), np.zeros(tables.shape, np.float32)
+    clean = check_attention(hip, q, codes, exps, tables, lens, starts, weights=w)
+    q[0, 5] = np.nan
+    out, wo = hip.paged_kv8_attention(*up(hip, q, codes, exps, tables, lens, starts),
+                                      weights=hip.tensor(w))
+    got = out.numpy().reshape(rows, Hq, D)
+    assert np.isnan(got[0, 0]).all() and np.isnan(wo.numpy()[0, 0])
+    dirty = np.zeros((rows, Hq), bool)
+    dirty[0, 0] = True
+    np.testing.assert_array_equal(got[~dirty], clean.reshape(rows, Hq, D)[~dirty])
+
+
 def test_shared_blocks_and_repeats(hip):
     """Sequences that share a prefix's blocks, and the same bits twice."""
     g = rng(37)
