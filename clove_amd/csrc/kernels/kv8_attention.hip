@@ -399,17 +399,20 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
     const int64_t units = ((int64_t)c.rows * G + c.num_seqs - 1) / c.num_seqs;
     const int64_t cap = (int64_t)c.max_blocks * bs;
     int residents;
+    // (16 speculating sequences of 22 rows and heads each: 52 us, as tiles 67)
     if (units <= (p.dp == 256 ? 16 : 32)) {
         p.kind = KV8_STREAM;
         p.tile = units <= 16 || p.dp == 256 ? 16 : 32;
         // Four heads of the same tokens side by side are 8 KB in a row to the memory
-        // (32 x 4096 tokens, 32 heads of 128: 98 against 109 us) but cut a tile
-        // into four times the pieces: where the heads' tiles are few, that costs
-        // more than it gives (one context of 131001 tokens: 57 against 47 us;
-        // speculated tokens: 59 against 50).
+        // (32 x 4096 tokens, 32 heads of 128: 98 against 109 us; 24 x 600 to 3000
+        // tokens, 16 heads of 96, 96 tiles of four heads: 49 against 51) but cut a
+        // tile into four times the pieces, which costs more than it gives where the
+        // tiles are few (one context of 131000 tokens, one tile: 57 against 47
+        // us), and two heads gain less (speculated tokens, 104 tiles: 60
+        // against 53).
         p.hw = kv8_stream_heads(p.dp, p.tile);
         if (c.num_heads % p.hw ||
-            2 * kv8_slots(c, p.tile, G, 1) * c.num_heads / p.hw < cus * kv8_stream_residents())
+            kv8_slots(c, p.tile, G, 1) * c.num_heads / p.hw < (p.hw == 4 ? cus / 4 : cus))
             p.hw = 1;
         p.step = 32 * 4 / p.hw;
         residents = kv8_stream_residents();
