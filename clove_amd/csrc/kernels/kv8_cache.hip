@@ -8,6 +8,12 @@
 //   code = round_e4m3(x * 2^-e),
 // and where e grew, the tokens before are rounded again, c * 2^(old - e).
 // Scaling by a power of two is exact, so every element is rounded once.
+//
+// Bound by memory: five bytes an element.  Eight prompts of 200 to 2048 rows, 32
+// heads of 128, stored and read back: 166 us for 10 bytes an element at 4.2 TB/s
+// (a large copy: 4.9; one workgroup a tile, the rows read twice: 371).  A token for
+// each of 32 sequences is two launches of 4 and 6 us, each a chain of dependent
+// loads (row range, context, block, exponent, rows): 13 us with their submission.
 #include <algorithm>
 
 #include "kv8.h"

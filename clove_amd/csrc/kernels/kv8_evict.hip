@@ -3,11 +3,17 @@
 // One workgroup a sequence.  Of its n = ceil(ctx / block_size) blocks the first
 // and last ones stay; of those between them the (budget - first - last) heaviest
 // do.  Weights are read once, as unsigned keys of the same order, into registers
-// (K a thread).  The least key that stays is
-// found bit by bit from the top: the largest x with at least `left` keys >= x,
-// counted by ballots, which ends early once exactly `left` are.  One scan then
-// gives every block its place: among equal weights the earlier blocks stay.
-// Only integers are counted, so results do not depend on timing.
+// (K a thread).  The least key that stays is found bit by bit from the top: the
+// largest x with at least `left` keys >= x, counted by ballots, which ends early
+// once exactly `left` are.  One scan then gives every block its place: among equal
+// weights the earlier blocks stay.  Only integers are counted, so results do not
+// depend on timing.
+//
+// Bound by latency, a round over the workgroup for each of the keys' bits: 256
+// sequences of 1250 to 4096 blocks down to 1024, 11 us (the weights and tables
+// are 4 us of memory traffic; keys read again from memory for every bit, one thread a
+// place: 44), 8 of 63 to 128 blocks 6 us; 15 us each with the call's four
+// allocations and submission.
 #include "kv8.h"
 
 namespace clove {

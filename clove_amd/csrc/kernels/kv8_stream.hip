@@ -1,11 +1,11 @@
 // kv8_stream.hip -- attention of a few query rows over the 8-bit paged cache:
 // decode steps, grouped heads, a handful of speculated tokens.
 //
-// Tiles of up to 16 * NC query rows of one kv head, their contexts in steps of
-// 128 tokens, and every workgroup an equal run of all steps (Kv8Split): ragged
-// batches keep every CU busy to the end.  Of a step each of the four waves takes
-// 32 tokens and streams their codes from memory into the operands of
-// v_mfma_f32_16x16x32_bf16:
+// Tiles of up to 16 * NC query rows of HW neighbouring kv heads, their contexts in
+// steps of 32 * 4 / HW tokens, and every workgroup an equal run of all steps
+// (Kv8Split): ragged batches keep every CU busy to the end.  Of a step each of the
+// four waves takes 32 tokens of a head and streams their codes from memory into the
+// operands of v_mfma_f32_16x16x32_bf16:
 //   S^T = K Q^T    A: lane (r, q) holds token r's dims 64s + 16q .. + 15 (one
 //                  16-byte load, two MFMA steps; q is laid out alike),
 //                  B: the 16 rows' q as three bf16 pieces, which hold all 24 bits;
@@ -15,6 +15,16 @@
 //                  exchange between lanes; P in three bf16 pieces.
 // A code times its tile's power of two is exact in bf16, so the conversion
 // applies the scale, and products are those of 32-bit values with f32 sums.
+//
+// Bound by memory, two bytes a dim of a token, once the contexts are long: 32
+// sequences of 511 to 4095 tokens, 32 heads of 128, 99 us with the join at 5.4
+// TB/s; a form that only loads the codes runs 5% faster.  64 of 500 to 8191, 8 kv
+// heads for 32: 103 us.  Few tiles are bound by latency besides: finding the
+// place, the tables and the first codes, and the join are dependent trips to
+// memory, some 15 of the 40 us of one context of 131000 tokens (3.3 TB/s).  The
+// table of an item's tokens is therefore fetched while the one before runs, and the
+// segment before goes out while the first codes are on their way.  Two workgroups
+// to a CU: a third would take registers that spill.
 #include "bf16x3.h"
 #include "kv8.h"
 #include "wave.h"
