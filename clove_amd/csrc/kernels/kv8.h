@@ -234,18 +234,20 @@ __device__ __forceinline__ Kv8Place kv8_find_place(const Kv8Args &c, int G, int 
                                                     int grid, int w, int *s_wave,
                                                     Kv8Place *s_place) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (c.num_seqs + 255) / 256;
-    // f(item, steps) for the tiles of sequence b
+    // a thread takes whole sequences, or (where there are few) part of one's tiles
+    const int per = (c.num_seqs + 255) / 256, share_b = max(256 / max(c.num_seqs, 1), 1);
+    const int b0 = tid / share_b * per, b1 = min(b0 + per, c.num_seqs), sub = tid % share_b;
+    // f(item, steps) for the thread's tiles of sequence b
     auto tiles = [&](int b, auto f) {
         int first, n;
         kv8_rows(c, b, &first, &n);
-        const int ctx = kv8_context(c, b);
-        for (int item = 0; item * tile < n * G; ++item)
+        const int ctx = kv8_context(c, b), items = (n * G + tile - 1) / tile;
+        const int each = (items + share_b - 1) / share_b;
+        for (int item = sub * each; item < min((sub + 1) * each, items); ++item)
             f(item, kv8_steps(ctx - n + (min((item + 1) * tile, n * G) - 1) / G + 1, step) * H);
     };
     int mine = 0;
-    for (int b = tid * per; b < min((tid + 1) * per, c.num_seqs); ++b)
-        tiles(b, [&](int, int n) { mine += n; });
+    for (int b = b0; b < b1; ++b) tiles(b, [&](int, int n) { mine += n; });
     int inc = mine;
     for (int o = 1; o < 64; o <<= 1) {
         const int up = __shfl_up(inc, o, 64);
@@ -260,7 +262,7 @@ __device__ __forceinline__ Kv8Place kv8_find_place(const Kv8Args &c, int G, int 
     const int share = max((total + grid - 1) / grid, 1);
     const int want = share * w;  // (the host keeps (tiles + grid) * steps below 2^31)
     if (want >= at && want < at + mine) {
-        for (int b = tid * per; b < min((tid + 1) * per, c.num_seqs); ++b)
+        for (int b = b0; b < b1; ++b)
             tiles(b, [&](int item, int n) {
                 if (want >= at && want < at + n) {
                     s_place->b = b;

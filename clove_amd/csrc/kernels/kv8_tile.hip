@@ -191,15 +191,14 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
 
         // this wave's rows, and the tokens each sees
         int lim[NR], lift[NR];
-        float lost = 0.0f;
         size_t rowhead[NR];
-        auto q_of = [&](int cc, int i, cl_f4 (&x)[2]) {
+        auto load_q = [&](int cc, int i, cl_f4 (&x)[2]) {
             const int d = 32 * i + 8 * q;
             x[0] = x[1] = (cl_f4){0.f, 0.f, 0.f, 0.f};
             if (16 * (NR * wave + cc) + r < T.rows && d < D) {
                 const cl_f4 *from = reinterpret_cast<const cl_f4 *>(a.q + rowhead[cc] * D + d);
-                x[0] = from[0] * (a.scale * kLog2e);  // (weights are powers of two)
-                x[1] = from[1] * (a.scale * kLog2e);
+                x[0] = from[0];
+                x[1] = from[1];
             }
         };
 #pragma unroll
@@ -237,29 +236,42 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
         // order of S^T's elements in a lane, twice four of them
         const int vpos = vquad / 8 * 32 + vquad % 4 * 8 + vquad / 4 % 2 * 4;
 
-        for (int c0 = s0 * KB; c0 < t_end; c0 += kChunk) {
-            const int c1 = min(c0 + kChunk, t_end);
+        // the table of the chunk from c0 on, whole at the next barrier
+        auto next_table = [&](int c0) {
             if (tid < 6) s_range[tid] = tid < 4 ? -1000 : 0;
             __syncthreads();  // the table and tiles before are done with
+            const int c1 = min(c0 + kChunk, t_end);
             if (__any(fill_table(c, at.b, h, c0, c1, KB, table, s_range)) && lane == 0)
                 s_range[4] = 1;
-            if (HALF && c0 == s0 * KB) {
-                // A row is lifted to 2^14 .. 2^15.  Elements below 2^-17 of its largest
-                // then lose bits: each is off by up to 2^-39 of the largest, `lost`
-                // times 2^-39 together.
+        };
+        // the rows' loads run beside the table's
+        u4 qf[NR][KI][HALF ? 2 : 3];
+        {
+            cl_f4 raw[NR][KI][2];
 #pragma unroll
-                for (int cc = 0; cc < NR; ++cc) {
-                    cl_f4 x[KI][2];
+            for (int cc = 0; cc < NR; ++cc)
+#pragma unroll
+                for (int i = 0; i < KI; ++i) load_q(cc, i, raw[cc][i]);
+            next_table(s0 * KB);
+#pragma unroll
+            for (int cc = 0; cc < NR; ++cc) {
+                if constexpr (!HALF) {
+#pragma unroll
+                    for (int i = 0; i < KI; ++i)
+                        split_q(raw[cc][i], a.scale * kLog2e, qf[cc][i]);
+                } else {
+                    // A row is lifted to 2^14 .. 2^15.  Elements below 2^-17 of its
+                    // largest then lose bits: each is off by up to 2^-39 of the
+                    // largest, `lost` times 2^-39 together.
                     float most = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < KI; ++i) {
-                        q_of(cc, i, x[i]);
+                    for (int i = 0; i < KI; ++i)
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            const float y = fabsf(x[i][e / 4][e & 3]);
+                            raw[cc][i][e / 4][e & 3] *= a.scale * kLog2e;  // (weights: powers of 2)
+                            const float y = fabsf(raw[cc][i][e / 4][e & 3]);
                             if (kv8_finite(y)) most = fmaxf(most, y);
                         }
-                    }
                     most = fmaxf(most, __shfl_xor(most, 16, 64));
                     most = fmaxf(most, __shfl_xor(most, 32, 64));
                     int small = 0;
@@ -267,7 +279,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                     for (int i = 0; i < KI; ++i)
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            const float y = fabsf(x[i][e / 4][e & 3]);
+                            const float y = fabsf(raw[cc][i][e / 4][e & 3]);
                             small += y > 0.0f && y < most * 0x1p-17f;
                         }
                     small += __shfl_xor(small, 16, 64);
@@ -276,11 +288,30 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                     if (q == 0)
                         atomicMax(&s_range[5],
                                   __float_as_int(lift[cc] < -60 ? INFINITY : small * most));
+                    const float up = kv8_pow2(max(lift[cc], -126));
+#pragma unroll
+                    for (int i = 0; i < KI; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            unsigned w1, w2;
+                            split_half(raw[cc][i][e / 2][2 * (e & 1)] * up,
+                                       raw[cc][i][e / 2][2 * (e & 1) + 1] * up, &w1, &w2);
+                            qf[cc][i][0][e] = w1;
+                            qf[cc][i][1][e] = w2;
+                        }
                 }
             }
-            __syncthreads();
+        }
+        __syncthreads();
+        const float lost = HALF ? __int_as_float(s_range[5]) : 0.0f;
+
+        for (int c0 = s0 * KB; c0 < t_end; c0 += kChunk) {
+            const int c1 = min(c0 + kChunk, t_end);
+            if (c0 != s0 * KB) {
+                next_table(c0);
+                __syncthreads();
+            }
             const bool bad = s_range[4];
-            if (HALF && c0 == s0 * KB) lost = __int_as_float(s_range[5]);
             // f16 holds codes times 2^(exponent - the largest + 7) exactly over 22
             // octaves of the tiles' exponents; with rows and weights lifted likewise,
             // two pieces of each do what three bf16 ones do, if what the rows lost
@@ -292,27 +323,6 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                 if (tid == 0) *declined = 1;
                 return;
             }
-            u4 qf[NR][KI][HALF ? 2 : 3];
-#pragma unroll
-            for (int cc = 0; cc < NR; ++cc)
-#pragma unroll
-                for (int i = 0; i < KI; ++i) {
-                    cl_f4 x[2];
-                    q_of(cc, i, x);
-                    if constexpr (HALF) {
-                        const float up = kv8_pow2(lift[cc]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            unsigned w1, w2;
-                            split_half(x[e / 2][2 * (e & 1)] * up,
-                                       x[e / 2][2 * (e & 1) + 1] * up, &w1, &w2);
-                            qf[cc][i][0][e] = w1;
-                            qf[cc][i][1][e] = w2;
-                        }
-                    } else {
-                        split_q(x, 1.0f, qf[cc][i]);
-                    }
-                }
             const float k_down = HALF ? kv8_pow2(7 - ke) : 1.0f;
             const float v_down = HALF ? kv8_pow2(7 - ve) : 1.0f;
             float down[NR];  // a score's factor
