@@ -164,13 +164,16 @@ __device__ __forceinline__ float kv8_decode(uint8_t code) {
 // sequence, tile by tile, head by head, and each workgroup gets an equal run of
 // them, whatever the lengths are: `share` steps, known on the device alone.  A
 // tile that one workgroup holds whole is written by it; of a tile cut in pieces
-// every workgroup stores its piece, at most one at the front of its run and
-// one at its end, and kv8_join puts them together.
+// every workgroup stores its piece, and kv8_join puts them together: at most one
+// that begins a tile, at the end of the run, and one that goes on with a tile, at
+// its front.  `extra` steps that hold no tokens stand before each tile's own, for the
+// time that a tile takes to begin and end.
 struct Kv8Split {
     int kind;          // one of the KV8_ kernels
     int dp;            // head_dim the kernel is laid out for
     int tile;
     int step;
+    int extra;
     int hw;            // heads that a workgroup takes together
     int grid;          // workgroups that share the steps, at most kKv8MaxGrid
     bool join;         // whether a tile may be cut
@@ -178,9 +181,9 @@ struct Kv8Split {
     int sums;          // tokens to a stored sum of weights, 0: none stored
     int groups;        // such sums a row
     // in the workspace, in floats
-    size_t o_at, ml_at;      // piece 2w (+ 1: at the end of the run) of workgroup w: of hw
+    size_t o_at, ml_at;      // piece 2w (+ 1: begins a tile) of workgroup w: of hw
                              // heads `stored` sums over V [D], and (maximum, sum) pairs
-    size_t start_at;         // share, then [slot, head / hw] first step of the tile
+    size_t start_at;         // share, then [slot, head / hw] the tile's first step with tokens
     size_t declined_at;      // KV8_TILE: whether a workgroup leaves its run to the bf16 form
     size_t row_ml_at;        // (maximum, 1 / sum) of every row and query head
     size_t sums_at;          // [row, query head][groups] (sum, maximum) pairs
@@ -231,7 +234,7 @@ struct Kv8Place {
 // All 256 threads: the steps before each sequence are summed up (in one order
 // everywhere), and step `share * w` is looked up in them.
 __device__ __forceinline__ Kv8Place kv8_find_place(const Kv8Args &c, int G, int H, int tile, int step,
-                                                    int grid, int w, int *s_wave,
+                                                    int extra, int grid, int w, int *s_wave,
                                                     Kv8Place *s_place) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // a thread takes whole sequences, or (where there are few) part of one's tiles
@@ -244,7 +247,10 @@ __device__ __forceinline__ Kv8Place kv8_find_place(const Kv8Args &c, int G, int 
         const int ctx = kv8_context(c, b), items = (n * G + tile - 1) / tile;
         const int each = (items + share_b - 1) / share_b;
         for (int item = sub * each; item < min((sub + 1) * each, items); ++item)
-            f(item, kv8_steps(ctx - n + (min((item + 1) * tile, n * G) - 1) / G + 1, step) * H);
+        {
+            const int n_steps = kv8_steps(ctx - n + (min((item + 1) * tile, n * G) - 1) / G + 1, step);
+            f(item, n_steps ? (n_steps + extra) * H : 0);
+        }
     };
     int mine = 0;
     for (int b = b0; b < b1; ++b) tiles(b, [&](int, int n) { mine += n; });
@@ -260,7 +266,7 @@ __device__ __forceinline__ Kv8Place kv8_find_place(const Kv8Args &c, int G, int 
     int at = inc - mine;
     for (int i = 0; i < wave; ++i) at += s_wave[i];
     const int share = max((total + grid - 1) / grid, 1);
-    const int want = share * w;  // (the host keeps (tiles + grid) * steps below 2^31)
+    const int want = share * w;  // (the host keeps all steps below 2^30, and the grid)
     if (want >= at && want < at + mine) {
         for (int b = b0; b < b1; ++b)
             tiles(b, [&](int item, int n) {

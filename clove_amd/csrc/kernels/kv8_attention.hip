@@ -158,11 +158,9 @@ __device__ void kv8_block_weights(const Kv8Attention &a, const Kv8Split &p, int 
             const int u = i * G + hq % G, item = u / p.tile;
             Kv8Tile T;
             int w0 = 0, np = 1;
-            bool cut = false;
             if (p.join && kv8_tile_of(c, G, b, item, p.tile, &T) && T.high > 0) {
                 const int start = starts[1 + (size_t)(slot + item) * (c.num_heads / p.hw) + h / p.hw];
                 np = kv8_pieces(p, starts[0], start, kv8_steps(T.high, p.step), &w0);
-                cut = start != w0 * starts[0];
             }
             float2 ml = make_float2(-INFINITY, 0.0f);
             if (np <= 1) {
@@ -177,7 +175,7 @@ __device__ void kv8_block_weights(const Kv8Attention &a, const Kv8Split &p, int 
                         const int y = y0 + 16 * z;
                         v[z] = make_float2(-INFINITY, 0.0f);
                         if (y < np)
-                            v[z] = piece_ml[(size_t)(2 * (w0 + y) + (y == 0 && cut ? 1 : 0)) * per_piece +
+                            v[z] = piece_ml[(size_t)(2 * (w0 + y) + (y == 0 ? 1 : 0)) * per_piece +
                                             row];
                     }
 #pragma unroll
@@ -252,9 +250,8 @@ __global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split
     if (np <= 1) return;  // written whole
     if (u >= T.rows) return;
     float top = -INFINITY, l = 0.0f, x[4] = {0.f, 0.f, 0.f, 0.f};
-    // the first piece ends its workgroup's run unless the run begins with it
     const size_t row = (size_t)(h % p.hw) * p.stored + u, per_piece = (size_t)p.hw * p.stored;
-    const size_t first = (2 * w0 + (start != w0 * share ? 1 : 0)) * per_piece + row;
+    const size_t first = (2 * w0 + 1) * per_piece + row;
     const float2 *ml = reinterpret_cast<const float2 *>(a.ws + p.ml_at);
     const float *o = a.ws + p.o_at;
     for (int i0 = wave; i0 < np; i0 += 8 * per) {
@@ -344,7 +341,7 @@ __global__ void __launch_bounds__(256) kv8_join_rows_kernel(Kv8Attention a, Kv8S
     const int u = x / D4, d4 = x - u * D4;
     if (np <= 1 || u >= T.rows) return;  // written whole, or no row
     const size_t row = (size_t)(h % p.hw) * p.stored + u, per_piece = (size_t)p.hw * p.stored;
-    const size_t first = (2 * w0 + (start != w0 * share ? 1 : 0)) * per_piece + row;
+    const size_t first = (2 * w0 + 1) * per_piece + row;
     const float2 *ml = reinterpret_cast<const float2 *>(a.ws + p.ml_at);
     const cl_f4 *o = reinterpret_cast<const cl_f4 *>(a.ws + p.o_at);
     float top = -INFINITY, l = 0.0f;
@@ -429,6 +426,10 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
         p.tile = units <= 64 || p.dp == 256 ? 64 : 128;
         p.hw = 1;
         p.step = p.dp == 256 ? 32 : 64;
+        // A tile's table, rows, first codes and stores take the time of some four
+        // steps: 2048 rows of 32 heads of 80, 175 us when runs are equal in steps
+        // alone, 118 / 105 / 109 with 2 / 4 / 7 more a tile; chunks 160, 150 / 147 / 152.
+        p.extra = 4;
         residents = 2;
     }
     p.stored = !c.row_starts && G < p.tile ? G : p.tile;
@@ -436,7 +437,7 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
     if (tiles >= (1 << 20) || kv8_slots(c, kKv8WeightPart, G, 1) > 65535) return plain();
     const int64_t steps = (cap + p.step - 1) / p.step;
     const int64_t room = std::min(kKv8MaxGrid, cus * residents);
-    if (tiles * steps >= (1ll << 30)) return plain();
+    if (tiles * (steps + p.extra) >= (1ll << 30)) return plain();
     p.join = steps > 1 && (p.kind == KV8_STREAM || tiles < 2 * room);
     p.grid = (int)(p.join || p.kind == KV8_STREAM ? std::min<int64_t>(room, tiles * steps) : tiles);
     if (p.join) {
@@ -454,7 +455,7 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
         } else if (bs % 16 == 0 && 8 * rh * (cap / 16) <= kKv8MaxSums) {
             // Eight bytes for 16 tokens of a row, written on the way and read once,
             // against all scores computed again: 2000 rows in chunks, 24 query
-            // heads of 80, contexts to 3700, 176 against 230 us.  They are stored
+            // heads of 80, contexts to 3700, 176 against 230 us when it came in.  They are stored
             // up to a GiB, a long prompt's are not.
             p.sums = 16;
             p.groups = (int)(cap / 16);

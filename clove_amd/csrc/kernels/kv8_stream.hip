@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(Kv8Attention a, Kv8Split
         return;
     }
     const int w = (int)blockIdx.x;
-    Kv8Place at = kv8_find_place(c, G, H / HW, p.tile, p.step, p.grid, w, s_wave, &s_place);
+    Kv8Place at = kv8_find_place(c, G, H / HW, p.tile, p.step, p.extra, p.grid, w, s_wave, &s_place);
     int *starts = reinterpret_cast<int *>(a.ws + p.start_at);
     if (p.join && w == 0 && tid == 0) starts[0] = at.share;
     const int run = min(at.share, at.total - at.share * w);
@@ -116,7 +116,6 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(Kv8Attention a, Kv8Split
             at.step = 0;
             ++at.h;
         }
-        const bool front = it.b < 0;
         if (left <= 0 || !kv8_next_tile(c, G, H / HW, p.tile, &at, &it.T)) return false;
         const int all = kv8_steps(it.T.high, kStep), s1 = min(all, at.step + left);
         if (p.join && at.step == 0 && tid == 0)
@@ -128,7 +127,7 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(Kv8Attention a, Kv8Split
         it.t_end = min(s1 * kStep, it.T.high);
         it.c1 = min(it.c0 + kChunk, it.t_end);
         it.whole = at.step == 0 && s1 == all;
-        it.piece = (size_t)(2 * w + (front ? 0 : 1)) * HW * p.stored;
+        it.piece = (size_t)(2 * w + (at.step == 0 ? 1 : 0)) * HW * p.stored;
         left -= s1 - at.step;
         return true;
     };

@@ -14,7 +14,7 @@
 //
 // Bound by the matrix cores: a prompt of 4096 rows, 32 heads of 128, takes 137
 // GFLOP once and twice that in pieces, 216 us at the 1271 TFLOP/s of a large bf16
-// product; 280 us measured, 77% of that (three bf16 pieces: 336).  Scores and
+// product; 264 us measured, 82% of that (three bf16 pieces cost 60 us more).  Scores and
 // weights stay in registers: S^T leaves the MFMA in the layout that P^T enters
 // it.  What the vector units do between (the exponentials, the pieces of P, the
 // widening of codes) runs beside the other workgroup's MFMAs.
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
     Kv8Place at;
     int left, run = 0;
     if (p.join) {
-        at = kv8_find_place(c, G, H, p.tile, p.step, p.grid, blockIdx.x, s_wave, &s_place);
+        at = kv8_find_place(c, G, H, p.tile, p.step, p.extra, p.grid, blockIdx.x, s_wave, &s_place);
         run = min(at.share, at.total - at.share * (int)blockIdx.x);
         left = run;
         if (blockIdx.x == 0 && tid == 0)
@@ -172,8 +172,6 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
         at.share = 0;
         left = 1;
     }
-    bool front = true;
-
     while (left > 0) {
         Kv8Tile T;
         if (p.join) {
@@ -182,7 +180,12 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
             return;
         }
         const int h = at.h, all = kv8_steps(T.high, KB);
-        const int s0 = at.step, s1 = p.join ? min(all, s0 + left) : all;
+        if (p.join && at.step < p.extra) {
+            left -= p.extra - at.step;
+            if (left <= 0) return;
+            at.step = p.extra;
+        }
+        const int s0 = p.join ? at.step - p.extra : 0, s1 = p.join ? min(all, s0 + left) : all;
         const int t_end = min(s1 * KB, T.high);
         if (p.join && s0 == 0 && tid == 0)
             reinterpret_cast<int *>(a.ws + p.start_at)
@@ -541,7 +544,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
         }
 
         const bool whole = s0 == 0 && s1 == all;
-        const size_t piece = (size_t)(2 * blockIdx.x + (front ? 0 : 1)) * p.stored;
+        const size_t piece = (size_t)(2 * blockIdx.x + (s0 == 0 ? 1 : 0)) * p.stored;
 #pragma unroll
         for (int cc = 0; cc < NR; ++cc) {
             float ls = l[cc];
@@ -565,7 +568,6 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
             }
         }
         left -= p.join ? s1 - s0 : 1;
-        front = false;
         at.step = 0;
         ++at.h;
     }
