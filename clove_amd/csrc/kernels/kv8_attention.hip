@@ -438,6 +438,8 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
     const int64_t steps = (cap + p.step - 1) / p.step;
     const int64_t room = std::min(kKv8MaxGrid, cus * residents);
     if (tiles * (steps + p.extra) >= (1ll << 30)) return plain();
+    // (the weights' workgroups stand behind the join's, 2^32 threads to a grid)
+    if (a.w_out && (int64_t)((c.max_blocks + 63) / 64) * c.num_seqs >= (1 << 21)) return plain();
     p.join = steps > 1 && (p.kind == KV8_STREAM || tiles < 2 * room);
     p.grid = (int)(p.join || p.kind == KV8_STREAM ? std::min<int64_t>(room, tiles * steps) : tiles);
     if (p.join) {

@@ -10,7 +10,7 @@
 // depend on timing.
 //
 // Bound by latency, a round over the workgroup for each of the keys' bits: 256
-// sequences of 1250 to 4096 blocks down to 1024, 11 us (the weights and tables
+// sequences of 1250 to 4096 blocks down to 1024, 12.5 us (the weights and tables
 // are 4 us of memory traffic; keys read again from memory for every bit, one thread a
 // place: 44), 8 of 63 to 128 blocks 6 us; 15 us each with the call's four
 // allocations and submission.
