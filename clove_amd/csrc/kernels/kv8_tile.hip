@@ -328,10 +328,13 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
             }
             const float k_down = HALF ? kv8_pow2(7 - ke) : 1.0f;
             const float v_down = HALF ? kv8_pow2(7 - ve) : 1.0f;
-            float down[NR];  // a score's factor
+            // A score's factor.  Never 0, which a masked score's -infinity would make
+            // NaN: below 2^-126 (rows of zeros over keys of zeros) the sums, 2^39 at
+            // most, come to nothing under either factor.
+            float down[NR];
 #pragma unroll
             for (int cc = 0; cc < NR; ++cc)
-                down[cc] = HALF ? kv8_pow2(ke - 7) * kv8_pow2(-lift[cc]) : 1.0f;
+                down[cc] = HALF ? fmaxf(kv8_pow2(ke - 7) * kv8_pow2(-lift[cc]), 0x1p-126f) : 1.0f;
             auto rescale = [&](float f) {
                 if (HALF)
 #pragma unroll

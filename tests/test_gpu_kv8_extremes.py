@@ -1,0 +1,67 @@
+"""GPU: attention over the 8-bit cache where magnitudes or sizes are extreme:
+rows and keys of zero or nearly so, values whose exponents lie far apart along a
+context, weights far below the largest, tables far wider than the contexts.
+Bounds as kv8_ref.attention derives them."""
+import numpy as np
+import pytest
+
+import kv8_ref as ref
+from conftest import rng
+from test_gpu_kv8 import check_attention, up, within
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- zero rows over zero keys ---------------------------------------------------
+
+# rows and earlier tokens of each sequence: a prompt; chunks cut over workgroups
+PROMPT, CUT = ([150], [0]), ([130, 70], [5000, 40])
+
+
+@pytest.mark.parametrize("rows,past", [PROMPT, CUT])
+@pytest.mark.parametrize("D,H,Hq", [(64, 2, 2), (80, 2, 6), (128, 2, 2), (256, 1, 2)])
+@pytest.mark.parametrize("what", ["all", "head", "rows", "tiny", "tinier"])
+def test_zero_and_tiny_rows_over_zero_and_tiny_keys(hip, D, H, Hq, rows, past, what):
+    """Scores that are all 0 (or too small to matter): a row's answer is the mean
+    of the values that it sees, in whatever form the kernel holds rows and keys.
+    all: a prompt of zeros; head: one kv head's rows and keys; rows: every third
+    row over tiny keys; tiny, tinier: small rows over small keys."""
+    g = rng(D + len(rows) + len(what))
+    bs = 16
+    lens = np.add(rows, past).astype(np.int32)
+    tables, nb = ref.pool(g, lens, bs, -(-int(lens.max()) // bs))
+    codes, exps = ref.cache(g, nb, H, bs, D)
+    q = g.standard_normal((sum(rows), Hq * D)).astype(np.float32)
+    heads = q.reshape(-1, H, Hq // H * D)
+    if what == "all":
+        codes[0], exps[0], q[:] = 0, -60, 0
+    elif what == "head":
+        codes[0, :, H - 1], exps[0, :, H - 1], heads[:, H - 1] = 0, -60, 0
+    elif what == "rows":
+        exps[0] -= 45
+        q[::3] = 0
+    elif what == "tiny":
+        exps[0] -= 40
+        q *= np.float32(2.0 ** -100)
+    else:
+        exps[0], codes[0, :, :, :, ::2] = -60, 0
+        q *= np.float32(2.0 ** -120)
+    check_attention(hip, q, codes, exps, tables, lens, ref.starts_of(rows),
+                    weights=g.random(tables.shape).astype(np.float32))
+
+
+def test_a_prompt_of_zeros_through_the_append(hip):
+    """What a dummy pass of zeros stores and reads."""
+    g = rng(61)
+    H, D, bs, n = 2, 64, 16, 200
+    lens, starts = np.array([n], np.int32), np.array([0, n], np.int32)
+    tables, nb = ref.pool(g, lens, bs, 13)
+    codes, exps = ref.cache(g, nb, H, bs, D)
+    zero = np.zeros((n, H * D), np.float32)
+    tc, te, tz, tt, tl, ts = up(hip, codes, exps, zero, tables, lens, starts)
+    hip.paged_kv8_append(tc, te, tz, tz, tt, tl, ts)
+    out, w = hip.paged_kv8_attention(tz, tc, te, tt, tl, ts,
+                                     weights=hip.tensor(np.zeros(tables.shape, np.float32)))
+    assert not out.numpy().any()
+    # a row's weights add up to 1 for each of H heads; n + 16 roundings a row and head
+    assert abs(float(w.numpy().astype(np.float64).sum()) - n * H) < n * H * (n + 16) * 2.0 ** -23
