@@ -143,7 +143,8 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
     const int H = c.num_heads, G = a.q_heads / H, D = c.head_dim, bs = c.block_size;
     __shared__ uint2 table[kChunk / 4];
     __shared__ __attribute__((aligned(16))) uint8_t sK[2][KB * PK], sV[2][DP * PV];
-    __shared__ int s_wave[4], s_range[6];  // (the last two: bad; lost, as a float's bits)
+    // fill_table's, then: bad; lost, as a float's bits; values' largest exponent so far
+    __shared__ int s_wave[4], s_range[7];
     __shared__ Kv8Place s_place;
 
     if ((int)blockIdx.x >= p.grid) {
@@ -249,6 +250,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
         };
         // the rows' loads run beside the table's
         u4 qf[NR][KI][HALF ? 2 : 3];
+        if (tid == 0) s_range[6] = -1000;
         {
             cl_f4 raw[NR][KI][2];
 #pragma unroll
@@ -319,13 +321,16 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
             // octaves of the tiles' exponents; with rows and weights lifted likewise,
             // two pieces of each do what three bf16 ones do, if what the rows lost
             // moves no score (base 2) by more than 2^-22, a quarter of a weight's ulp.
+            // The sums over the values so far (2^55 2^v_top at most: 2^31 tokens with
+            // weights to 2^15) take on this chunk's factor 2^(7 - ve) inside f32's range.
             const int ke = s_range[0], ve = s_range[2];
             if (HALF && (ke == -1000 || ke > 60 || ke + s_range[1] > 22 || ve > 60 ||
-                         ve + s_range[3] > 22 ||
+                         ve + s_range[3] > 22 || s_range[6] > ve + 60 ||
                          lost * (0x1p-17f * kE4m3Max) * kv8_pow2(ke) > 1.0f)) {
                 if (tid == 0) *declined = 1;
                 return;
             }
+            if (HALF && tid == 0) s_range[6] = max(s_range[6], ve);  // (no condition changes by it)
             const float k_down = HALF ? kv8_pow2(7 - ke) : 1.0f;
             const float v_down = HALF ? kv8_pow2(7 - ve) : 1.0f;
             // A score's factor.  Never 0, which a masked score's -infinity would make

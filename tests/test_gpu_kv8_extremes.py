@@ -65,3 +65,45 @@ def test_a_prompt_of_zeros_through_the_append(hip):
     assert not out.numpy().any()
     # a row's weights add up to 1 for each of H heads; n + 16 roundings a row and head
     assert abs(float(w.numpy().astype(np.float64).sum()) - n * H) < n * H * (n + 16) * 2.0 ** -23
+
+
+# ---- values of very different sizes along a context ----------------------------
+
+def check_some_rows(hip, q, codes, exps, tables, ctx, past, heads, rows):
+    """One sequence's attention; `rows` of `heads` against the definition, each
+    as a sequence of its own that ends at the row's position."""
+    H, D = codes.shape[2], codes.shape[4]
+    n = len(q)
+    got = hip.paged_kv8_attention(*up(hip, q, codes, exps, tables, np.array([ctx], np.int32),
+                                      np.array([0, n], np.int32))).numpy().reshape(n, H, D)
+    hip.synchronize()
+    rows = np.array(rows)
+    for h in heads:
+        want, _, tol, _ = ref.attention(q.reshape(n, H, D)[rows, h], codes[:, :, h:h + 1],
+                                        exps[:, :, h:h + 1], np.repeat(tables, len(rows), 0),
+                                        past + rows + 1)
+        within(got[rows, h], want, tol, f"head {h}")
+
+
+@pytest.mark.parametrize("D,H,n,past", [(64, 64, 2048, 6000), (128, 64, 2048, 6000),
+                                        (256, 16, 4096, 0)])
+@pytest.mark.parametrize("first,then", [(45, None), (45, -55), (-55, 45), (None, 45), (60, -60)])
+def test_values_of_different_sizes_along_a_context(hip, D, H, n, past, first, then):
+    """Value exponents of a context's first tokens and of those behind them (None:
+    zeros, as the append stores them), far apart; enough tiles that each workgroup
+    walks a whole context and meets both."""
+    g = rng(D + H)
+    bs, ctx = 16, past + n
+    tables, nb = ref.pool(g, [ctx], bs, -(-ctx // bs))
+    codes = np.empty((2, nb, H, bs, D), np.uint8)
+    some, _ = ref.cache(g, 40, 1, bs, D)  # (random codes, repeated: they are many)
+    codes[:] = some[:, g.integers(0, 40, nb * H), 0].reshape(2, nb, H, bs, D)
+    exps = np.full((2, nb, H), -8, np.int32)
+    half = (2048 if D > 128 else 4096) // bs
+    for ids, e in ((tables[0, :half], first), (tables[0, half:], then)):
+        exps[1, ids] = -60 if e is None else e
+        if e is None:
+            codes[1, ids] = 0
+    q = g.standard_normal((n, H * D), np.float32)
+    check_some_rows(hip, q, codes, exps, tables, ctx, past, (0, H - 1),
+                    (0, 1, n // 2 - 1, n // 2, n - 100, n - 1))
