@@ -7,14 +7,16 @@
 // values as columns of eight tokens; the next step's codes are on their way from
 // memory meanwhile.  The products are those of kv8_stream.hip (S^T = K Q^T with
 // q, O^T = V^T P^T with P, as three bf16 pieces each), and an operand read from
-// LDS feeds 3 * NR MFMAs.  Where the exponents of the tiles and the magnitudes
-// within each row of q lie close enough together, which is nearly always, f16
-// takes the place of bf16: two pieces of 11 bits do for q and P what three of 8
-// bits do, two thirds of the MFMAs.
+// LDS feeds 3 * NR MFMAs.  Where the exponents of the keys' tiles and the magnitudes
+// within each row of q lie close enough together, which is nearly always, the
+// scores take f16 in the place of bf16: two pieces of 11 bits hold q to 2^-23 of
+// itself, two thirds of the MFMAs.  P stays in bf16: f16 ends at 2^-24, and a weight
+// that far below the largest is all there is where the tokens ahead have no value.
 //
-// Bound by the matrix cores: a prompt of 4096 rows, 32 heads of 128, takes 137
-// GFLOP once and twice that in pieces, 216 us at the 1271 TFLOP/s of a large bf16
-// product; 264 us measured, 82% of that (three bf16 pieces cost 60 us more).  Scores and
+// Bound by the matrix cores: a prompt of 4096 rows, 32 heads of 128, takes 69
+// GFLOP for the scores and as many for the sums over V, in two and three pieces:
+// 270 us at the 1271 TFLOP/s of a large bf16 product; 313 to 322 us measured (all in
+// bf16 pieces 333; P in two f16 pieces as well 264 to 270, less what they lose).  Scores and
 // weights stay in registers: S^T leaves the MFMA in the layout that P^T enters
 // it.  What the vector units do between (the exponentials, the pieces of P, the
 // widening of codes) runs beside the other workgroup's MFMAs.
@@ -89,10 +91,10 @@ __device__ __forceinline__ void split_half(float a, float b, unsigned *w1, unsig
 // tokens' first and the scales of its key and value tile as bf16, 0 outside the
 // pool.  Tokens behind the end take the first place.  True: some are outside.
 // range (-1000s before): the keys' largest exponent and their least one's
-// negative, then the values'.
+// negative.
 __device__ __forceinline__ int fill_table(const Kv8Args &c, int b, int h, int c0, int c1,
                                           int step, uint2 *table, int *range = nullptr) {
-    int bad = 0, ends[4] = {-1000, -1000, -1000, -1000};
+    int bad = 0, ends[2] = {-1000, -1000};
     for (int i = threadIdx.x; i < (c1 - c0 + step - 1) / step * (step / 4); i += 256) {
         const int t = c0 + 4 * i < c1 ? c0 + 4 * i : c0;
         const int64_t id = kv8_block(c, b, t / c.block_size, h == 0);
@@ -101,18 +103,16 @@ __device__ __forceinline__ int fill_table(const Kv8Args &c, int b, int h, int c0
             e.x = (unsigned)((id * c.num_heads + h) * c.block_size + t % c.block_size);
             e.y = __float_as_uint(kv8_scale(c.exps[kv8_tile(c, 0, id, h)])) |
                   __float_as_uint(kv8_scale(c.exps[kv8_tile(c, 1, id, h)])) >> 16;
-            const int ke = (int)(e.y >> 23) - 127, ve = (int)(e.y >> 7 & 255) - 127;
+            const int ke = (int)(e.y >> 23) - 127;
             ends[0] = max(ends[0], ke);
             ends[1] = max(ends[1], -ke);
-            ends[2] = max(ends[2], ve);
-            ends[3] = max(ends[3], -ve);
         }
         bad |= id < 0;
         table[i] = e;
     }
     if (range) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 2; ++j) {
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) ends[j] = max(ends[j], __shfl_xor(ends[j], o, 64));
             if ((threadIdx.x & 63) == 0) atomicMax(&range[j], ends[j]);
@@ -122,8 +122,8 @@ __device__ __forceinline__ int fill_table(const Kv8Args &c, int b, int h, int c0
 }
 
 // FULL: head_dim = DP; else MFMA steps and blocks past it are left out.
-// HALF: f16 pieces, two of each; a workgroup whose tiles or rows do not let it
-// leaves its run to the bf16 form (p.declined), which otherwise finds nothing to do.
+// HALF: q in two f16 pieces; a workgroup whose keys or rows do not let it leaves
+// its run to the bf16 form (p.declined), which otherwise finds nothing to do.
 // SUMS: the weights of every 16 tokens go out, for kv8_tile_weights.
 template <int DP, int NR, bool FULL, bool HALF, bool SUMS>
 __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p) {
@@ -143,8 +143,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
     const int H = c.num_heads, G = a.q_heads / H, D = c.head_dim, bs = c.block_size;
     __shared__ uint2 table[kChunk / 4];
     __shared__ __attribute__((aligned(16))) uint8_t sK[2][KB * PK], sV[2][DP * PV];
-    // fill_table's, then: bad; lost, as a float's bits; values' largest exponent so far
-    __shared__ int s_wave[4], s_range[7];
+    __shared__ int s_wave[4], s_range[4];  // (the last two: bad; lost, as a float's bits)
     __shared__ Kv8Place s_place;
 
     if ((int)blockIdx.x >= p.grid) {
@@ -242,15 +241,14 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
 
         // the table of the chunk from c0 on, whole at the next barrier
         auto next_table = [&](int c0) {
-            if (tid < 6) s_range[tid] = tid < 4 ? -1000 : 0;
+            if (tid < 4) s_range[tid] = tid < 2 ? -1000 : 0;
             __syncthreads();  // the table and tiles before are done with
             const int c1 = min(c0 + kChunk, t_end);
             if (__any(fill_table(c, at.b, h, c0, c1, KB, table, s_range)) && lane == 0)
-                s_range[4] = 1;
+                s_range[2] = 1;
         };
         // the rows' loads run beside the table's
         u4 qf[NR][KI][HALF ? 2 : 3];
-        if (tid == 0) s_range[6] = -1000;
         {
             cl_f4 raw[NR][KI][2];
 #pragma unroll
@@ -291,7 +289,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                     small += __shfl_xor(small, 32, 64);
                     lift[cc] = min(14 + 127 - (int)(__float_as_uint(most) >> 23), 100);
                     if (q == 0)
-                        atomicMax(&s_range[5],
+                        atomicMax(&s_range[3],
                                   __float_as_int(lift[cc] < -60 ? INFINITY : small * most));
                     const float up = kv8_pow2(max(lift[cc], -126));
 #pragma unroll
@@ -308,7 +306,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
             }
         }
         __syncthreads();
-        const float lost = HALF ? __int_as_float(s_range[5]) : 0.0f;
+        const float lost = HALF ? __int_as_float(s_range[3]) : 0.0f;
 
         for (int c0 = s0 * KB; c0 < t_end; c0 += kChunk) {
             const int c1 = min(c0 + kChunk, t_end);
@@ -316,23 +314,18 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                 next_table(c0);
                 __syncthreads();
             }
-            const bool bad = s_range[4];
+            const bool bad = s_range[2];
             // f16 holds codes times 2^(exponent - the largest + 7) exactly over 22
-            // octaves of the tiles' exponents; with rows and weights lifted likewise,
-            // two pieces of each do what three bf16 ones do, if what the rows lost
-            // moves no score (base 2) by more than 2^-22, a quarter of a weight's ulp.
-            // The sums over the values so far (2^55 2^v_top at most: 2^31 tokens with
-            // weights to 2^15) take on this chunk's factor 2^(7 - ve) inside f32's range.
-            const int ke = s_range[0], ve = s_range[2];
-            if (HALF && (ke == -1000 || ke > 60 || ke + s_range[1] > 22 || ve > 60 ||
-                         ve + s_range[3] > 22 || s_range[6] > ve + 60 ||
+            // octaves of the tiles' exponents; with rows lifted likewise, two pieces
+            // do what three bf16 ones do, if what the rows lost moves no score
+            // (base 2) by more than 2^-22, a quarter of a weight's ulp.
+            const int ke = s_range[0];
+            if (HALF && (ke == -1000 || ke > 60 || ke + s_range[1] > 22 ||
                          lost * (0x1p-17f * kE4m3Max) * kv8_pow2(ke) > 1.0f)) {
                 if (tid == 0) *declined = 1;
                 return;
             }
-            if (HALF && tid == 0) s_range[6] = max(s_range[6], ve);  // (no condition changes by it)
             const float k_down = HALF ? kv8_pow2(7 - ke) : 1.0f;
-            const float v_down = HALF ? kv8_pow2(7 - ve) : 1.0f;
             // A score's factor.  Never 0, which a masked score's -infinity would make
             // NaN: below 2^-126 (rows of zeros over keys of zeros) the sums, 2^39 at
             // most, come to nothing under either factor.
@@ -340,14 +333,6 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
 #pragma unroll
             for (int cc = 0; cc < NR; ++cc)
                 down[cc] = HALF ? fmaxf(kv8_pow2(ke - 7) * kv8_pow2(-lift[cc]), 0x1p-126f) : 1.0f;
-            auto rescale = [&](float f) {
-                if (HALF)
-#pragma unroll
-                    for (int cc = 0; cc < NR; ++cc)
-#pragma unroll
-                        for (int jb = 0; jb < JB; ++jb) o[cc][jb] *= f;
-            };
-            rescale(v_down);
             u4 rk[NK];
             unsigned rv[4][JV / 4];
             float ksc[NK], vsc;
@@ -364,7 +349,6 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                 }
                 const uint2 e = table[((kb - c0) >> 2) + vquad];
                 vsc = __uint_as_float(e.y << 16);
-                if (HALF) vsc *= v_down;
                 const uint8_t *row = vbase + (size_t)e.x * D;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -407,7 +391,7 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                         unsigned w[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            w[i] = hi ? widen<HALF, true>(rv[i][e], vsc) : widen<HALF, false>(rv[i][e], vsc);
+                            w[i] = hi ? kv8_widen<true>(rv[i][e], vsc) : kv8_widen<false>(rv[i][e], vsc);
                         uint8_t *to = &sV[buf][(vdim + 4 * e + 2 * hi) * PV + 2 * vpos];
                         *reinterpret_cast<uint2 *>(to) =
                             make_uint2(__builtin_amdgcn_perm(w[1], w[0], 0x05040100u),
@@ -475,16 +459,13 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                         for (int u = 0; u < 2; ++u)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) top = fmaxf(top, s[cc][u][i]);
-                        // weights are up to 2^8 with bf16 pieces; with f16 ones, which are
-                        // off by 2^-25 or less, the largest is 2^10 .. 2^15
-                        constexpr float kMost = HALF ? 15.0f : kKv8Slack, kAim = HALF ? 10.0f : 0.0f;
                         if (HALF) top *= down[cc];
-                        if (__any(top > m[cc] + kMost)) {
+                        if (__any(top > m[cc] + kKv8Slack)) {
                             // a row moves its maximum by its own scores alone, so
                             // that its bits do not depend on the rows beside it
                             top = fmaxf(top, __shfl_xor(top, 16, 64));
                             top = fmaxf(top, __shfl_xor(top, 32, 64));
-                            const float m_new = top > m[cc] + kMost ? top - kAim : m[cc];
+                            const float m_new = top > m[cc] + kKv8Slack ? top : m[cc];
                             const float f0 =
                                 m_new == m[cc] ? 1.0f : __builtin_amdgcn_exp2f(m[cc] - m_new);
                             l[cc] *= f0;
@@ -504,12 +485,9 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                             l[cc] += part_sum[u];
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                unsigned w1, w2, w3 = 0;
-                                if constexpr (HALF)
-                                    split_half(s[cc][u][2 * e], s[cc][u][2 * e + 1], &w1, &w2);
-                                else
-                                    split_pair<false>(s[cc][u][2 * e], s[cc][u][2 * e + 1], &w1,
-                                                      &w2, &w3);
+                                unsigned w1, w2, w3;
+                                split_pair<false>(s[cc][u][2 * e], s[cc][u][2 * e + 1], &w1, &w2,
+                                                  &w3);
                                 pf[cc][0][2 * u + e] = w1;
                                 pf[cc][1][2 * u + e] = w2;
                                 pf[cc][2][2 * u + e] = w3;
@@ -536,19 +514,18 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
                             v[i] = *reinterpret_cast<const u4 *>(
                                 &sV[buf][(16 * (jb + i) + r) * PV + 64 * sub + 16 * q]);
 #pragma unroll
-                        for (int x = HALF ? 1 : 2; x >= 0; --x)
+                        for (int x = 2; x >= 0; --x)
 #pragma unroll
                             for (int cc = 0; cc < NR; ++cc)
 #pragma unroll
                                 for (int i = 0; i < JG; ++i)
-                                    o[cc][jb + i] = product<HALF>(v[i], pf[cc][x], o[cc][jb + i]);
+                                    o[cc][jb + i] = mfma(v[i], pf[cc][x], o[cc][jb + i]);
                     }
                 }
                 __builtin_amdgcn_s_setprio(0);
                 if (more) store(kb + KB, buf ^ 1);
                 __syncthreads();
             }
-            if (HALF) rescale(kv8_pow2(ve - 7));
         }
 
         const bool whole = s0 == 0 && s1 == all;

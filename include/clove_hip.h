@@ -285,7 +285,11 @@ int clove_hip_paged_kv8_read(CTensor codes, CTensor exps, CTensor block_tables,
  * weights (f32 [B, max_blocks]) and weights_out go together, both or neither:
  * *weights_out receives a new tensor weights[b][j] + the sum, over the rows and
  * query heads of sequence b and the tokens of its block j, of the softmax
- * weights; entries past a context are copied.  Sums run in a fixed order. */
+ * weights; entries past a context are copied.  Sums run in a fixed order.
+ * Products are those of 32-bit values with 32-bit sums, but for q where sequences
+ * have many rows: its elements may then be off by 2^-23 of themselves, and those
+ * below 2^-17 of their row's largest together by what moves a score by 2^-22 at
+ * most.  A row's bits may thus depend on how many rows the call has. */
 CTensor clove_hip_paged_kv8_attention(CTensor q, CTensor codes, CTensor exps,
                                       CTensor block_tables, CTensor context_lens,
                                       CTensor row_starts, float scale, CTensor weights,

@@ -107,3 +107,28 @@ def test_values_of_different_sizes_along_a_context(hip, D, H, n, past, first, th
     q = g.standard_normal((n, H * D), np.float32)
     check_some_rows(hip, q, codes, exps, tables, ctx, past, (0, H - 1),
                     (0, 1, n // 2 - 1, n // 2, n - 100, n - 1))
+
+
+# ---- weights far below the largest ------------------------------------------------
+
+@pytest.mark.parametrize("lead", [20, 24, 28, 33, 36, 40])
+@pytest.mark.parametrize("rows,past", [(8, 192), (60, 140), (130, 70), (130, 5000)])
+def test_small_weights_beside_a_token_without_value(hip, lead, rows, past):
+    """A token 2^lead ahead of the others whose value is 0, in all dims or in every
+    other: what the others' weights make has to keep its own precision."""
+    g = rng(lead + rows)
+    H, D, bs, n = 2, 64, 16, rows + past
+    lens = np.array([n], np.int32)
+    tables, nb = ref.pool(g, lens, bs, -(-n // bs))
+    codes, exps = ref.cache(g, nb, H, bs, D)
+    exps[0] = -10
+    q = g.standard_normal((rows, H * D)).astype(np.float32)
+    q.reshape(rows, H, D)[:, :, 0] = 5.0
+    codes[0, :, :, :, 0] = 0
+    codes[0, tables[0, 2]] = 0
+    codes[1, tables[0, 2], 0, 5] = 0
+    codes[1, tables[0, 2], 1, 5, ::2] = 0
+    codes[0, tables[0, 2], :, 5, 0] = ref.encode(np.array(lead * np.log(2) / 5 * 64))
+    exps[0, tables[0, 2]] = -6
+    check_attention(hip, q, codes, exps, tables, lens, np.array([0, rows], np.int32), scale=1.0,
+                    weights=np.zeros(tables.shape, np.float32))
