@@ -180,6 +180,9 @@ struct Kv8Split {
     int stored;        // rows of a piece
     int sums;          // tokens to a stored sum of weights, 0: none stored
     int groups;        // such sums a row
+    int range;         // none stored: tokens whose scores are computed again at a time
+    bool late;         // the blocks' weights come behind the join, which then leaves
+                       // every row's maximum and sum
     // in the workspace, in floats
     size_t o_at, ml_at;      // piece 2w (+ 1: begins a tile) of workgroup w: of hw
                              // heads `stored` sums over V [D], and (maximum, sum) pairs
@@ -344,11 +347,14 @@ __device__ __forceinline__ unsigned kv8_widen(unsigned codes, float scale) {
 int kv8_stream_residents();
 void kv8_stream(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
 void kv8_tiles(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
-// The weights of the blocks (kv8_tiles has left every row's maximum and sum): from
-// sums that it stored as well, or the scores computed again.
+// The weights of the blocks, p.late: from sums that kv8_tiles stored, or the scores
+// computed again.
 constexpr int kKv8WeightPart = 512;
-constexpr int64_t kKv8MaxSums = 1ll << 30;  // bytes of such sums
-void kv8_tile_weights(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
+// Bytes of sums, however wide the tables are: where a sum for every 16 or 4 tokens of
+// the tables and every row and head would take more, the scores are computed again, a
+// range of the tables' blocks at a time.
+constexpr int64_t kKv8MaxSums = 1ll << 30;
+void kv8_late_weights(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
 
 }  // namespace k
 }  // namespace clove

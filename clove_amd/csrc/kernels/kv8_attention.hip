@@ -312,8 +312,7 @@ __global__ void __launch_bounds__(1024) kv8_join_kernel(Kv8Attention a, Kv8Split
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (lane + 64 * e < D) a.out[rh * D + lane + 64 * e] = x[e] * inv;
-    // (for the tiles' weights)
-    if (lane == 0 && a.w_out && p.kind == KV8_TILE)
+    if (lane == 0 && p.late)
         reinterpret_cast<float2 *>(a.ws + p.row_ml_at)[rh] = make_float2(top, inv);
 }
 
@@ -373,7 +372,7 @@ __global__ void __launch_bounds__(256) kv8_join_rows_kernel(Kv8Attention a, Kv8S
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const size_t rh = (size_t)(T.first + (T.r0 + u) / G) * a.q_heads + h * G + (T.r0 + u) % G;
     reinterpret_cast<cl_f4 *>(a.out)[rh * D4 + d4] = sum * inv;
-    if (d4 == 0 && a.w_out && p.kind == KV8_TILE)
+    if (d4 == 0 && p.late)
         reinterpret_cast<float2 *>(a.ws + p.row_ml_at)[rh] = make_float2(top, inv);
 }
 
@@ -450,22 +449,25 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
     if (p.kind == KV8_TILE) p.declined_at = take(p.grid);
     if (a.w_out) {
         p.row_ml_at = take(2 * rh);
-        if (p.kind == KV8_STREAM) {
-            p.sums = bs % 16 == 0 ? 16 : 4;
-            p.groups = (int)((cap + p.sums - 1) / p.sums);
-            p.sums_at = take(2 * rh * p.groups);
-        } else if (bs % 16 == 0 && 8 * rh * (cap / 16) <= kKv8MaxSums) {
-            // Eight bytes for 16 tokens of a row, written on the way and read once,
-            // against all scores computed again: 2000 rows in chunks, 24 query
-            // heads of 80, contexts to 3700, 176 against 230 us when it came in.  They are stored
-            // up to a GiB, a long prompt's are not.
-            p.sums = 16;
-            p.groups = (int)(cap / 16);
+        // Eight bytes for 16 tokens of a row, written on the way and read once,
+        // against all scores computed again: 2000 rows in chunks, 24 query
+        // heads of 80, contexts to 3700, 176 against 230 us when it came in.  They are
+        // stored up to a GiB; a long prompt's are not, nor those of very wide tables.
+        const int sums = bs % 16 == 0 ? 16 : 4;
+        const int64_t pairs = kv8_slots(c, kKv8WeightPart, G, 1) * c.num_heads;
+        if ((p.kind == KV8_STREAM || sums == 16) && 8 * rh * (cap / sums) <= kKv8MaxSums) {
+            p.sums = sums;
+            p.groups = (int)(cap / sums);
             p.sums_at = take(2 * rh * p.groups);
         } else {
-            p.groups = (int)((cap + 3) / 4);
-            p.sums_at = take(kv8_slots(c, kKv8WeightPart, G, 1) * c.num_heads * p.groups);
+            // four bytes for four tokens of a part of a sequence's rows
+            const int64_t blocks = std::min<int64_t>(kKv8MaxSums / (pairs * bs), c.max_blocks);
+            if (blocks == 0) return plain();
+            p.range = (int)(blocks * bs);
+            p.groups = p.range / 4;
+            p.sums_at = take(pairs * p.groups);
         }
+        p.late = p.kind == KV8_TILE || !p.sums;
     }
     return p;
 }
@@ -491,9 +493,9 @@ void kv8_attention(const Kv8Attention &a, int cus, hipStream_t s) {
         kv8_stream(a, p, s);
     else
         kv8_tiles(a, p, s);
-    // the blocks' weights: with the join, or after the tiles' one
+    // the blocks' weights: with the join, or behind it
     const unsigned blocks =
-        weights && p.kind == KV8_STREAM ? (unsigned)((c.max_blocks + 63) / 64) * c.num_seqs : 0;
+        weights && !p.late ? (unsigned)((c.max_blocks + 63) / 64) * c.num_seqs : 0;
     if (p.join) {
         const unsigned tiles = (unsigned)kv8_slots(c, p.tile, a.q_heads / c.num_heads, 1) * c.num_heads;
         // pieces to a tile: 2 on the average where there are as many tiles as runs
@@ -511,7 +513,7 @@ void kv8_attention(const Kv8Attention &a, int cus, hipStream_t s) {
     } else if (blocks) {
         kv8_weights_kernel<<<blocks, 256, 0, s>>>(a, p);
     }
-    if (weights && p.kind == KV8_TILE) kv8_tile_weights(a, p, s);
+    if (weights && p.late) kv8_late_weights(a, p, s);
 }
 
 }  // namespace k

@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(Kv8Attention a, Kv8Split
         if (q == 0) {
             if (!it.whole)
                 reinterpret_cast<float2 *>(a.ws + p.ml_at)[piece] = make_float2(mm, ll);
-            else if (SUMS)
+            else if (a.w_out)
                 reinterpret_cast<float2 *>(a.ws + p.row_ml_at)[rh] = make_float2(mm, inv);
         }
     };

@@ -124,7 +124,7 @@ __device__ __forceinline__ int fill_table(const Kv8Args &c, int b, int h, int c0
 // FULL: head_dim = DP; else MFMA steps and blocks past it are left out.
 // HALF: q in two f16 pieces; a workgroup whose keys or rows do not let it leaves
 // its run to the bf16 form (p.declined), which otherwise finds nothing to do.
-// SUMS: the weights of every 16 tokens go out, for kv8_tile_weights.
+// SUMS: the weights of every 16 tokens go out, for kv8_late_weights.
 template <int DP, int NR, bool FULL, bool HALF, bool SUMS>
 __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p) {
     constexpr int KI = DP / 32;               // MFMA steps of q . k
@@ -563,17 +563,17 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
 // MFMA operands in registers, and walks the rows that see them, 32 at a time, in
 // pieces through LDS (the next 32 on their way meanwhile).  A row's weights are
 // 2^(s - m) / sum.  Long runs of rows are cut into parts of kPart pairs, each with
-// sums of its own.
+// sums of its own.  One launch is for tokens [t0, t1), a range of whole blocks.
 constexpr int kPart = kKv8WeightPart;
 template <int DP>
 __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
-    tile_weights_kernel(Kv8Attention a, Kv8Split p) {
+    tile_weights_kernel(Kv8Attention a, Kv8Split p, int t0, int t1) {
     constexpr int KI = DP / 32;
     const Kv8Args &c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r = lane & 15, q = lane >> 4;
     const int H = c.num_heads, G = a.q_heads / H, D = c.head_dim;
-    const int h = blockIdx.y, slot = blockIdx.z, c0 = blockIdx.x * 256;
+    const int h = blockIdx.y, slot = blockIdx.z, c0 = t0 + blockIdx.x * 256;
     constexpr int NQ = (2 * KI * 64 + 255) / 256;  // eight dims of a row each
     __shared__ uint2 table[64];
     __shared__ u4 sq[2][2 * KI * 3 * 64];
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
     const int b = kv8_slot(c, slot, kPart, G, 1, &part);
     int first, n;
     kv8_rows(c, b, &first, &n);
-    const int ctx = kv8_context(c, b), c1 = min(c0 + 256, ctx);
+    const int ctx = kv8_context(c, b), c1 = min(c0 + 256, min(t1, ctx));
     if (part < 0 || part * kPart >= n * G || c0 >= c1) return;
     const int bad = __syncthreads_or(fill_table(c, b, 0, c0, c1, 256, table));
     // the keys: token 16u + r of the wave's, dims 32i + 8q .. + 7
@@ -708,34 +708,35 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2)
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) x += __shfl_xor(x, o, 64);
         const int t = c0 + 64 * wave + 16 * u + 4 * q;
-        if (r == 0 && t < c1) out[t >> 2] = x;
+        if (r == 0 && t < c1) out[(t - t0) >> 2] = x;
     }
 }
 
-// The quads' sums of all parts and heads into the blocks' weights; lanes take 64
-// blocks, the sixteen waves the parts and heads in turn.
-__global__ void __launch_bounds__(1024) block_weights_kernel(Kv8Attention a, Kv8Split p) {
+// The quads' sums of all parts and heads into the weights of blocks [j0, j1); lanes
+// take 64 blocks, the sixteen waves the parts and heads in turn.
+__global__ void __launch_bounds__(1024)
+    block_weights_kernel(Kv8Attention a, Kv8Split p, int j0, int j1) {
     const Kv8Args &c = a.c;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int j = blockIdx.x * 64 + lane, b = blockIdx.y, per = c.block_size / 4;
+    const int j = j0 + blockIdx.x * 64 + lane, b = blockIdx.y, per = c.block_size / 4;
     __shared__ float part[16][64];
     const int ctx = kv8_context(c, b);
     int first, n;
     kv8_rows(c, b, &first, &n);
     float w = 0.0f;
-    if (n > 0 && j < c.max_blocks && j * c.block_size < ctx) {
+    if (n > 0 && j < j1 && j * c.block_size < ctx) {
         const int G = a.q_heads / c.num_heads, quads = min(per, (ctx - j * c.block_size + 3) / 4);
         const int parts = (n * G + kPart - 1) / kPart;
         const size_t slot = kv8_first_slot(c, b, kPart, G, 1);
         for (int x = wave; x < parts * c.num_heads; x += 16) {
-            const float *y = a.ws + p.sums_at + (slot * c.num_heads + x) * p.groups + (size_t)j * per;
+            const float *y = a.ws + p.sums_at + (slot * c.num_heads + x) * p.groups + (size_t)(j - j0) * per;
 #pragma unroll 4
             for (int i = 0; i < quads; ++i) w += y[i];
         }
     }
     part[wave][lane] = w;
     __syncthreads();
-    if (wave == 0 && j < c.max_blocks) {
+    if (wave == 0 && j < j1) {
         const size_t at = (size_t)b * c.max_blocks + j;
         for (int x = 1; x < 16; ++x) w += part[x][lane];
         a.w_out[at] = a.w_in[at] + w;
@@ -839,7 +840,7 @@ void kv8_tiles(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
     }
 }
 
-void kv8_tile_weights(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
+void kv8_late_weights(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
     const Kv8Args &c = a.c;
     if (p.sums) {
         const int blocks = std::max(1, 64 / c.block_size);
@@ -847,12 +848,17 @@ void kv8_tile_weights(const Kv8Attention &a, const Kv8Split &p, hipStream_t s) {
             a, p, blocks);
         return;
     }
-    const dim3 grid((c.max_blocks * c.block_size + 255) / 256, c.num_heads,
-                    (unsigned)kv8_slots(c, kPart, a.q_heads / c.num_heads, 1));
-    if (p.dp == 64) tile_weights_kernel<64><<<grid, 256, 0, s>>>(a, p);
-    if (p.dp == 128) tile_weights_kernel<128><<<grid, 256, 0, s>>>(a, p);
-    if (p.dp == 256) tile_weights_kernel<256><<<grid, 256, 0, s>>>(a, p);
-    block_weights_kernel<<<dim3((c.max_blocks + 63) / 64, c.num_seqs), 1024, 0, s>>>(a, p);
+    const int per = p.range / c.block_size;
+    const unsigned parts = (unsigned)kv8_slots(c, kPart, a.q_heads / c.num_heads, 1);
+    for (int j0 = 0; j0 < c.max_blocks; j0 += per) {
+        const int n = std::min(per, c.max_blocks - j0), t0 = j0 * c.block_size;
+        const int t1 = t0 + n * c.block_size;
+        const dim3 grid((n * c.block_size + 255) / 256, c.num_heads, parts);
+        if (p.dp == 64) tile_weights_kernel<64><<<grid, 256, 0, s>>>(a, p, t0, t1);
+        if (p.dp == 128) tile_weights_kernel<128><<<grid, 256, 0, s>>>(a, p, t0, t1);
+        if (p.dp == 256) tile_weights_kernel<256><<<grid, 256, 0, s>>>(a, p, t0, t1);
+        block_weights_kernel<<<dim3((n + 63) / 64, c.num_seqs), 1024, 0, s>>>(a, p, j0, j0 + n);
+    }
 }
 
 }  // namespace k

@@ -132,3 +132,43 @@ def test_small_weights_beside_a_token_without_value(hip, lead, rows, past):
     exps[0, tables[0, 2]] = -6
     check_attention(hip, q, codes, exps, tables, lens, np.array([0, rows], np.int32), scale=1.0,
                     weights=np.zeros(tables.shape, np.float32))
+
+
+# ---- tables far wider than the contexts -------------------------------------------
+
+GIB = 1 << 30
+
+
+@pytest.mark.parametrize("rows,H,Hq,bs,width,seqs,longest", [
+    # decode: sums of 16 tokens, of 4; joined contexts; 4096 tokens to a part of the tables
+    (1, 64, 64, 64, 256, 4096, 9000), (1, 64, 128, 8, 1024, 2048, 8100),
+    # chunks whose sums are not stored (16 does not divide the block), 32768 to a part
+    (40, 16, 16, 24, 4000, 2048, 70000)])
+def test_weights_of_wide_tables(hip, rows, H, Hq, bs, width, seqs, longest):
+    """The workspace of the blocks' weights stays below 1 GiB however wide the
+    tables are, and weights in all parts of a table are right."""
+    g = rng(seqs + width)
+    D = 16
+    n = np.full(seqs, rows)
+    lens = np.zeros(seqs, np.int32)          # most rows stand before any token: zeros
+    lens[::97] = g.integers(1, 3 * bs, len(lens[::97]))
+    lens[5], lens[-1] = longest, longest - 2 * bs - 1
+    if rows > 1:
+        n[5], n[-1] = 3, 2
+    tables, nb = ref.pool(g, lens, bs, width)
+    codes, exps = ref.cache(g, nb, H, bs, D)
+    starts = None if rows == 1 else ref.starts_of(n)
+    q = g.standard_normal((int(n.sum()), Hq * D), np.float32)
+    w = g.random(tables.shape, np.float32)
+    args = up(hip, q, codes, exps, tables, lens, starts)
+    tw = hip.tensor(w)
+    hip.synchronize()
+    before = hip.memory_reserved()
+    out, wo = hip.paged_kv8_attention(*args, weights=tw)
+    hip.synchronize()
+    # the results, the pieces of contexts (at most 1024 x 2 x 128 rows of 16 and 2)
+    # and the rows' maxima and sums come to less than a quarter of it
+    assert hip.memory_reserved() - before < GIB + GIB // 4
+    want, ww, tol, wtol = ref.attention(q, codes, exps, tables, lens, starts, weights=w)
+    within(out.numpy(), want, tol, "out")
+    within(wo.numpy(), ww, wtol + 1e-37, "weights")
