@@ -351,8 +351,8 @@ void kv8_tiles(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
 // computed again.
 constexpr int kKv8WeightPart = 512;
 // Bytes of sums, however wide the tables are: where a sum for every 16 or 4 tokens of
-// the tables and every row and head would take more, the scores are computed again, a
-// range of the tables' blocks at a time.
+// the tables and every row and head would take more, decode steps go in several turns,
+// and others have the scores computed again, a range of the tables' blocks at a time.
 constexpr int64_t kKv8MaxSums = 1ll << 30;
 void kv8_late_weights(const Kv8Attention &a, const Kv8Split &p, hipStream_t s);
 

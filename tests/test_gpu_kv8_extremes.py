@@ -140,8 +140,12 @@ GIB = 1 << 30
 
 
 @pytest.mark.parametrize("rows,H,Hq,bs,width,seqs,longest", [
-    # decode: sums of 16 tokens, of 4; joined contexts; 4096 tokens to a part of the tables
+    # decode in turns: sums of 16 tokens, of 4; joined contexts
     (1, 64, 64, 64, 256, 4096, 9000), (1, 64, 128, 8, 1024, 2048, 8100),
+    # few rows each, scores computed again, 4096 tokens to a part of the tables
+    (2, 64, 64, 64, 256, 4096, 9000),
+    # a decode step of which one sequence's sums are too many
+    (1, 8, 64, 4096, 9000, 2, 3000),
     # chunks whose sums are not stored (16 does not divide the block), 32768 to a part
     (40, 16, 16, 24, 4000, 2048, 70000)])
 def test_weights_of_wide_tables(hip, rows, H, Hq, bs, width, seqs, longest):
@@ -152,9 +156,9 @@ def test_weights_of_wide_tables(hip, rows, H, Hq, bs, width, seqs, longest):
     n = np.full(seqs, rows)
     lens = np.zeros(seqs, np.int32)          # most rows stand before any token: zeros
     lens[::97] = g.integers(1, 3 * bs, len(lens[::97]))
-    lens[5], lens[-1] = longest, longest - 2 * bs - 1
-    if rows > 1:
-        n[5], n[-1] = 3, 2
+    lens[seqs // 2], lens[-1] = longest, longest - min(2 * bs, 1000) - 1
+    if rows > 2:
+        n[seqs // 2], n[-1] = 3, 2
     tables, nb = ref.pool(g, lens, bs, width)
     codes, exps = ref.cache(g, nb, H, bs, D)
     starts = None if rows == 1 else ref.starts_of(n)
