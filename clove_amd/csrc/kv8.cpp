@@ -135,6 +135,9 @@ TensorNode HipBackend::paged_kv8_attention(const Tensor &q, const Tensor &codes,
     k::Kv8Attention a{};
     a.c = cache_args(codes, exps, bt, cl, rs, q.numel / X);
     a.q_heads = (int)(X / (size_t)a.c.head_dim);
+    // (the kernels number tokens in 31 bits, up to a table of 4096 past the last)
+    CLOVE_REQUIRE(bt.shape[1] * (size_t)a.c.block_size <= (1ull << 31) - 8192, CLOVE_HIP_ERR_SHAPE,
+                  "attention supports a capacity of up to 2^31 - 8192 tokens a context");
     CLOVE_REQUIRE((size_t)a.c.rows * (size_t)a.q_heads < (1ull << 31) && a.q_heads <= 65535,
                   CLOVE_HIP_ERR_SHAPE, "too many rows and query heads");
     if (weights) {

@@ -281,7 +281,8 @@ int clove_hip_paged_kv8_read(CTensor codes, CTensor exps, CTensor block_tables,
  * key head h / G.  A row sees the tokens up to its own position; out (q's
  * shape) = softmax(scale * q.K^T) V, scale <= 0 selects 1/sqrt(D).  Without
  * row_starts this is the decode step, with them a later chunk of a prompt, a
- * whole prompt, speculated tokens, or any mixture.
+ * whole prompt, speculated tokens, or any mixture.  max_blocks * block_size is at
+ * most 2^31 - 8192 here.
  * weights (f32 [B, max_blocks]) and weights_out go together, both or neither:
  * *weights_out receives a new tensor weights[b][j] + the sum, over the rows and
  * query heads of sequence b and the tokens of its block j, of the softmax

@@ -176,3 +176,36 @@ def test_weights_of_wide_tables(hip, rows, H, Hq, bs, width, seqs, longest):
     want, ww, tol, wtol = ref.attention(q, codes, exps, tables, lens, starts, weights=w)
     within(out.numpy(), want, tol, "out")
     within(wo.numpy(), ww, wtol + 1e-37, "weights")
+
+
+# ---- capacities next to 2^31 tokens -------------------------------------------------
+
+def test_capacities_next_to_2_31(hip):
+    """Tables whose capacity a kernel's token numbers would leave are refused; the
+    widest ones that are not hold a context to their last token."""
+    g = rng(71)
+    B, H, D, width, tokens = 1, 1, 16, 2048, 1 << 20
+    q = g.standard_normal((B, H * D), np.float32)
+    full = np.array([width * (tokens - 4)], np.int32)
+    for bs, lens, code in ((tokens - 1, [100], "refused"), (tokens - 4, [100], None),
+                           (tokens - 4, full, None)):
+        tables, lens = np.zeros((1, width), np.int32), np.asarray(lens, np.int32)
+        codes = ref.encode(g.standard_normal((2, 1, H, 1024, D)) * 120).repeat(1024, 3)[:, :, :, :bs]
+        exps = np.full((2, 1, H), -7, np.int32)
+        args = up(hip, q, np.ascontiguousarray(codes), exps, tables, lens)
+        if code:
+            with pytest.raises(hip.CloveError) as e:
+                hip.paged_kv8_attention(*args)
+            assert e.value.code == hip.ERR_SHAPE and "2^31" in str(e.value)
+            continue
+        out = hip.paged_kv8_attention(*args).numpy()
+        hip.synchronize()
+        # the block over and over: as over one of them
+        one = np.minimum(lens, bs).astype(np.int32)
+        want, _, _, _ = ref.attention(q, codes, exps, tables[:, :1], one)
+        x, _ = ref.tokens(codes, exps, tables[:, :1], 0, int(one[0]))
+        s = (x[0, :, 0] @ q[0].astype(np.float64)) / np.sqrt(D)
+        p = np.exp(s - s.max())
+        mag = (p / p.sum()) @ np.abs(x[1, :, 0])
+        # every sum of a lane takes at most 2^17 tokens, then as many pieces again
+        within(out, want, (2.0 ** 18 * 2.0 ** -24 + 2.0 ** -18) * mag[None], f"{bs} {lens}")
