@@ -407,7 +407,7 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
     const int64_t units = ((int64_t)c.rows * G + c.num_seqs - 1) / c.num_seqs;
     const int64_t cap = (int64_t)c.max_blocks * bs;
     int residents;
-    // (16 speculating sequences of 22 rows and heads each: 52 us, as tiles 67)
+    // (16 speculating sequences of 22 rows and heads each: 54 us, as tiles 59)
     if (units <= (p.dp == 256 ? 16 : 32)) {
         p.kind = KV8_STREAM;
         p.tile = units <= 16 || p.dp == 256 ? 16 : 32;
@@ -430,8 +430,8 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
         p.hw = 1;
         p.step = p.dp == 256 ? 32 : 64;
         // A tile's table, rows, first codes and stores take the time of some four
-        // steps: 2048 rows of 32 heads of 80, 175 us when runs are equal in steps
-        // alone, 118 / 105 / 109 with 2 / 4 / 7 more a tile; chunks 160, 150 / 147 / 152.
+        // steps: 2048 rows of 32 heads of 80, 180 us when runs are equal in steps
+        // alone, 120 / 114 / 120 with 2 / 4 / 7 more a tile; chunks 170, 154 / 155 / 162.
         p.extra = 4;
         residents = 2;
     }
@@ -455,8 +455,8 @@ Kv8Split kv8_split(const Kv8Attention &a, int cus) {
         p.row_ml_at = take(2 * rh);
         // Eight bytes for 16 tokens of a row, written on the way and read once,
         // against all scores computed again: 2000 rows in chunks, 24 query
-        // heads of 80, contexts to 3700, 176 against 230 us when it came in.  They are
-        // stored up to a GiB; a long prompt's are not, nor those of very wide tables.
+        // heads of 80, contexts to 3700, 155 against 217 us.  They are stored up to a
+        // GiB; a long prompt's are not, nor those of very wide tables.
         const int64_t pairs = kv8_slots(c, kKv8WeightPart, G, 1) * c.num_heads;
         if ((p.kind == KV8_STREAM || sums == 16) && 8 * rh * (cap / sums) <= kKv8MaxSums) {
             p.sums = sums;

@@ -13,13 +13,14 @@
 // itself, two thirds of the MFMAs.  P stays in bf16: f16 ends at 2^-24, and a weight
 // that far below the largest is all there is where the tokens ahead have no value.
 //
-// Bound by the matrix cores: a prompt of 4096 rows, 32 heads of 128, takes 69
-// GFLOP for the scores and as many for the sums over V, in two and three pieces:
-// 270 us at the 1271 TFLOP/s of a large bf16 product; 313 to 322 us measured (all in
-// bf16 pieces 333; P in two f16 pieces as well 264 to 270, less what they lose).  Scores and
-// weights stay in registers: S^T leaves the MFMA in the layout that P^T enters
-// it.  What the vector units do between (the exponentials, the pieces of P, the
-// widening of codes) runs beside the other workgroup's MFMAs.
+// A prompt of 4096 rows, 32 heads of 128, takes 69 GFLOP for the scores and as many
+// for the sums over V, in two and three pieces: 270 us at the 1271 TFLOP/s of a large
+// bf16 product; 313 to 322 us measured, from box to box (all in bf16 pieces 333).  The
+// MFMAs take 47% of the SIMDs' cycles there, and the time has followed their number
+// (five pieces for four: 1.19 times the time).  Scores and weights stay in registers:
+// S^T leaves the MFMA in the layout that P^T enters it.  What the vector units do
+// between (the exponentials, the pieces of P, the widening of codes) runs beside the
+// other workgroup's MFMAs.
 #include <algorithm>
 #include <type_traits>
 
@@ -131,7 +132,9 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(Kv8Attention a, Kv8Split p
     constexpr int KB = DP > 128 ? 32 : 64;    // tokens of a step
     constexpr int JB = DP / 16;               // 16-dim blocks of O^T
     constexpr int JG = FULL ? 4 : 2;          // of them at a time
-    constexpr int PK = 2 * DP + 16, PV = 2 * KB + 16;  // LDS pitches: no bank conflicts
+    // (rows of operands start four banks apart; what conflicts remain take 12% of the
+    // CUs' cycles in that prompt)
+    constexpr int PK = 2 * DP + 16, PV = 2 * KB + 16;  // LDS pitches
     constexpr int NK = KB * DP / 16 / 256;    // 16-byte pieces of keys a thread stages
     constexpr int JV = DP * KB / 4 / 256;     // dims of four tokens' values a thread stages
     // tokens whose rows the table holds (two workgroups to a CU in any case)
