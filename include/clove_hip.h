@@ -268,7 +268,8 @@ CTensor clove_hip_paged_gather_indices(CTensor block_tables, CTensor context_len
  * lost only where a code becomes subnormal).  Slots behind the new rows keep their bytes.
  * NaN is stored as 0 and an infinity as the largest value of its tile, and both
  * are reported like an index error.  No two sequences of a call may write the
- * same block (such a block's tile holds a mixture, always finite). */
+ * same block, nor may one whose table names it twice (such a block's tile holds a
+ * mixture, always finite). */
 int clove_hip_paged_kv8_append(CTensor codes, CTensor exps, CTensor k, CTensor v,
                                CTensor block_tables, CTensor context_lens, CTensor row_starts);
 /* The inverse: *k and *v receive new f32 [rows, H*D] tensors with the values
