@@ -119,6 +119,11 @@ def _declare(lib: C.CDLL) -> None:
                                                C.POINTER(vp)]),
         "clove_hip_paged_kv8_attention": (vp, [vp, vp, vp, vp, vp, vp, f, vp, C.POINTER(vp)]),
         "clove_hip_paged_evict": (C.c_int, [vp, vp, vp] + [C.c_int] * 4 + [C.POINTER(vp)] * 4),
+        "clove_hip_rms_norm": (vp, [vp, vp, vp, f, C.POINTER(vp)]),
+        "clove_hip_rms_norm_e4m3": (C.c_int, [vp, vp, vp, f] + [C.POINTER(vp)] * 3),
+        "clove_hip_rms_norm_backward": (C.c_int, [vp, vp, vp, vp, f] + [C.POINTER(vp)] * 2),
+        "clove_hip_quantize_e4m3": (C.c_int, [vp, C.c_int] + [C.POINTER(vp)] * 4),
+        "clove_hip_matmul_e4m3": (vp, [vp] * 5),
         "clove_hip_relu_backward": (vp, [vp, vp]),
         "clove_hip_gelu_backward": (vp, [vp, vp]),
         "clove_hip_softmax_backward": (vp, [vp, vp]),
@@ -302,7 +307,7 @@ class Tensor:
 
 def tensor(data, dtype=None) -> Tensor:
     """Uploads a numpy array (f32, int32 for block tables / lengths, or with
-    dtype=np.uint8 the e4m3 codes of an 8-bit cache)."""
+    dtype=np.uint8 e4m3 codes)."""
     a = np.asarray(data)
     if dtype is None:
         dtype = np.int32 if a.dtype.kind in "iu" else np.float32
@@ -574,6 +579,57 @@ def paged_evict(block_tables: Tensor, context_lens: Tensor, weights: Tensor, blo
                                        block_size, budget, first, last,
                                        *[C.byref(o) for o in outs]))
     return tuple(Tensor(o.value) for o in outs)
+
+
+def rms_norm(x: Tensor, gamma: Tensor, residual: Optional[Tensor] = None, eps: float = 1e-5):
+    """h * gamma / sqrt(mean(h^2) + eps) over the last dimension, h = x or
+    x + residual; with a residual the result is (out, h)."""
+    if residual is None:
+        return _handle(lib().clove_hip_rms_norm(x.handle, None, gamma.handle, eps, None))
+    h = C.c_void_p()
+    out = _handle(lib().clove_hip_rms_norm(x.handle, residual.handle, gamma.handle, eps,
+                                           C.byref(h)))
+    return out, Tensor(h.value)
+
+
+def rms_norm_e4m3(x: Tensor, gamma: Tensor, residual: Optional[Tensor] = None,
+                  eps: float = 1e-5):
+    """rms_norm's output in 8 bits, an exponent for each 128 elements of a row:
+    (codes, exps), and h behind them with a residual."""
+    outs = [C.c_void_p() for _ in range(3)]
+    _check(lib().clove_hip_rms_norm_e4m3(x.handle, _opt(residual), gamma.handle, eps,
+                                         C.byref(outs[2]) if residual is not None else None,
+                                         C.byref(outs[0]), C.byref(outs[1])))
+    return tuple(Tensor(o.value) for o in outs[:2 if residual is None else 3])
+
+
+def rms_norm_backward(h: Tensor, gamma: Tensor, grad_out: Tensor,
+                      grad_sum: Optional[Tensor] = None, eps: float = 1e-5):
+    """(grad_h, grad_gamma) of rms_norm; grad_sum, the gradient that reaches h
+    from the residual stream, is added to grad_h."""
+    gh, gg = C.c_void_p(), C.c_void_p()
+    _check(lib().clove_hip_rms_norm_backward(h.handle, gamma.handle, grad_out.handle,
+                                             _opt(grad_sum), eps, C.byref(gh), C.byref(gg)))
+    return Tensor(gh.value), Tensor(gg.value)
+
+
+def quantize_e4m3(x: Tensor, block_rows: int = 1, straight: bool = True,
+                  transposed: bool = False):
+    """x [.., K] in 8 bits, blocks of block_rows (1 or 128) rows by 128 elements:
+    (codes, exps) as x stands, of its transpose, or both pairs in that order."""
+    outs = [C.c_void_p() if want else None for want in (straight, straight, transposed,
+                                                        transposed)]
+    _check(lib().clove_hip_quantize_e4m3(x.handle, block_rows,
+                                         *[None if o is None else C.byref(o) for o in outs]))
+    return tuple(Tensor(o.value) for o in outs if o is not None)
+
+
+def matmul_e4m3(a: Tensor, a_exps: Tensor, b: Tensor, b_exps: Tensor,
+                bias: Optional[Tensor] = None) -> Tensor:
+    """a . b^T (+ bias) of two matrices in 8 bits, a [.., Kp] and b [N, Kp], in
+    f32; exponents are those of rows or of 128 x 128 blocks, by their shapes."""
+    return _handle(lib().clove_hip_matmul_e4m3(a.handle, a_exps.handle, b.handle, b_exps.handle,
+                                               _opt(bias)))
 
 
 class FusedChain:

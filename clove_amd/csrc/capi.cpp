@@ -423,6 +423,69 @@ int clove_hip_paged_evict(CTensor block_tables, CTensor context_lens, CTensor we
     });
 }
 
+// ---- the root-mean-square norm and linear layers in 8 bits -----------------
+
+CTensor clove_hip_rms_norm(CTensor x, CTensor residual, CTensor gamma, float eps, CTensor *sum) {
+    CTensor out = nullptr;
+    CTensor *const outs[2] = {&out, sum};
+    TensorNode made[2];
+    guarded_outputs(outs, made, 2, [&] {
+        made[0] = HipBackend::rms_norm(deref(x, "x"),
+                                       residual ? &deref(residual, "residual") : nullptr,
+                                       deref(gamma, "gamma"), eps, sum ? &made[1] : nullptr);
+    });
+    return out;
+}
+
+int clove_hip_rms_norm_e4m3(CTensor x, CTensor residual, CTensor gamma, float eps, CTensor *sum,
+                            CTensor *codes, CTensor *exps) {
+    CTensor *const outs[3] = {sum, codes, exps};
+    TensorNode made[3];
+    return guarded_outputs(outs, made, 3, [&] {
+        if (!codes || !exps) clove::fail(CLOVE_HIP_ERR_INVALID, "codes or exps is NULL");
+        HipBackend::rms_norm_e4m3(deref(x, "x"),
+                                  residual ? &deref(residual, "residual") : nullptr,
+                                  deref(gamma, "gamma"), eps, sum ? &made[0] : nullptr, &made[1],
+                                  &made[2]);
+    });
+}
+
+int clove_hip_rms_norm_backward(CTensor h, CTensor gamma, CTensor grad_out, CTensor grad_sum,
+                                float eps, CTensor *grad_h, CTensor *grad_gamma) {
+    CTensor *const outs[2] = {grad_h, grad_gamma};
+    TensorNode made[2];
+    return guarded_outputs(outs, made, 2, [&] {
+        HipBackend::rms_norm_backward(deref(h, "h"), deref(gamma, "gamma"),
+                                      deref(grad_out, "grad_out"),
+                                      grad_sum ? &deref(grad_sum, "grad_sum") : nullptr, eps,
+                                      grad_h ? &made[0] : nullptr,
+                                      grad_gamma ? &made[1] : nullptr);
+    });
+}
+
+int clove_hip_quantize_e4m3(CTensor x, int block_rows, CTensor *codes, CTensor *exps,
+                            CTensor *codes_t, CTensor *exps_t) {
+    CTensor *const outs[4] = {codes, exps, codes_t, exps_t};
+    TensorNode made[4];
+    return guarded_outputs(outs, made, 4, [&] {
+        if (!codes != !exps || !codes_t != !exps_t)
+            clove::fail(CLOVE_HIP_ERR_INVALID,
+                        "pass codes and exps, codes_t and exps_t, together or not at all");
+        HipBackend::quantize_e4m3(deref(x, "x"), block_rows, codes ? &made[0] : nullptr,
+                                  codes ? &made[1] : nullptr, codes_t ? &made[2] : nullptr,
+                                  codes_t ? &made[3] : nullptr);
+    });
+}
+
+CTensor clove_hip_matmul_e4m3(CTensor a, CTensor a_exps, CTensor b, CTensor b_exps,
+                              CTensor bias) {
+    return guarded_tensor([&] {
+        return HipBackend::matmul_e4m3(deref(a, "a"), deref(a_exps, "a_exps"), deref(b, "b"),
+                                       deref(b_exps, "b_exps"),
+                                       bias ? &deref(bias, "bias") : nullptr);
+    });
+}
+
 // ---- backward passes and losses ------------------------------------------
 
 CTensor clove_hip_relu_backward(CTensor x, CTensor grad_out) {

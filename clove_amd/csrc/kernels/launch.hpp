@@ -282,5 +282,61 @@ struct EvictArgs {
 };
 void paged_evict(const EvictArgs &a, hipStream_t s);
 
+// norm8.hip -- the root-mean-square norm.  h = x + residual (or x), out =
+// h * gamma / sqrt(mean(h^2) + eps) in 32 bits (out) or 8 (codes and exps, blocks
+// of 128 of a row); sum, where given, receives h.
+struct RmsNormArgs {
+    const float *x, *residual, *gamma;  // residual may be null
+    float *sum, *out;                   // sum may be null; out null: codes and exps
+    uint8_t *codes;
+    int32_t *exps;
+    double *stats;                      // rms_norm_stats() doubles
+    size_t rows;
+    int cols;
+    float eps;
+};
+size_t rms_norm_stats(size_t rows, int cols);
+void rms_norm(const RmsNormArgs &a, hipStream_t s);
+// grad_h = r (g - h r^2 mean(g h)) + grad_sum with g = grad_out * gamma, r the
+// row's 1 / sqrt(mean(h^2) + eps); part receives rms_norm_grad_parts() rows of
+// cols partial sums of grad_out * h * r, for the caller to add up.
+struct RmsNormGradArgs {
+    const float *h, *gamma, *grad_out, *grad_sum;  // grad_sum may be null
+    float *grad_h, *part;                          // either may be null
+    double *stats;                                 // rms_norm_grad_stats() doubles
+    size_t rows;
+    int cols;
+    float eps;
+};
+size_t rms_norm_grad_parts(size_t rows, int cols, int num_cus);
+size_t rms_norm_grad_stats(size_t rows, int cols);
+void rms_norm_grad(const RmsNormGradArgs &a, int num_cus, hipStream_t s);
+
+// quant8.hip -- a matrix in 8 bits with blocks of block_rows (1 or 128) rows by
+// 128 columns, as it stands (codes, exps) and transposed (codes_t, exps_t: the
+// same of x^T); either pair may be null.
+struct Quant8Args {
+    const float *x;
+    uint8_t *codes, *codes_t;
+    int32_t *exps, *exps_t;
+    size_t rows, cols;
+    int block_rows;
+};
+void quantize8(const Quant8Args &a, hipStream_t s);
+
+// gemm8.hip -- out[m][n] = sum_k a[m][k] b[n][k] (+ bias[n]) of two matrices in 8
+// bits, 16-byte aligned codes.  a_tiles, b_tiles: exponents of 128 x 128 blocks
+// rather than of 128 elements of a row.
+struct Gemm8Args {
+    const uint8_t *a, *b;
+    const int32_t *a_exps, *b_exps;
+    const float *bias;  // may be null
+    float *out, *ws;    // gemm8_workspace() floats
+    int m, n, blocks;   // blocks of 128 along k
+    bool a_tiles, b_tiles;
+};
+size_t gemm8_workspace(const Gemm8Args &a, int num_cus);
+void gemm8(const Gemm8Args &a, int num_cus, hipStream_t s);
+
 }  // namespace k
 }  // namespace clove

@@ -129,6 +129,20 @@ struct HipBackend {
                             const Tensor &weights, int block_size, int budget, int first,
                             int last, TensorNode out[4]);
 
+    // The root-mean-square norm and linear layers in 8 bits (linear8.cpp); null
+    // outputs are not wanted (quantize_e4m3: a pair at a time).
+    static TensorNode rms_norm(const Tensor &x, const Tensor *residual, const Tensor &gamma,
+                               float eps, TensorNode *sum);
+    static void rms_norm_e4m3(const Tensor &x, const Tensor *residual, const Tensor &gamma,
+                              float eps, TensorNode *sum, TensorNode *codes, TensorNode *exps);
+    static void rms_norm_backward(const Tensor &h, const Tensor &gamma, const Tensor &grad_out,
+                                  const Tensor *grad_sum, float eps, TensorNode *grad_h,
+                                  TensorNode *grad_gamma);
+    static void quantize_e4m3(const Tensor &x, int block_rows, TensorNode *codes,
+                              TensorNode *exps, TensorNode *codes_t, TensorNode *exps_t);
+    static TensorNode matmul_e4m3(const Tensor &a, const Tensor &a_exps, const Tensor &b,
+                                  const Tensor &b_exps, const Tensor *bias);
+
     // Backward passes and losses (grad.cpp; the autograd closures of
     // backend.rs).
     static TensorNode relu_backward(const TensorNode &x, const TensorNode &grad_out);

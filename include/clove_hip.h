@@ -45,7 +45,7 @@ enum clove_hip_status {
     CLOVE_HIP_ERR_RANGE = 7      /* an index (block table, context length) is out of range */
 };
 
-/* E4M3: one byte an element (the codes of an 8-bit KV cache: sign, 4 exponent
+/* E4M3: one byte an element (the codes of 8-bit caches and matrices: sign, 4 exponent
  * bits of bias 7, 3 fraction bits; no infinities, 0x7F and 0xFF are NaN). */
 enum clove_hip_dtype { CLOVE_HIP_F32 = 0, CLOVE_HIP_I32 = 1, CLOVE_HIP_E4M3 = 2 };
 
@@ -309,6 +309,52 @@ CTensor clove_hip_paged_kv8_attention(CTensor q, CTensor codes, CTensor exps,
 int clove_hip_paged_evict(CTensor block_tables, CTensor context_lens, CTensor weights,
                           int block_size, int budget, int first, int last, CTensor *tables_out,
                           CTensor *lens_out, CTensor *weights_out, CTensor *evicted);
+
+/* ---------------------------------------------------------------------- */
+/* Linear layers in 8 bits and the root-mean-square norm (no counterpart   */
+/* in the reference): the norm before a layer with the residual's addition */
+/* and an 8-bit output, its gradient, the quantiser, and the product.      */
+/* ---------------------------------------------------------------------- */
+
+/* A matrix [rows, K] in 8 bits is two tensors:
+ *   codes  e4m3  [rows, Kp], Kp = K rounded up to a multiple of 128, zeros behind K
+ *   exps   int32 [rows, Kp / 128], a block being 128 elements of a row, or
+ *                [ceil(rows / 128), Kp / 128], a block being 128 x 128 elements
+ * and an element stands for its code times 2^exp of its block.  exp is the
+ * smallest e in [-100, 119] with |x| <= 448 * 2^e for the block's finite elements;
+ * codes are x * 2^-e rounded to nearest, ties to even, so an element is off by at
+ * most 2^-4 of itself (half of 2^(e-9) for the smallest).  Magnitudes past 448 *
+ * 2^119 become that; infinities and NaN become NaN, which products carry on.
+ * Leading dimensions of x are rows; codes (and exps of rows) keep them. */
+
+/* h = x + residual (or x where residual is NULL), out = h * gamma /
+ * sqrt(mean(h^2) + eps) over the last dimension, x f32 [.., cols], residual x's
+ * shape, gamma f32 of cols elements, eps >= 0.  sum, where not NULL, receives h
+ * (it needs a residual).  Computed in 64 bits and rounded once. */
+CTensor clove_hip_rms_norm(CTensor x, CTensor residual, CTensor gamma, float eps, CTensor *sum);
+/* The same in 8 bits, one exponent for each 128 elements of a row: bit for bit
+ * clove_hip_quantize_e4m3 of clove_hip_rms_norm. */
+int clove_hip_rms_norm_e4m3(CTensor x, CTensor residual, CTensor gamma, float eps, CTensor *sum,
+                            CTensor *codes, CTensor *exps);
+/* Gradients of out with respect to h and gamma (with respect to x and residual:
+ * h's).  grad_sum (h's shape, or NULL) is the gradient that reaches h from
+ * elsewhere, the residual stream, and is added to *grad_h.  Either output may be
+ * NULL.  Sums run in a fixed order. */
+int clove_hip_rms_norm_backward(CTensor h, CTensor gamma, CTensor grad_out, CTensor grad_sum,
+                                float eps, CTensor *grad_h, CTensor *grad_gamma);
+/* x f32 [.., K] in 8 bits with blocks of block_rows (1 or 128) rows by 128
+ * elements: codes and exps as x stands, codes_t and exps_t those of its transpose
+ * ([K, rows up to a multiple of 128]), in one pass over x; either pair may be NULL.
+ * For a layer y = x . w with w [K, N]: w's transposed pair and x's straight one
+ * (rows) multiply to y, the output gradient's straight pair and w's straight one to
+ * x's gradient, x's and the output gradient's transposed pairs to w's. */
+int clove_hip_quantize_e4m3(CTensor x, int block_rows, CTensor *codes, CTensor *exps,
+                            CTensor *codes_t, CTensor *exps_t);
+/* out[.., n] = sum_k a[.., k] * b[n, k] (+ bias[n]): a [.., Kp] and b [N, Kp] in 8
+ * bits, each with exponents of rows or of 128 x 128 blocks, bias f32 of N elements
+ * or NULL.  Products are exact and sums 32 bits wide, in a fixed order.  Kp is a
+ * multiple of 128 below 2^23, codes are 16-byte aligned, exponents in [-100, 119]. */
+CTensor clove_hip_matmul_e4m3(CTensor a, CTensor a_exps, CTensor b, CTensor b_exps, CTensor bias);
 
 /* ---------------------------------------------------------------------- */
 /* Backward passes and losses: the autograd closures WgpuBackend attaches  */
