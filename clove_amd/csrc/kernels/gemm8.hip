@@ -10,6 +10,7 @@
 // largest of them with 13 bits below it, the rest cut off: 1.5e-5 off on normal
 // data, 7e-5 and always low on positive data, where these sums are 2e-7 off.
 #include <algorithm>
+#include <cmath>
 
 #include "bf16x3.h"
 #include "gemm_common.h"
@@ -51,72 +52,107 @@ __device__ __forceinline__ bool tile_of(int L, int tiles_m, int tiles_n, int *tm
     return true;
 }
 
-constexpr int vmcnt_imm(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
+// One operand's buffer from row r0 on, `rows` rows at most: a row past the matrix's
+// end lies past the buffer, where reads give zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t codes_from(const uint8_t *p, int r0, int rows,
+                                                             int all, uint32_t kp) {
+    return make_rsrc(p + (size_t)r0 * kp, (uint32_t)min(rows, all - r0) * kp);
+}
 
-// BM x BN tiles, four waves of WM x WN, slabs of BK codes that move by buffer->LDS
-// DMA into a ring of ST stages.  In LDS a row is BK bytes, its 16-byte slots
-// permuted by the row so that a fragment read (lane l: row l % 32) meets every bank.
-template <int BM, int BN, int WM, int WN, int BK, int ST, int MINW>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MINW)))
-gemm8_kernel(Gemm8Args g, Plan p) {
-    constexpr int IB = WM / 32, JB = WN / 32, SL = BK / 16, RPI = 64 / SL;
-    constexpr int IA = BM / RPI / 4, IBW = BN / RPI / 4;  // DMAs a wave and slab
-    constexpr int STAGE = (BM + BN) * BK;
-    static_assert((BM / WM) * (BN / WN) == 4, "four waves");
-    static_assert(IA >= 1 && IBW >= 1 && BM % (4 * RPI) == 0 && BN % (4 * RPI) == 0, "whole DMAs");
-    __shared__ __attribute__((aligned(16))) char smem[ST * STAGE];
+// Where row r's exponents lie, in bytes behind those of row r0's line.
+__device__ __forceinline__ uint32_t exps_at(int r, int r0, bool tiles, int blocks) {
+    return (uint32_t)((tiles ? r >> 7 : r) - (tiles ? r0 >> 7 : r0)) * (uint32_t)blocks * 4u;
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t exps_from(const int32_t *p, int r0, int rows,
+                                                            bool tiles, int blocks) {
+    return make_rsrc(p + (size_t)(tiles ? r0 >> 7 : r0) * blocks,
+                     (uint32_t)rows * (uint32_t)blocks * 4u);
+}
+
+// In LDS a row of a block is 128 bytes, its eight 16-byte slots permuted by the
+// row: eight lanes that read one slot of eight rows meet every bank, and a DMA of
+// eight rows (lane l: slot l % 8 of row l / 8) still reads whole lines.
+__device__ __forceinline__ int slot_of(int row, int k16) { return 16 * (k16 ^ (row & 7)); }
+
+// BM x BN tiles in KG groups of waves of WM x WN each; group k takes the chunks k,
+// k + KG, ... (32 codes) of every block, and the groups' sums are added at the end:
+// more waves a CU without smaller tiles for each, whose operands would be widened
+// more often.  Blocks of both operands and their exponents move by buffer->LDS DMA
+// into two stages, one filling while the other is multiplied (in registers the
+// exponents would make every block wait for all DMAs in flight).
+//
+// What bounds it: 4096^3 in 256 x 256 tiles of sixteen waves 114-117 us, 1180-1207
+// TFLOP/s, of which the 64 MiB of results are some 13 us at the end; a large bf16
+// library product runs at 1208 on the same card, at its power limit.  Four waves
+// of 128 x 64 on 256 x 128 tiles 134 us, of 64 x 64 on 128 x 128 124-134.  Results
+// stored with the non-temporal policy: 8192 x 4096 x 1024 86 us, 92 without.
+template <int BM, int BN, int WM, int WN, int KG, int MINW>
+__global__ void __launch_bounds__(BM / WM * (BN / WN) * KG * 64)
+    __attribute__((amdgpu_waves_per_eu(MINW))) gemm8_kernel(Gemm8Args g, Plan p) {
+    constexpr int WG = BM / WM * (BN / WN), NW = WG * KG;  // waves of a group, and all
+    constexpr int IB = WM / 32, JB = WN / 32;
+    constexpr int OWN = IB * JB * 4 / KG;                  // quarter blocks that a group stores
+    constexpr int STAGE = (BM + BN) * 128;
+    constexpr int ND = (BM + BN) / 8, IW = (ND + NW - 1) / NW;   // DMAs a block, and a wave's
+    constexpr int XD = (BM + BN) / 64, XW = (XD + NW - 1) / NW;  // of exponents
+    static_assert(BM % 64 == 0 && BN % 64 == 0, "whole DMAs of exponents");
+    static_assert(IB * JB * 4 % KG == 0 && 4 % KG == 0, "equal shares");
+    static_assert(KG == 1 || NW * OWN * 1024 <= 2 * STAGE, "a round of sums fits");
+    __shared__ __attribute__((aligned(16))) char smem[2 * (STAGE + XD * 256)];
     int tm, tn;
     if (!tile_of(blockIdx.x, p.tiles_m, p.tiles_n, &tm, &tn)) return;
     const int m0 = tm * BM, n0 = tn * BN;
     const int kb0 = blockIdx.y * p.per_split;
     const int blocks = min(p.per_split, g.blocks - kb0);
-    const int slabs = blocks * (128 / BK);
     const uint32_t kp = (uint32_t)g.blocks * 128u;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l32 = lane & 31, h = lane >> 5;
-    const int wm0 = wave / (BN / WN) * WM, wn0 = wave % (BN / WN) * WN;
-    // rows past the end lie past the buffers: the DMA writes zeros
-    const __amdgpu_buffer_rsrc_t ra =
-        make_rsrc(g.a + (size_t)m0 * kp, (uint32_t)min(BM, g.m - m0) * kp);
-    const __amdgpu_buffer_rsrc_t rb =
-        make_rsrc(g.b + (size_t)n0 * kp, (uint32_t)min(BN, g.n - n0) * kp);
-    const auto swz = [](int r) { return BK == 128 ? r & 7 : (r >> 1) & 3; };
-    uint32_t aoff[IA], boff[IBW];
+    const int kg = wave / WG;
+    const int wm0 = wave % WG / (BN / WN) * WM, wn0 = wave % (BN / WN) * WN;
+    const __amdgpu_buffer_rsrc_t ra = codes_from(g.a, m0, BM, g.m, kp);
+    const __amdgpu_buffer_rsrc_t rb = codes_from(g.b, n0, BN, g.n, kp);
+    const __amdgpu_buffer_rsrc_t rxa = exps_from(g.a_exps, m0, BM, g.a_tiles, g.blocks);
+    const __amdgpu_buffer_rsrc_t rxb = exps_from(g.b_exps, n0, BN, g.b_tiles, g.blocks);
+    // DMA d moves eight rows, those of a first
+    uint32_t off[IW], xoff[XW];
 #pragma unroll
-    for (int u = 0; u < IA; ++u) {
-        const int r = (wave * IA + u) * RPI + lane / SL;
-        aoff[u] = (uint32_t)r * kp + 16u * (lane % SL ^ swz(r)) + (uint32_t)kb0 * 128u;
+    for (int u = 0; u < IW; ++u) {
+        const int d = u * NW + wave, r = (d < BM / 8 ? d : d - BM / 8) * 8 + lane / 8;
+        off[u] = (uint32_t)r * kp + (uint32_t)slot_of(r, lane % 8) + (uint32_t)kb0 * 128u;
     }
+    // DMA d of exponents has those of 64 rows (past the end: the last one's)
 #pragma unroll
-    for (int u = 0; u < IBW; ++u) {
-        const int r = (wave * IBW + u) * RPI + lane / SL;
-        boff[u] = (uint32_t)r * kp + 16u * (lane % SL ^ swz(r)) + (uint32_t)kb0 * 128u;
+    for (int u = 0; u < XW; ++u) {
+        const int at = (u * NW + wave) * 64 + lane;
+        xoff[u] = (at < BM ? exps_at(min(m0 + at, g.m - 1), m0, g.a_tiles, g.blocks)
+                           : exps_at(min(n0 + at - BM, g.n - 1), n0, g.b_tiles, g.blocks)) +
+                  (uint32_t)kb0 * 4u;
     }
-    auto dma = [&](int sl) {
-        char *st = smem + sl % ST * STAGE;
+    const auto stage = [&](int kb) { return smem + (kb & 1) * (STAGE + XD * 256); };
+    const auto dma = [&](int kb) {
+        char *st = stage(kb);
 #pragma unroll
-        for (int u = 0; u < IA; ++u)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                ra, (lds_void *)(st + (wave * IA + u) * 1024), 16, (int)aoff[u], sl * BK, 0, 0);
+        for (int u = 0; u < XW; ++u) {
+            const int d = u * NW + wave;
+            if (d < BM / 64)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rxa, (lds_void *)(st + STAGE + d * 256), 4,
+                                                         (int)xoff[u], kb * 4, 0, 0);
+            else if (d < XD)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rxb, (lds_void *)(st + STAGE + d * 256), 4,
+                                                         (int)xoff[u], kb * 4, 0, 0);
+        }
 #pragma unroll
-        for (int u = 0; u < IBW; ++u)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                rb, (lds_void *)(st + BM * BK + (wave * IBW + u) * 1024), 16, (int)boff[u],
-                sl * BK, 0, 0);
+        for (int u = 0; u < IW; ++u) {
+            const int d = u * NW + wave;
+            if ((u + 1) * NW <= BM / 8 || (u * NW < BM / 8 && d < BM / 8))
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void *)(st + d * 1024), 16,
+                                                         (int)off[u], kb * 128, 0, 0);
+            else if ((u + 1) * NW <= ND || d < ND)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *)(st + d * 1024), 16,
+                                                         (int)off[u], kb * 128, 0, 0);
+        }
     };
-    // this lane's rows' exponents (rows past the end take the last one's)
-    const int32_t *ea[IB], *eb[JB];
-#pragma unroll
-    for (int i = 0; i < IB; ++i) {
-        const int r = min(m0 + wm0 + 32 * i + l32, g.m - 1);
-        ea[i] = g.a_exps + (size_t)(g.a_tiles ? r >> 7 : r) * g.blocks + kb0;
-    }
-#pragma unroll
-    for (int j = 0; j < JB; ++j) {
-        const int r = min(n0 + wn0 + 32 * j + l32, g.n - 1);
-        eb[j] = g.b_exps + (size_t)(g.b_tiles ? r >> 7 : r) * g.blocks + kb0;
-    }
     f16v acc[IB][JB];
 #pragma unroll
     for (int i = 0; i < IB; ++i)
@@ -124,209 +160,377 @@ gemm8_kernel(Gemm8Args g, Plan p) {
         for (int j = 0; j < JB; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    int xa[IB], xb[JB];
-    auto exps = [&](int kb) {
-#pragma unroll
-        for (int i = 0; i < IB; ++i) xa[i] = ea[i][kb];
-#pragma unroll
-        for (int j = 0; j < JB; ++j) xb[j] = eb[j][kb];
-    };
-    if (blocks > 0) exps(0);
-#pragma unroll
-    for (int sl = 0; sl < ST - 1; ++sl)
-        if (sl < slabs) dma(sl);
+    if (blocks > 0) dma(0);
     for (int kb = 0; kb < blocks; ++kb) {
+        // this wave's DMAs of the block have landed and its reads of the stage
+        // before are done; past the barrier, every wave's
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        lds_barrier();
+        if (kb + 1 < blocks) dma(kb + 1);
+        const char *sA = stage(kb), *sB = sA + BM * 128;
+        const int *x = reinterpret_cast<const int *>(sA + STAGE);
         float sa[IB], sb[JB];
 #pragma unroll
-        for (int i = 0; i < IB; ++i) sa[i] = lin8_pow2(xa[i]);
+        for (int i = 0; i < IB; ++i) sa[i] = lin8_pow2(x[wm0 + 32 * i + l32]);
 #pragma unroll
-        for (int j = 0; j < JB; ++j) sb[j] = lin8_pow2(xb[j]);
+        for (int j = 0; j < JB; ++j) sb[j] = lin8_pow2(x[BM + wn0 + 32 * j + l32]);
+        __builtin_amdgcn_s_setprio(1);
+        // chunk c: lanes 0-31 hold its codes 0-15, lanes 32-63 16-31, of both operands
 #pragma unroll
-        for (int half = 0; half < 128 / BK; ++half) {
-            const int sl = kb * (128 / BK) + half;
-            // slab sl has landed once at most the later slab's DMAs are out (and
-            // what was set out after them, if anything)
-            if (ST >= 3 && sl + 1 < slabs) __builtin_amdgcn_s_waitcnt(vmcnt_imm((ST - 2) * (IA + IBW)));
-            else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-            lds_barrier();
-            if (half == 0 && kb + 1 < blocks) exps(kb + 1);
-            if (sl + ST - 1 < slabs) dma(sl + ST - 1);
-            const char *sA = smem + sl % ST * STAGE, *sB = sA + BM * BK;
-            __builtin_amdgcn_s_setprio(1);
+        for (int u = 0; u < 4 / KG; ++u) {
+            const int c = u * KG + kg, slot = slot_of(l32, 2 * c + h);
+            bf8 fa[IB][2], fb[JB][2];
 #pragma unroll
-            for (int c = 0; c < BK / 32; ++c) {
-                bf8 fa[IB][2], fb[JB][2];
-#pragma unroll
-                for (int i = 0; i < IB; ++i) {
-                    const int r = wm0 + 32 * i + l32;
-                    const u4 v = *reinterpret_cast<const u4 *>(sA + r * BK +
-                                                               16 * ((2 * c + h) ^ swz(r)));
-                    fa[i][0] = widen8(v[0], v[1], sa[i]);
-                    fa[i][1] = widen8(v[2], v[3], sa[i]);
-                }
-#pragma unroll
-                for (int j = 0; j < JB; ++j) {
-                    const int r = wn0 + 32 * j + l32;
-                    const u4 v = *reinterpret_cast<const u4 *>(sB + r * BK +
-                                                               16 * ((2 * c + h) ^ swz(r)));
-                    fb[j][0] = widen8(v[0], v[1], sb[j]);
-                    fb[j][1] = widen8(v[2], v[3], sb[j]);
-                }
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-#pragma unroll
-                    for (int i = 0; i < IB; ++i)
-#pragma unroll
-                        for (int j = 0; j < JB; ++j)
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                                fa[i][q], fb[j][q], acc[i][j], 0, 0, 0);
+            for (int i = 0; i < IB; ++i) {
+                const u4 v = *reinterpret_cast<const u4 *>(sA + (wm0 + 32 * i + l32) * 128 + slot);
+                fa[i][0] = widen8(v[0], v[1], sa[i]);
+                fa[i][1] = widen8(v[2], v[3], sa[i]);
             }
-            __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+            for (int j = 0; j < JB; ++j) {
+                const u4 v = *reinterpret_cast<const u4 *>(sB + (wn0 + 32 * j + l32) * 128 + slot);
+                fb[j][0] = widen8(v[0], v[1], sb[j]);
+                fb[j][1] = widen8(v[2], v[3], sb[j]);
+            }
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int i = 0; i < IB; ++i)
+#pragma unroll
+                    for (int j = 0; j < JB; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i][q], fb[j][q],
+                                                                            acc[i][j], 0, 0, 0);
         }
+        __builtin_amdgcn_s_setprio(0);
+    }
+    // group o stores quarter blocks o OWN .. o OWN + OWN - 1 of its waves' tiles: in
+    // round t it gets them from group o - t, so their sums are added in one order
+    const auto quarter = [&](int o, int u, auto f) {
+        const int q = o * OWN + u;
+        f(acc[q / 4 / JB][q / 4 % JB], q % 4);
+    };
+#pragma unroll
+    for (int t = 1; t < KG; ++t) {
+        f4 *const sums = reinterpret_cast<f4 *>(smem);
+        lds_barrier();
+#pragma unroll
+        for (int o = 0; o < KG; ++o)
+            if (kg == (o + KG - t) % KG)
+#pragma unroll
+                for (int u = 0; u < OWN; ++u)
+                    quarter(o, u, [&](f16v &v, int e) {
+                        sums[(wave * OWN + u) * 64 + lane] =
+                            (f4){v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]};
+                    });
+        lds_barrier();
+#pragma unroll
+        for (int o = 0; o < KG; ++o)
+            if (kg == o)
+#pragma unroll
+                for (int u = 0; u < OWN; ++u)
+                    quarter(o, u, [&](f16v &v, int e) {
+                        const int from = (o + KG - t) % KG * WG + wave % WG;
+                        const f4 w = sums[(from * OWN + u) * 64 + lane];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) v[4 * e + q] += w[q];
+                    });
     }
     // element e of block (i, j): row 32 i + 8 (e / 4) + 4 h + e % 4, column 32 j + l % 32
     float *out = p.splits > 1 ? g.ws + (size_t)blockIdx.y * g.m * g.n : g.out;
 #pragma unroll
-    for (int j = 0; j < JB; ++j) {
-        const int col = n0 + wn0 + 32 * j + l32;
-        if (col >= g.n) continue;
-        const float b = g.bias && p.splits == 1 ? g.bias[col] : 0.0f;
+    for (int i = 0; i < IB; ++i)
 #pragma unroll
-        for (int i = 0; i < IB; ++i)
+        for (int j = 0; j < JB; ++j) {
+            const int col = n0 + wn0 + 32 * j + l32;
+            if (col >= g.n) continue;
+            const float b = g.bias && p.splits == 1 ? g.bias[col] : 0.0f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int row = m0 + wm0 + 32 * i + 8 * (e / 4) + 4 * h + e % 4;
-                if (row < g.m) out[(size_t)row * g.n + col] = acc[i][j][e] + b;
+                if (kg == ((i * JB + j) * 4 + e / 4) / OWN && row < g.m)
+                    __builtin_nontemporal_store(acc[i][j][e] + b, out + (size_t)row * g.n + col);
             }
-    }
+        }
 }
 
-// The splits' sums, in their order, and the bias.
+// The splits' sums, in their order, and the bias; four elements a thread (the last
+// ones one by one), at any 4 bytes.
 __global__ void __launch_bounds__(256) join_kernel(Gemm8Args g, int splits) {
     const size_t n = (size_t)g.m * g.n;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        float s = g.ws[i];
-        for (int j = 1; j < splits; ++j) s += g.ws[(size_t)j * n + i];
-        g.out[i] = s + (g.bias ? g.bias[i % g.n] : 0.0f);
+    for (size_t i = 4 * ((size_t)blockIdx.x * 256 + threadIdx.x); i < n;
+         i += (size_t)gridDim.x * 1024) {
+        if (i + 4 <= n) {
+            lin8_f4u s = *reinterpret_cast<const lin8_f4u *>(g.ws + i);
+            for (int j = 1; j < splits; ++j)
+                s += *reinterpret_cast<const lin8_f4u *>(g.ws + (size_t)j * n + i);
+            if (g.bias)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[e] += g.bias[(i + e) % g.n];
+            *reinterpret_cast<lin8_f4u *>(g.out + i) = s;
+        } else {
+            for (size_t e = i; e < n; ++e) {
+                float s = g.ws[e];
+                for (int j = 1; j < splits; ++j) s += g.ws[(size_t)j * n + e];
+                g.out[e] = s + (g.bias ? g.bias[e % g.n] : 0.0f);
+            }
+        }
     }
 }
 
-// Few rows of a (up to 16 MT): a workgroup of W waves takes 16 rows of b, whose
-// codes go from memory straight into MFMA operands; wave w has the blocks w, w + W,
-// ... of k, and the waves' sums are added in wave order in LDS.
-template <int MT, int W>
-__global__ void __launch_bounds__(64 * W) thin_kernel(Gemm8Args g) {
-    __shared__ float part[W][MT][16][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int r = lane & 15, q = lane >> 4;
-    const int n0 = blockIdx.x * 16;
-    const size_t kp = (size_t)g.blocks * 128;
-    // (rows past the end read the last one's; their results are not stored)
-    const int nr = min(n0 + r, g.n - 1);
-    const uint8_t *b = g.b + nr * kp + 32 * q;
-    const int32_t *eb = g.b_exps + (size_t)(g.b_tiles ? nr >> 7 : nr) * g.blocks;
-    const uint8_t *a[MT];
-    const int32_t *ea[MT];
-    f4 acc[MT];
+// Up to MB rows of a: a workgroup of W waves takes RB rows of b and the waves share
+// out the blocks of k (w, w + W, ...).  Each streams its blocks of both operands
+// through two stages of its own in LDS, by DMA of whole 128-byte lines,
+// so no wave waits for another until their sums are added, in wave order.
+template <int RB, int MB, int W>
+__global__ void __launch_bounds__(64 * W) stream_kernel(Gemm8Args g) {
+    constexpr int IB = RB / 32, JB = MB / 32, STAGE = (RB + MB) * 128;
+    constexpr int ND = (RB + MB) / 8, XD = (RB + MB + 63) / 64, RING = STAGE + XD * 256;
+    static_assert(W * IB * JB * 4096 <= W * 2 * RING, "the sums fit");
+    __shared__ __attribute__((aligned(16))) char smem[W * 2 * RING];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l32 = lane & 31, h = lane >> 5;
+    const int n0 = blockIdx.x * RB;
+    const uint32_t kp = (uint32_t)g.blocks * 128u;
+    const __amdgpu_buffer_rsrc_t rb = codes_from(g.b, n0, RB, g.n, kp);
+    const __amdgpu_buffer_rsrc_t ra = codes_from(g.a, 0, MB, g.m, kp);
+    const __amdgpu_buffer_rsrc_t rxb = exps_from(g.b_exps, n0, RB, g.b_tiles, g.blocks);
+    const __amdgpu_buffer_rsrc_t rxa = exps_from(g.a_exps, 0, MB, g.a_tiles, g.blocks);
+    // DMA d moves eight rows, those of b first
+    const uint32_t off = (uint32_t)(lane / 8) * kp + (uint32_t)slot_of(lane / 8, lane % 8);
+    uint32_t xb[XD], xa[XD];  // where this lane's row of b or a has its exponents
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int mr = min(16 * t + r, g.m - 1);
-        a[t] = g.a + mr * kp + 32 * q;
-        ea[t] = g.a_exps + (size_t)(g.a_tiles ? mr >> 7 : mr) * g.blocks;
-        acc[t] = (f4){0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < XD; ++u) {
+        const int at = u * 64 + lane;
+        xb[u] = exps_at(min(n0 + min(at, RB - 1), g.n - 1), n0, g.b_tiles, g.blocks);
+        xa[u] = exps_at(min(max(at - RB, 0), g.m - 1), 0, g.a_tiles, g.blocks);
     }
-    constexpr int U = MT == 4 ? 2 : 4;  // blocks in flight
-    auto some = [&](auto count, int kb) {
-        constexpr int C = decltype(count)::value;
-        u4 vb[C][2], va[C][MT][2];
-        int xb[C], xa[C][MT];
+    char *const ring = smem + wave * (2 * RING);
+    const auto dma = [&](int i) {
+        char *st = ring + (i & 1) * RING;
+        const int kb = wave + i * W;
 #pragma unroll
-        for (int u = 0; u < C; ++u) {
-            const size_t at = (size_t)(kb + u * W) * 128;
-            vb[u][0] = *reinterpret_cast<const u4 *>(b + at);
-            vb[u][1] = *reinterpret_cast<const u4 *>(b + at + 16);
-            xb[u] = eb[kb + u * W];
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                va[u][t][0] = *reinterpret_cast<const u4 *>(a[t] + at);
-                va[u][t][1] = *reinterpret_cast<const u4 *>(a[t] + at + 16);
-                xa[u][t] = ea[t][kb + u * W];
-            }
+        for (int u = 0; u < XD; ++u) {
+            // (RB is a whole number of half waves: a lane's row is of one operand)
+            if (u * 64 + 64 <= RB)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rxb, (lds_void *)(st + STAGE + u * 256), 4,
+                                                         (int)xb[u], kb * 4, 0, 0);
+            else if (u * 64 >= RB)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rxa, (lds_void *)(st + STAGE + u * 256), 4,
+                                                         (int)xa[u], kb * 4, 0, 0);
+            else if (lane < RB % 64)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rxb, (lds_void *)(st + STAGE + u * 256), 4,
+                                                         (int)xb[u], kb * 4, 0, 0);
+            else
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rxa, (lds_void *)(st + STAGE + u * 256), 4,
+                                                         (int)xa[u], kb * 4, 0, 0);
         }
 #pragma unroll
-        for (int u = 0; u < C; ++u) {
-            const float sb = lin8_pow2(xb[u]);
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const bf8 fb = widen8(vb[u][s / 2][s % 2 * 2], vb[u][s / 2][s % 2 * 2 + 1], sb);
-#pragma unroll
-                for (int t = 0; t < MT; ++t)
-                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        fb, widen8(va[u][t][s / 2][s % 2 * 2], va[u][t][s / 2][s % 2 * 2 + 1],
-                                   lin8_pow2(xa[u][t])),
-                        acc[t], 0, 0, 0);
-            }
+        for (int d = 0; d < ND; ++d) {
+            if (d < RB / 8)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *)(st + d * 1024), 16,
+                                                         (int)(off + d * 8 * kp), kb * 128, 0, 0);
+            else if (8 * (d - RB / 8) < g.m)  // (columns past g.m are not stored)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    ra, (lds_void *)(st + d * 1024), 16, (int)(off + (d - RB / 8) * 8 * kp),
+                    kb * 128, 0, 0);
         }
     };
-    int kb = wave;
-    for (; kb + (U - 1) * W < g.blocks; kb += U * W) some(std::integral_constant<int, U>(), kb);
-    for (; kb < g.blocks; kb += W) some(std::integral_constant<int, 1>(), kb);
-    // lane: column m = r of the product, its rows n = 4 q ..
+    f16v acc[IB][JB];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) *reinterpret_cast<f4 *>(&part[wave][t][r][4 * q]) = acc[t];
+    for (int i = 0; i < IB; ++i)
+#pragma unroll
+        for (int j = 0; j < JB; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    const int count = (g.blocks - wave + W - 1) / W;  // (0 or less: none)
+    if (count > 0) dma(0);
+    for (int i = 0; i < count; ++i) {
+        // the block has landed, and the one before it is read
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if (i + 1 < count) dma(i + 1);
+        const char *st = ring + (i & 1) * RING;
+        const int *x = reinterpret_cast<const int *>(st + STAGE);
+        float sb[IB], sa[JB];
+#pragma unroll
+        for (int r = 0; r < IB; ++r) sb[r] = lin8_pow2(x[32 * r + l32]);
+#pragma unroll
+        for (int t = 0; t < JB; ++t) sa[t] = lin8_pow2(x[RB + 32 * t + l32]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int slot = slot_of(l32, 2 * c + h);
+            bf8 fb[IB][2], fa[JB][2];
+#pragma unroll
+            for (int r = 0; r < IB; ++r) {
+                const u4 v = *reinterpret_cast<const u4 *>(st + (32 * r + l32) * 128 + slot);
+                fb[r][0] = widen8(v[0], v[1], sb[r]);
+                fb[r][1] = widen8(v[2], v[3], sb[r]);
+            }
+#pragma unroll
+            for (int t = 0; t < JB; ++t) {
+                const u4 v = *reinterpret_cast<const u4 *>(st + (RB + 32 * t + l32) * 128 + slot);
+                fa[t][0] = widen8(v[0], v[1], sa[t]);
+                fa[t][1] = widen8(v[2], v[3], sa[t]);
+            }
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int r = 0; r < IB; ++r)
+#pragma unroll
+                    for (int t = 0; t < JB; ++t)
+                        acc[r][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[r][q], fa[t][q],
+                                                                            acc[r][t], 0, 0, 0);
+        }
+    }
     __syncthreads();
-    for (int i = threadIdx.x; i < MT * 256; i += 64 * W) {
-        const int m = i / 16, n = n0 + i % 16;
-        float s = part[0][m / 16][m % 16][i % 16];
+    f4 *const sums = reinterpret_cast<f4 *>(smem);
 #pragma unroll
-        for (int w = 1; w < W; ++w) s += part[w][m / 16][m % 16][i % 16];
-        if (m < g.m && n < g.n) g.out[(size_t)m * g.n + n] = s + (g.bias ? g.bias[n] : 0.0f);
+    for (int r = 0; r < IB; ++r)
+#pragma unroll
+        for (int t = 0; t < JB; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                sums[((wave * IB * JB + r * JB + t) * 4 + e) * 64 + lane] =
+                    (f4){acc[r][t][4 * e], acc[r][t][4 * e + 1], acc[r][t][4 * e + 2],
+                         acc[r][t][4 * e + 3]};
+    __syncthreads();
+    // quarter e of block (r, t): rows 32 r + 8 e + 4 h .. of b, row 32 t + l % 32 of a
+    for (int u = wave; u < IB * JB * 4; u += W) {
+        f4 s = sums[u * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < W; ++w) s += sums[(w * IB * JB * 4 + u) * 64 + lane];
+        const int m = u / 4 % JB * 32 + l32, n = n0 + u / 4 / JB * 32 + 8 * (u % 4) + 4 * h;
+        if (m >= g.m) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < g.n)
+                g.out[(size_t)m * g.n + n + e] = s[e] + (g.bias ? g.bias[n + e] : 0.0f);
     }
 }
 
-bool thin(const Gemm8Args &a) { return a.m <= 64 && a.n < (1 << 24); }
+// ---- which kernel ------------------------------------------------------------
+//
+// Every kernel is priced in microseconds with what it measured: a start, so much
+// for a step along k of the workgroups that share a CU (step[i] with i + 1 of them),
+// the results on their way out at 5.5 TB/s, and for products cut along k a second
+// launch that joins them.  The cheapest runs.
 
-Plan plan_of(const Gemm8Args &a, int num_cus) {
-    Plan p{};
-    const auto tiles = [&](int bm, int bn) {
-        p.bm = bm;
-        p.bn = bn;
-        p.tiles_m = (int)(((int64_t)a.m + bm - 1) / bm);
-        p.tiles_n = (int)(((int64_t)a.n + bn - 1) / bn);
-        return (int64_t)p.tiles_m * p.tiles_n;
-    };
-    int64_t n = tiles(256, 128);
-    if (n < num_cus) n = tiles(128, 128);
-    int splits = 1;
-    while (n * splits * 2 <= num_cus && a.blocks >= 4 * splits) splits *= 2;
-    p.per_split = a.blocks ? (a.blocks + splits - 1) / splits : 0;
-    p.splits = a.blocks ? (a.blocks + p.per_split - 1) / p.per_split : 1;
-    return p;
+struct Tiles {
+    int bm, bn, per_cu;
+    double start, step[4];
+};
+constexpr Tiles kTiles[] = {
+    {64, 64, 4, 2.6, {0.50, 0.70, 1.00, 1.22}},
+    {64, 128, 3, 3.8, {0.62, 1.08, 1.55}},
+    {128, 128, 2, 5.0, {1.00, 1.85}},
+    {256, 256, 1, 3.0, {3.10}},
+};
+
+double tiles_us(const Gemm8Args &g, const Tiles &t, int splits, int num_cus, Plan *p) {
+    p->bm = t.bm;
+    p->bn = t.bn;
+    p->tiles_m = (int)(((int64_t)g.m + t.bm - 1) / t.bm);
+    p->tiles_n = (int)(((int64_t)g.n + t.bn - 1) / t.bn);
+    p->per_split = g.blocks ? (g.blocks + splits - 1) / splits : 0;
+    p->splits = g.blocks ? (g.blocks + p->per_split - 1) / p->per_split : 1;
+    const double out = 4e-6 * g.m * (double)g.n;  // MB
+    double left = (double)p->tiles_m * p->tiles_n * p->splits / num_cus;
+    double us = t.start + p->splits * out / 5.5;
+    const double full = std::floor(left / t.per_cu);
+    us += full * p->per_split * t.step[t.per_cu - 1];
+    left -= full * t.per_cu;
+    if (left > 0) {
+        // some CUs have one workgroup more than others: half way between
+        const int most = (int)std::ceil(left);
+        const double fewer = most > 1 ? t.step[most - 2] : 0.0;
+        const double some = left - (most - 1);
+        us += p->per_split * (t.step[most - 1] - (most > 1 ? 0.5 * (1 - some) *
+                                                                 (t.step[most - 1] - fewer)
+                                                           : 0.0));
+    }
+    if (p->splits > 1) us += 3.0 + (p->splits + 1) * out / 4.5;
+    return us;
+}
+
+// Waves of the streaming kernel for up to 32 or 64 rows of a; 0: none.  One
+// workgroup a CU has eight waves (six with 64 rows), more of them four, so that two
+// (for 64 rows: twice the rows of b) share a CU: 32 x 14336 x 4096 12.4 us, 15.9 with
+// eight; 32 x 4096 x 4096 6.4 us, 7.9 with four.
+struct Stream {
+    int rows_b = 0, rows_a = 0, waves = 0;
+    double us = 0;
+};
+Stream stream_of(const Gemm8Args &g, int num_cus) {
+    Stream r;
+    if (g.m > 64) return r;
+    const bool one = ((int64_t)g.n + 31) / 32 <= num_cus;
+    r.rows_a = g.m <= 32 ? 32 : 64;
+    r.rows_b = r.rows_a == 64 && !one ? 64 : 32;
+    r.waves = !one ? 4 : r.rows_a == 32 ? 8 : 6;
+    const int per_cu = !one && r.rows_a == 32 ? 2 : 1;
+    const double step = r.rows_b == 64 ? 1.75 : r.rows_a == 64 ? 1.3 : one ? 0.95 : 1.25;
+    const double turns = std::ceil(std::ceil((double)g.n / r.rows_b) / ((double)num_cus * per_cu));
+    r.us = 2.5 + turns * ((g.blocks + r.waves - 1) / r.waves) * step;
+    return r;
+}
+
+struct Choice {
+    Stream stream;
+    Plan tiles{};
+};
+Choice choose(const Gemm8Args &g, int num_cus) {
+    Choice c;
+    const Stream s = stream_of(g, num_cus);
+    double best = 0;
+    for (const Tiles &t : kTiles)
+        for (int splits = 1; splits <= 8; splits *= 2) {
+            Plan p{};
+            if (splits > 1 && g.blocks < 2 * splits) break;
+            const double us = tiles_us(g, t, splits, num_cus, &p);
+            if (c.tiles.bm == 0 || us < best) {
+                best = us;
+                c.tiles = p;
+            }
+        }
+    // (up to 32 rows no tiles measured faster)
+    if (s.waves && (g.m <= 32 || s.us <= best)) c.stream = s;
+    return c;
+}
+
+template <int BM, int BN, int WM, int WN, int KG, int MINW>
+void run_tiles(const Gemm8Args &g, const Plan &p, hipStream_t s) {
+    const dim3 grid((unsigned)((p.tiles_m * p.tiles_n + 7) / 8 * 8), (unsigned)p.splits);
+    gemm8_kernel<BM, BN, WM, WN, KG, MINW><<<grid, BM / WM * (BN / WN) * KG * 64, 0, s>>>(g, p);
+}
+
+template <int RB, int MB, int W>
+void run_stream(const Gemm8Args &g, hipStream_t s) {
+    stream_kernel<RB, MB, W><<<(unsigned)(((int64_t)g.n + RB - 1) / RB), 64 * W, 0, s>>>(g);
 }
 
 }  // namespace
 
 size_t gemm8_workspace(const Gemm8Args &a, int num_cus) {
-    if (thin(a)) return 0;
-    const Plan p = plan_of(a, num_cus);
-    return p.splits > 1 ? (size_t)p.splits * a.m * a.n : 0;
+    if (a.m == 0 || a.n == 0) return 0;
+    const Choice c = choose(a, num_cus);
+    return !c.stream.waves && c.tiles.splits > 1 ? (size_t)c.tiles.splits * a.m * a.n : 0;
 }
 
 void gemm8(const Gemm8Args &a, int num_cus, hipStream_t s) {
     if (a.m == 0 || a.n == 0) return;
-    if (thin(a)) {
-        const unsigned n = (unsigned)((a.n + 15) / 16);
-        if (a.m <= 16) thin_kernel<1, 8><<<n, 512, 0, s>>>(a);
-        else if (a.m <= 32) thin_kernel<2, 8><<<n, 512, 0, s>>>(a);
-        else thin_kernel<4, 8><<<n, 512, 0, s>>>(a);
+    const Choice c = choose(a, num_cus);
+    if (const Stream &r = c.stream; r.waves) {
+        if (r.rows_a == 32) r.waves == 8 ? run_stream<32, 32, 8>(a, s) : run_stream<32, 32, 4>(a, s);
+        else r.rows_b == 32 ? run_stream<32, 64, 6>(a, s) : run_stream<64, 64, 4>(a, s);
         return;
     }
-    const Plan p = plan_of(a, num_cus);
-    const dim3 grid((unsigned)((p.tiles_m * p.tiles_n + 7) / 8 * 8), (unsigned)p.splits);
-    if (p.bm == 256) gemm8_kernel<256, 128, 128, 64, 64, 3, 2><<<grid, 256, 0, s>>>(a, p);
-    else gemm8_kernel<128, 128, 64, 64, 64, 3, 3><<<grid, 256, 0, s>>>(a, p);
+    const Plan &p = c.tiles;
+    if (p.bm == 256) run_tiles<256, 256, 64, 64, 1, 4>(a, p, s);
+    else if (p.bm == 128) run_tiles<128, 128, 64, 64, 2, 2>(a, p, s);
+    else if (p.bn == 128) run_tiles<64, 128, 32, 64, 2, 4>(a, p, s);
+    else run_tiles<64, 64, 32, 32, 2, 4>(a, p, s);
     if (p.splits > 1) {
-        const size_t work = ((size_t)a.m * a.n + 255) / 256;
+        const size_t work = ((size_t)a.m * a.n + 1023) / 1024;
         join_kernel<<<(unsigned)std::min(work, (size_t)num_cus * 16), 256, 0, s>>>(a, p.splits);
     }
 }

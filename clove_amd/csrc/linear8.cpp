@@ -212,9 +212,9 @@ TensorNode HipBackend::matmul_e4m3(const Tensor &a, const Tensor &a_exps, const 
                       "bias must hold " + std::to_string(n) + " elements, got " +
                           shape_str(bias->shape));
     }
-    // (tiles are counted in 32 bits and a grid holds 2^32 threads)
-    CLOVE_REQUIRE(((m + 127) / 128) * ((n + 127) / 128) < (size_t(1) << 22), CLOVE_HIP_ERR_SHAPE,
-                  "matmul_e4m3: the result has too many tiles of 128 x 128");
+    // (a grid holds 2^32 threads, up to 512 a tile)
+    CLOVE_REQUIRE(((m + 63) / 64) * ((n + 63) / 64) < (size_t(1) << 22), CLOVE_HIP_ERR_SHAPE,
+                  "matmul_e4m3: the result has 2^22 tiles of 64 x 64 or more");
     TensorNode out = new_tensor(with_last(a, n), CLOVE_HIP_F32);
     g.a = a.u8();
     g.b = b.u8();
