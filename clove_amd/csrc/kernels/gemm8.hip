@@ -74,23 +74,27 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t exps_from(const int32_t *p, in
 // eight rows (lane l: slot l % 8 of row l / 8) still reads whole lines.
 __device__ __forceinline__ int slot_of(int row, int k16) { return 16 * (k16 ^ (row & 7)); }
 
-// BM x BN tiles in KG groups of waves of WM x WN each; group k takes the chunks k,
+// BM x BN tiles in KG groups of waves of 64 x 64 each; group k takes the chunks k,
 // k + KG, ... (32 codes) of every block, and the groups' sums are added at the end:
 // more waves a CU without smaller tiles for each, whose operands would be widened
-// more often.  Blocks of both operands and their exponents move by buffer->LDS DMA
-// into two stages, one filling while the other is multiplied (in registers the
-// exponents would make every block wait for all DMAs in flight).
+// more often (four conversions an MFMA here, eight with waves of 32 x 32).  Blocks of
+// both operands and their exponents move by buffer->LDS DMA into two stages, one
+// filling while the other is multiplied (in registers the exponents would make every
+// block wait for all DMAs in flight).
 //
 // What bounds it: 4096^3 in 256 x 256 tiles of sixteen waves 114-117 us, 1180-1207
 // TFLOP/s, of which the 64 MiB of results are some 13 us at the end; a large bf16
 // library product runs at 1208 on the same card, at its power limit.  Four waves
 // of 128 x 64 on 256 x 128 tiles 134 us, of 64 x 64 on 128 x 128 124-134.  Results
-// stored with the non-temporal policy: 8192 x 4096 x 1024 86 us, 92 without.
-template <int BM, int BN, int WM, int WN, int KG, int MINW>
-__global__ void __launch_bounds__(BM / WM * (BN / WN) * KG * 64)
+// stored with the non-temporal policy: 8192 x 4096 x 1024 86 us, 92 without.  Small
+// products are bound by a block's chain of barrier, reads, conversions and MFMAs
+// (0.5-0.65 us with a workgroup a CU; three to six stages no quicker): 768 x 768 x
+// 1554 9.2 us, waves of 32 x 32 on 64 x 64 tiles 9.2-10.5.
+template <int BM, int BN, int KG, int MINW>
+__global__ void __launch_bounds__(BM / 64 * (BN / 64) * KG * 64)
     __attribute__((amdgpu_waves_per_eu(MINW))) gemm8_kernel(Gemm8Args g, Plan p) {
-    constexpr int WG = BM / WM * (BN / WN), NW = WG * KG;  // waves of a group, and all
-    constexpr int IB = WM / 32, JB = WN / 32;
+    constexpr int WG = BM / 64 * (BN / 64), NW = WG * KG;  // waves of a group, and all
+    constexpr int IB = 2, JB = 2;                          // a wave's 32 x 32 blocks
     constexpr int OWN = IB * JB * 4 / KG;                  // quarter blocks that a group stores
     constexpr int STAGE = (BM + BN) * 128;
     constexpr int ND = (BM + BN) / 8, IW = (ND + NW - 1) / NW;   // DMAs a block, and a wave's
@@ -109,7 +113,7 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * KG * 64)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l32 = lane & 31, h = lane >> 5;
     const int kg = wave / WG;
-    const int wm0 = wave % WG / (BN / WN) * WM, wn0 = wave % (BN / WN) * WN;
+    const int wm0 = wave % WG / (BN / 64) * 64, wn0 = wave % (BN / 64) * 64;
     const __amdgpu_buffer_rsrc_t ra = codes_from(g.a, m0, BM, g.m, kp);
     const __amdgpu_buffer_rsrc_t rb = codes_from(g.b, n0, BN, g.n, kp);
     const __amdgpu_buffer_rsrc_t rxa = exps_from(g.a_exps, m0, BM, g.a_tiles, g.blocks);
@@ -236,33 +240,54 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * KG * 64)
                     });
     }
     // element e of block (i, j): row 32 i + 8 (e / 4) + 4 h + e % 4, column 32 j + l % 32
-    float *out = p.splits > 1 ? g.ws + (size_t)blockIdx.y * g.m * g.n : g.out;
+    const int row0 = m0 + wm0 + 4 * h, col0 = n0 + wn0 + l32;
+    const size_t n = (size_t)g.n;
+    float *const out = (p.splits > 1 ? g.ws + (size_t)blockIdx.y * g.m * n : g.out) +
+                       (size_t)row0 * n + col0;
+    float bias[JB];
 #pragma unroll
-    for (int i = 0; i < IB; ++i)
+    for (int j = 0; j < JB; ++j)
+        bias[j] = g.bias && p.splits == 1 && col0 + 32 * j < g.n ? g.bias[col0 + 32 * j] : 0.0f;
+    const auto store = [&](auto whole) {
 #pragma unroll
-        for (int j = 0; j < JB; ++j) {
-            const int col = n0 + wn0 + 32 * j + l32;
-            if (col >= g.n) continue;
-            const float b = g.bias && p.splits == 1 ? g.bias[col] : 0.0f;
+        for (int o = 0; o < KG; ++o)
+            if (kg == o)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int row = m0 + wm0 + 32 * i + 8 * (e / 4) + 4 * h + e % 4;
-                if (kg == ((i * JB + j) * 4 + e / 4) / OWN && row < g.m)
-                    __builtin_nontemporal_store(acc[i][j][e] + b, out + (size_t)row * g.n + col);
-            }
-        }
+                for (int u = 0; u < OWN; ++u) {
+                    const int q = o * OWN + u, i = q / 4 / JB, j = q / 4 % JB;
+                    if (!decltype(whole)::value && col0 + 32 * j >= g.n) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int down = 32 * i + 8 * (q % 4) + e;
+                        if (decltype(whole)::value || row0 + down < g.m)
+                            __builtin_nontemporal_store(acc[i][j][4 * (q % 4) + e] + bias[j],
+                                                        out + down * n + 32 * j);
+                    }
+                }
+    };
+    // (a check for each element costs more than its store)
+    if (m0 + BM <= g.m && n0 + BN <= g.n)
+        store(std::true_type());
+    else
+        store(std::false_type());
 }
 
-// The splits' sums, in their order, and the bias; four elements a thread (the last
-// ones one by one), at any 4 bytes.
+// The splits' sums (up to kMaxSplits), in their order, and the bias; four elements a
+// thread (the last ones one by one), at any 4 bytes, all loads on their way first.
+constexpr int kMaxSplits = 8;
 __global__ void __launch_bounds__(256) join_kernel(Gemm8Args g, int splits) {
     const size_t n = (size_t)g.m * g.n;
     for (size_t i = 4 * ((size_t)blockIdx.x * 256 + threadIdx.x); i < n;
          i += (size_t)gridDim.x * 1024) {
         if (i + 4 <= n) {
-            lin8_f4u s = *reinterpret_cast<const lin8_f4u *>(g.ws + i);
-            for (int j = 1; j < splits; ++j)
-                s += *reinterpret_cast<const lin8_f4u *>(g.ws + (size_t)j * n + i);
+            lin8_f4u v[kMaxSplits];
+#pragma unroll
+            for (int j = 0; j < kMaxSplits; ++j)
+                if (j < splits) v[j] = *reinterpret_cast<const lin8_f4u *>(g.ws + j * n + i);
+            lin8_f4u s = v[0];
+#pragma unroll
+            for (int j = 1; j < kMaxSplits; ++j)
+                if (j < splits) s += v[j];
             if (g.bias)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[e] += g.bias[(i + e) % g.n];
@@ -270,7 +295,7 @@ __global__ void __launch_bounds__(256) join_kernel(Gemm8Args g, int splits) {
         } else {
             for (size_t e = i; e < n; ++e) {
                 float s = g.ws[e];
-                for (int j = 1; j < splits; ++j) s += g.ws[(size_t)j * n + e];
+                for (int j = 1; j < splits; ++j) s += g.ws[j * n + e];
                 g.out[e] = s + (g.bias ? g.bias[e % g.n] : 0.0f);
             }
         }
@@ -420,9 +445,9 @@ struct Tiles {
     double start, step[4];
 };
 constexpr Tiles kTiles[] = {
-    {64, 64, 4, 2.6, {0.50, 0.70, 1.00, 1.22}},
-    {64, 128, 3, 3.8, {0.62, 1.08, 1.55}},
-    {128, 128, 2, 5.0, {1.00, 1.85}},
+    {64, 64, 4, 2.3, {0.50, 0.59, 0.82, 1.16}},
+    {64, 128, 3, 1.8, {0.64, 0.98, 1.45}},
+    {128, 128, 2, 2.0, {1.05, 1.85}},
     {256, 256, 1, 3.0, {3.10}},
 };
 
@@ -435,19 +460,15 @@ double tiles_us(const Gemm8Args &g, const Tiles &t, int splits, int num_cus, Pla
     p->splits = g.blocks ? (g.blocks + p->per_split - 1) / p->per_split : 1;
     const double out = 4e-6 * g.m * (double)g.n;  // MB
     double left = (double)p->tiles_m * p->tiles_n * p->splits / num_cus;
-    double us = t.start + p->splits * out / 5.5;
     const double full = std::floor(left / t.per_cu);
-    us += full * p->per_split * t.step[t.per_cu - 1];
+    double step = full * t.step[t.per_cu - 1];
     left -= full * t.per_cu;
-    if (left > 0) {
-        // some CUs have one workgroup more than others: half way between
+    if (left > 0) {  // between so many workgroups on every CU and one more on some
         const int most = (int)std::ceil(left);
-        const double fewer = most > 1 ? t.step[most - 2] : 0.0;
-        const double some = left - (most - 1);
-        us += p->per_split * (t.step[most - 1] - (most > 1 ? 0.5 * (1 - some) *
-                                                                 (t.step[most - 1] - fewer)
-                                                           : 0.0));
+        const double fewer = most > 1 ? t.step[most - 2] : t.step[0];
+        step += fewer + (t.step[most - 1] - fewer) * (left - (most - 1));
     }
+    double us = t.start + p->per_split * step + p->splits * out / 5.5;
     if (p->splits > 1) us += 3.0 + (p->splits + 1) * out / 4.5;
     return us;
 }
@@ -483,7 +504,7 @@ Choice choose(const Gemm8Args &g, int num_cus) {
     const Stream s = stream_of(g, num_cus);
     double best = 0;
     for (const Tiles &t : kTiles)
-        for (int splits = 1; splits <= 8; splits *= 2) {
+        for (int splits = 1; splits <= kMaxSplits; splits *= 2) {
             Plan p{};
             if (splits > 1 && g.blocks < 2 * splits) break;
             const double us = tiles_us(g, t, splits, num_cus, &p);
@@ -497,10 +518,10 @@ Choice choose(const Gemm8Args &g, int num_cus) {
     return c;
 }
 
-template <int BM, int BN, int WM, int WN, int KG, int MINW>
+template <int BM, int BN, int KG, int MINW>
 void run_tiles(const Gemm8Args &g, const Plan &p, hipStream_t s) {
     const dim3 grid((unsigned)((p.tiles_m * p.tiles_n + 7) / 8 * 8), (unsigned)p.splits);
-    gemm8_kernel<BM, BN, WM, WN, KG, MINW><<<grid, BM / WM * (BN / WN) * KG * 64, 0, s>>>(g, p);
+    gemm8_kernel<BM, BN, KG, MINW><<<grid, BM / 64 * (BN / 64) * KG * 64, 0, s>>>(g, p);
 }
 
 template <int RB, int MB, int W>
@@ -525,10 +546,10 @@ void gemm8(const Gemm8Args &a, int num_cus, hipStream_t s) {
         return;
     }
     const Plan &p = c.tiles;
-    if (p.bm == 256) run_tiles<256, 256, 64, 64, 1, 4>(a, p, s);
-    else if (p.bm == 128) run_tiles<128, 128, 64, 64, 2, 2>(a, p, s);
-    else if (p.bn == 128) run_tiles<64, 128, 32, 64, 2, 4>(a, p, s);
-    else run_tiles<64, 64, 32, 32, 2, 4>(a, p, s);
+    if (p.bm == 256) run_tiles<256, 256, 1, 4>(a, p, s);
+    else if (p.bm == 128) run_tiles<128, 128, 2, 2>(a, p, s);
+    else if (p.bn == 128) run_tiles<64, 128, 2, 2>(a, p, s);
+    else run_tiles<64, 64, 4, 4>(a, p, s);
     if (p.splits > 1) {
         const size_t work = ((size_t)a.m * a.n + 1023) / 1024;
         join_kernel<<<(unsigned)std::min(work, (size_t)num_cus * 16), 256, 0, s>>>(a, p.splits);
