@@ -298,17 +298,17 @@ struct RmsNormArgs {
 size_t rms_norm_stats(size_t rows, int cols);
 void rms_norm(const RmsNormArgs &a, hipStream_t s);
 // grad_h = r (g - h r^2 mean(g h)) + grad_sum with g = grad_out * gamma, r the
-// row's 1 / sqrt(mean(h^2) + eps); part receives rms_norm_grad_parts() rows of
-// cols partial sums of grad_out * h * r, for the caller to add up.
+// row's 1 / sqrt(mean(h^2) + eps); grad_gamma = the sum over rows of grad_out h r.
 struct RmsNormGradArgs {
     const float *h, *gamma, *grad_out, *grad_sum;  // grad_sum may be null
-    float *grad_h, *part;                          // either may be null
-    double *stats;                                 // rms_norm_grad_stats() doubles
+    float *grad_h, *grad_gamma;                    // either may be null
+    float *part;    // rms_norm_grad_floats() floats, null without grad_gamma
+    double *stats;  // rms_norm_grad_stats() doubles
     size_t rows;
     int cols;
     float eps;
 };
-size_t rms_norm_grad_parts(size_t rows, int cols, int num_cus);
+size_t rms_norm_grad_floats(size_t rows, int cols, int num_cus);
 size_t rms_norm_grad_stats(size_t rows, int cols);
 void rms_norm_grad(const RmsNormGradArgs &a, int num_cus, hipStream_t s);
 

@@ -8,6 +8,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "launch.hpp"
@@ -53,11 +54,15 @@ __device__ __forceinline__ unsigned lin8_mag4(cl_f4 x) {
     return max(max(lin8_mag(x.x), lin8_mag(x.y)), max(lin8_mag(x.z), lin8_mag(x.w)));
 }
 
-// The maximum over the 32 lanes of each half of the wave.
+// The maximum over the 32 lanes of each half of the wave: four rotations of 16
+// lanes (row_ror 8, 4, 2, 1), then the two rows of a half against each other.
 __device__ __forceinline__ unsigned half_umax(unsigned v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
-    return v;
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x124, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x122, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x121, 0xf, 0xf, false));
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return max((unsigned)r[0], (unsigned)r[1]);
 }
 
 // Elements 4c .. 4c + 3 of a row of `cols`, zeros past its end.  ODD: the row
@@ -96,6 +101,15 @@ __device__ __forceinline__ void lin8_store4(float *row, int c, int cols, cl_f4 v
             if (left > 2) p[2] = v.z;
         }
     }
+}
+
+// A grid holds 2^32 threads: launch(workgroups, workgroups before) for n of them,
+// 2^21 (of up to 1024 threads) at a time.
+template <class F>
+void lin8_grids(size_t n, F launch) {
+    constexpr size_t most = size_t(1) << 21;
+    for (size_t done = 0; done < n; done += most)
+        launch((unsigned)std::min(most, n - done), done);
 }
 
 }  // namespace k

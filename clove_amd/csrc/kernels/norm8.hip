@@ -11,8 +11,6 @@
 //   grad_gamma = sum over rows of grad_out h r
 //
 // with the two sums of a row in 64 bits (h^2 leaves f32's range from 2^64 on).
-#include <algorithm>
-
 #include "linear8.h"
 
 namespace clove {
@@ -148,21 +146,13 @@ __global__ void __launch_bounds__(256) norm_apply_kernel(RmsNormArgs a, unsigned
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// A grid holds 2^32 threads: more workgroups go in several launches.
-constexpr size_t kGrid = size_t(1) << 21;
-template <class F>
-void in_grids(size_t n, F launch) {
-    for (size_t done = 0; done < n; done += kGrid)
-        launch((unsigned)std::min(kGrid, n - done), done);
-}
-
 template <bool ODD, bool OUT8>
 void norm_any(const RmsNormArgs &a, hipStream_t s) {
     // (with an 8-bit output the lanes behind the row write its padding)
     const int64_t cols = OUT8 ? ((int64_t)a.cols + 127) / 128 * 128 : a.cols;
     auto go = [&](auto kernel, int t, int tr) {
         const size_t per = t / tr;
-        in_grids((a.rows + per - 1) / per, [&](unsigned n, size_t done) {
+        lin8_grids((a.rows + per - 1) / per, [&](unsigned n, size_t done) {
             kernel<<<n, t, 0, s>>>(a, done * per);
         });
     };
@@ -174,11 +164,11 @@ void norm_any(const RmsNormArgs &a, hipStream_t s) {
     if (cols <= 4096) return go(norm_kernel<256, 256, 4, ODD, OUT8>, 256, 256);
     if (cols <= 8192) return go(norm_kernel<256, 256, 8, ODD, OUT8>, 256, 256);
     if (cols <= kWide) return go(norm_kernel<1024, 1024, 4, ODD, OUT8>, 1024, 1024);
-    in_grids(a.rows, [&](unsigned n, size_t done) {
+    lin8_grids(a.rows, [&](unsigned n, size_t done) {
         norm_stats_kernel<ODD><<<n, 1024, 0, s>>>(a, done);
     });
     const unsigned parts = (unsigned)((cols + 1023) / 1024);
-    in_grids(a.rows * parts, [&](unsigned n, size_t done) {
+    lin8_grids(a.rows * parts, [&](unsigned n, size_t done) {
         norm_apply_kernel<ODD, OUT8><<<n, 256, 0, s>>>(a, parts, done);
     });
 }
@@ -198,12 +188,12 @@ __device__ __forceinline__ void coefficients(double sq, double gh, int cols, flo
     *m = *r * *r * *r * (gh / (double)cols);
 }
 
-// Chunk c of row `row`: grad_h out, grad_out h r added to *acc.
+// Chunk c of row `row`: grad_h out, grad_out h r added to *acc; ds: grad_sum's chunk.
 template <bool ODD>
 __device__ __forceinline__ void grad_chunk(const RmsNormGradArgs &a, size_t row, int c, cl_f4 h,
-                                           cl_f4 gy, cl_f4 gamma, double r, double m, cl_f4 *acc) {
-    cl_f4 ds = {0.f, 0.f, 0.f, 0.f}, dh;
-    if (a.grad_sum) ds = lin8_load4<ODD>(a.grad_sum + row * a.cols, c, a.cols);
+                                           cl_f4 gy, cl_f4 ds, cl_f4 gamma, double r, double m,
+                                           cl_f4 *acc) {
+    cl_f4 dh;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         (*acc)[e] += gy[e] * (float)((double)h[e] * r);
@@ -213,42 +203,104 @@ __device__ __forceinline__ void grad_chunk(const RmsNormGradArgs &a, size_t row,
     if (a.grad_h) lin8_store4<ODD>(a.grad_h + row * a.cols, c, a.cols, dh);
 }
 
-// A workgroup walks the rows blockIdx.x, + gridDim.x, ...; its threads keep the
-// sums of their columns and write them as one row of `part`.
-template <int T, int NV, bool ODD>
+// Floats of a row of `part`: whole vectors, zeros behind the columns.
+__host__ __device__ __forceinline__ size_t part_pitch(int cols) {
+    return ((size_t)cols + 3) / 4 * 4;
+}
+
+// TR threads a row.  A workgroup walks the rows from blockIdx.x * T / TR on, the
+// next one on its way while one is reduced; its threads keep the sums of their
+// columns and write them, those of its T / TR rows added up, as one row of `part`.
+template <int T, int TR, int NV, bool ODD>
 __global__ void __launch_bounds__(T) grad_kernel(RmsNormGradArgs a) {
+    constexpr int PER = T / TR;
     __shared__ double red[2 * T / 64];
-    const int t = threadIdx.x;
-    cl_f4 gamma[NV], acc[NV];
+    __shared__ cl_f4 sums[PER > 1 ? PER - 1 : 1][PER > 1 ? NV * TR : 1];
+    const int t = threadIdx.x % TR, mine = threadIdx.x / TR;
+    cl_f4 gamma[NV], acc[NV], h[2][NV], gy[2][NV], ds[2][NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        gamma[i] = lin8_load4<ODD>(a.gamma, t + T * i, a.cols);
+        gamma[i] = lin8_load4<ODD>(a.gamma, t + TR * i, a.cols);
         acc[i] = (cl_f4){0.f, 0.f, 0.f, 0.f};
     }
-    for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        cl_f4 h[NV], gy[NV];
+    const auto load = [&](size_t row, int s) {
+        const bool in = row < a.rows;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            h[i] = lin8_load4<ODD>(a.h + row * a.cols, t + T * i, a.cols);
-            gy[i] = lin8_load4<ODD>(a.grad_out + row * a.cols, t + T * i, a.cols);
+            const int cols = in ? a.cols : 0, c = t + TR * i;
+            h[s][i] = lin8_load4<ODD>(a.h + row * a.cols, c, cols);
+            gy[s][i] = lin8_load4<ODD>(a.grad_out + row * a.cols, c, cols);
+            ds[s][i] = lin8_load4<ODD>(a.grad_sum + row * a.cols, c, a.grad_sum ? cols : 0);
         }
-        double s[2] = {0.0, 0.0};
+    };
+    const auto work = [&](size_t row, int s) {
+        double v[2] = {0.0, 0.0};
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            s[0] = square_sum(h[i], s[0]);
-            s[1] = dot(gy[i] * gamma[i], h[i], s[1]);
+            v[0] = square_sum(h[s][i], v[0]);
+            v[1] = dot(gy[s][i] * gamma[i], h[s][i], v[1]);
         }
-        row_sum<T, T>(s, red);
+        row_sum<T, TR>(v, red);
         double r, m;
-        coefficients(s[0], s[1], a.cols, a.eps, &r, &m);
+        coefficients(v[0], v[1], a.cols, a.eps, &r, &m);
+        if (row < a.rows)
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            grad_chunk<ODD>(a, row, t + T * i, h[i], gy[i], gamma[i], r, m, &acc[i]);
+            for (int i = 0; i < NV; ++i)
+                grad_chunk<ODD>(a, row, t + TR * i, h[s][i], gy[s][i], ds[s][i], gamma[i], r, m,
+                                &acc[i]);
+    };
+    // (whole workgroups walk together: their barriers are in row_sum)
+    const size_t step = (size_t)gridDim.x * PER;
+    size_t row0 = (size_t)blockIdx.x * PER;
+    load(row0 + mine, 0);
+    while (true) {
+        if (row0 + step < a.rows) load(row0 + step + mine, 1);
+        work(row0 + mine, 0);
+        if ((row0 += step) >= a.rows) break;
+        if (row0 + step < a.rows) load(row0 + step + mine, 0);
+        work(row0 + mine, 1);
+        if ((row0 += step) >= a.rows) break;
     }
-    if (a.part)
+    if (!a.part) return;
+    if constexpr (PER > 1) {
+        if (mine)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) sums[mine - 1][t + TR * i] = acc[i];
+        __syncthreads();
+        if (mine) return;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            lin8_store4<ODD>(a.part + (size_t)blockIdx.x * a.cols, t + T * i, a.cols, acc[i]);
+#pragma unroll
+            for (int w = 1; w < PER; ++w) acc[i] += sums[w - 1][t + TR * i];
+    }
+    const size_t pitch = part_pitch(a.cols);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (4 * (size_t)(t + TR * i) < pitch)
+            *reinterpret_cast<cl_f4 *>(a.part + blockIdx.x * pitch + 4 * (t + TR * i)) = acc[i];
+}
+
+// grad_gamma: the rows of `part` added up, 64 columns to a workgroup, 64 threads
+// to four of them, every 64th row each and then in their order.
+__global__ void __launch_bounds__(1024) grad_join_kernel(RmsNormGradArgs a, int parts,
+                                                          size_t done) {
+    __shared__ cl_f4 sums[64][16];
+    const size_t pitch = part_pitch(a.cols);
+    const int q = threadIdx.x & 15, group = threadIdx.x >> 4;
+    const size_t col0 = (done + blockIdx.x) * 64, at = col0 + 4 * q;
+    cl_f4 s = {0.f, 0.f, 0.f, 0.f};
+    if (at < pitch)
+#pragma unroll 8
+        for (int p = group; p < parts; p += 64)
+            s += *reinterpret_cast<const cl_f4 *>(a.part + p * pitch + at);
+    sums[group][q] = s;
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    const size_t col = col0 + threadIdx.x;
+    float total = 0.0f;
+#pragma unroll 16
+    for (int g = 0; g < 64; ++g) total += sums[g][threadIdx.x / 4][threadIdx.x % 4];
+    if (col < (size_t)a.cols) a.grad_gamma[col] = total;
 }
 
 // Rows that registers do not hold (sixteen columns a thread and four arrays of them
@@ -280,20 +332,43 @@ __global__ void __launch_bounds__(256) grad_apply_kernel(RmsNormGradArgs a, unsi
     for (size_t row = share; row < a.rows; row += shares) {
         const cl_f4 h = lin8_load4<ODD>(a.h + row * a.cols, c, a.cols);
         const cl_f4 gy = lin8_load4<ODD>(a.grad_out + row * a.cols, c, a.cols);
-        grad_chunk<ODD>(a, row, c, h, gy, gamma, a.stats[2 * row], a.stats[2 * row + 1], &acc);
+        const cl_f4 ds =
+            lin8_load4<ODD>(a.grad_sum + row * a.cols, c, a.grad_sum ? a.cols : 0);
+        grad_chunk<ODD>(a, row, c, h, gy, ds, gamma, a.stats[2 * row], a.stats[2 * row + 1], &acc);
     }
-    if (a.part) lin8_store4<ODD>(a.part + (size_t)share * a.cols, c, a.cols, acc);
+    const size_t pitch = part_pitch(a.cols);
+    if (a.part && 4 * (size_t)c < pitch)
+        *reinterpret_cast<cl_f4 *>(a.part + share * pitch + 4 * (size_t)c) = acc;
+}
+
+// Rows that a workgroup of grad_kernel takes at once.
+size_t grad_rows(int cols) { return cols <= 128 ? 8 : cols <= 1024 ? 4 : 1; }
+// Workgroups, and rows of `part`.  With a row on its way one a CU keeps the memory
+// busy where there are many rows of full registers ([8192, 4096] 101 us, 104 with
+// four, whose join takes 2.6 us more; without the row ahead 179 and 104); fewer or
+// shorter rows need two, narrow ones four ([32768, 200] 29 us with one, 18 with four).
+size_t grad_parts(size_t rows, int cols, int num_cus) {
+    const size_t cus = (size_t)num_cus;
+    if (cols > kWideGrad) {  // so many shares for each group of 1024 columns
+        const size_t groups = ((size_t)cols + 1023) / 1024;
+        return std::min(rows, std::max(cus * 4 / groups, (size_t)1));
+    }
+    const size_t per = grad_rows(cols);
+    const bool one = cols > 4096 || (cols > 2048 && rows >= 16 * cus);
+    return std::min((rows + per - 1) / per, cus * (one ? 1 : cols > 256 ? 2 : 4));
 }
 
 template <bool ODD>
-void grad_any(const RmsNormGradArgs &a, int num_cus, hipStream_t s) {
-    const unsigned n = (unsigned)rms_norm_grad_parts(a.rows, a.cols, num_cus);
-    if (a.cols <= 256) return (void)(grad_kernel<64, 1, ODD><<<n, 64, 0, s>>>(a));
-    if (a.cols <= 1024) return (void)(grad_kernel<256, 1, ODD><<<n, 256, 0, s>>>(a));
-    if (a.cols <= 2048) return (void)(grad_kernel<256, 2, ODD><<<n, 256, 0, s>>>(a));
-    if (a.cols <= 4096) return (void)(grad_kernel<256, 4, ODD><<<n, 256, 0, s>>>(a));
-    if (a.cols <= 8192) return (void)(grad_kernel<512, 4, ODD><<<n, 512, 0, s>>>(a));
-    in_grids(a.rows, [&](unsigned g, size_t done) {
+void grad_any(const RmsNormGradArgs &a, unsigned n, hipStream_t s) {
+    const auto go = [&](auto kernel, int t) { kernel<<<n, t, 0, s>>>(a); };
+    if (a.cols <= 128) return go(grad_kernel<256, 32, 1, ODD>, 256);
+    if (a.cols <= 256) return go(grad_kernel<256, 64, 1, ODD>, 256);
+    if (a.cols <= 512) return go(grad_kernel<256, 64, 2, ODD>, 256);
+    if (a.cols <= 1024) return go(grad_kernel<256, 64, 4, ODD>, 256);
+    if (a.cols <= 2048) return go(grad_kernel<256, 256, 2, ODD>, 256);
+    if (a.cols <= 4096) return go(grad_kernel<256, 256, 4, ODD>, 256);
+    if (a.cols <= kWideGrad) return go(grad_kernel<512, 512, 4, ODD>, 512);
+    lin8_grids(a.rows, [&](unsigned g, size_t done) {
         grad_stats_kernel<ODD><<<g, 1024, 0, s>>>(a, done);
     });
     const unsigned parts = (unsigned)(((size_t)a.cols + 1023) / 1024);
@@ -314,20 +389,21 @@ void rms_norm(const RmsNormArgs &a, hipStream_t s) {
         odd ? norm_any<true, true>(a, s) : norm_any<false, true>(a, s);
 }
 
-size_t rms_norm_grad_parts(size_t rows, int cols, int num_cus) {
-    // (wide rows: so many shares for each group of 1024 columns)
-    const size_t groups = cols > kWideGrad ? ((size_t)cols + 1023) / 1024 : 1;
-    const size_t per_cu = cols <= 256 ? 16 : cols <= 1024 ? 8 : cols <= 4096 ? 4 : 2;
-    return std::min(rows, std::max((size_t)num_cus * per_cu / groups, (size_t)1));
+size_t rms_norm_grad_floats(size_t rows, int cols, int num_cus) {
+    return grad_parts(rows, cols, num_cus) * part_pitch(cols);
 }
 size_t rms_norm_grad_stats(size_t rows, int cols) { return cols > kWideGrad ? 2 * rows : 0; }
 
 void rms_norm_grad(const RmsNormGradArgs &a, int num_cus, hipStream_t s) {
     if (a.rows == 0 || a.cols == 0) return;
     const bool odd = a.cols % 4 || !aligned16(a.h) || !aligned16(a.gamma) ||
-                     !aligned16(a.grad_out) || !aligned16(a.grad_sum) || !aligned16(a.grad_h) ||
-                     !aligned16(a.part);
-    odd ? grad_any<true>(a, num_cus, s) : grad_any<false>(a, num_cus, s);
+                     !aligned16(a.grad_out) || !aligned16(a.grad_sum) || !aligned16(a.grad_h);
+    const size_t parts = grad_parts(a.rows, a.cols, num_cus);
+    odd ? grad_any<true>(a, (unsigned)parts, s) : grad_any<false>(a, (unsigned)parts, s);
+    if (a.grad_gamma)
+        lin8_grids(((size_t)a.cols + 63) / 64, [&](unsigned n, size_t done) {
+            grad_join_kernel<<<n, 1024, 0, s>>>(a, (int)parts, done);
+        });
 }
 
 }  // namespace k

@@ -151,11 +151,11 @@ void HipBackend::rms_norm_backward(const Tensor &h, const Tensor &gamma, const T
         a.grad_h = (*grad_h)->f32();
     }
     TensorNode part, stats;
-    const size_t parts = k::rms_norm_grad_parts(a.rows, a.cols, cus);
     if (grad_gamma) {
         *grad_gamma = new_tensor(gamma.shape, CLOVE_HIP_F32);
-        if (a.rows == 0 && cols) k::fill_uniform((*grad_gamma)->f32(), cols, 0, 0.0f, 0.0f, s);
-        part = new_tensor({parts * cols}, CLOVE_HIP_F32);
+        a.grad_gamma = (*grad_gamma)->f32();
+        if (a.rows == 0 && cols) k::fill_uniform(a.grad_gamma, cols, 0, 0.0f, 0.0f, s);
+        part = new_tensor({k::rms_norm_grad_floats(a.rows, a.cols, cus)}, CLOVE_HIP_F32);
         a.part = part->f32();
     }
     if (a.rows == 0 || cols == 0) return;
@@ -164,11 +164,6 @@ void HipBackend::rms_norm_backward(const Tensor &h, const Tensor &gamma, const T
         a.stats = static_cast<double *>(stats->data);
     }
     k::rms_norm_grad(a, cus, s);
-    if (grad_gamma) {
-        const size_t n = parts * cols;
-        TensorNode ws = new_tensor({k::broadcast_grad_workspace(n, cols)}, CLOVE_HIP_F32);
-        k::broadcast_grad(a.part, n, cols, false, ws->f32(), (*grad_gamma)->f32(), s);
-    }
 }
 
 void HipBackend::quantize_e4m3(const Tensor &x, int block_rows, TensorNode *codes,
