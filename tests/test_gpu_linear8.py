@@ -270,6 +270,20 @@ def test_matmul(hip, m, n, k, a_tiles, b_tiles):
     np.testing.assert_array_equal(hip.matmul_e4m3(*t).numpy(), got.numpy())
 
 
+# few rows against a long b, and results of many tiles, past every tile's edge
+@pytest.mark.parametrize("m,n,k", [(1, 8200, 300), (32, 8225, 1200), (64, 1000, 1500),
+                                   (48, 5000, 2100), (61, 16380, 700), (1930, 3970, 390),
+                                   (3841, 4000, 390)])
+@pytest.mark.parametrize("a_tiles", [False, True])
+def test_matmul_of_many(hip, m, n, k, a_tiles):
+    g = rng(m + n * 5 + k)
+    ops = operands(g, m, n, k, a_tiles, not a_tiles)
+    bias = g.standard_normal(n).astype(np.float32) if a_tiles else None
+    t = put(hip, *ops) + [None if bias is None else hip.tensor(bias)]
+    want, tol = ref.matmul(*ops, bias)
+    within(hip.matmul_e4m3(*t).numpy(), want, tol)
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 200, 700), (40, 100, 1300), (200, 300, 900),
                                    (600, 2000, 260), (130, 140, 9000)])
 def test_matmul_of_small_whole_numbers_is_exact(hip, m, n, k):
@@ -412,6 +426,45 @@ def test_refusals(hip):
     room = hip.empty((200 * 384 + 16,), np.uint8)
     moved = hip.wrap(room.device_ptr + 4, (200, 384), np.uint8)
     refused(hip.ERR_INVALID, hip.matmul_e4m3, moved, a[1], *b)
+
+
+# ---- more workgroups than one launch holds ------------------------------------------
+
+def test_many_rows(hip):
+    """Rows past 2^21 workgroups equal the same rows in a call of their own."""
+    rows = (1 << 24) + 1000
+    x = hip.empty((rows, 3)).fill_normal(1)
+    gamma = hip.tensor(np.array([0.5, 1, 2], np.float32))
+    out = hip.rms_norm(x, gamma)
+    for first in (0, (1 << 24) - 300, rows - 600):
+        part = x.read(first * 3, 1800).reshape(600, 3)
+        want = hip.rms_norm(hip.tensor(part), gamma).numpy()
+        np.testing.assert_array_equal(out.read(first * 3, 1800).reshape(600, 3), want)
+
+
+def test_many_rows_transposed(hip):
+    rows = (1 << 28) + 300
+    x = hip.empty((rows, 1)).fill_normal(2)
+    codes, exps = hip.quantize_e4m3(x, 1, False, True)
+    assert codes.shape == (1, (1 << 28) + 384) and exps.shape == (1, (1 << 21) + 3)
+    for first in (0, (1 << 28) - 256, 1 << 28):
+        part = x.read(first, min(512, rows - first)).reshape(1, -1)
+        c, e = ref.quantize(part)
+        np.testing.assert_array_equal(exps.read(first // 128, e.size), e[0])
+        ref.same_codes(codes.read(first, c.size), c[0])
+
+
+def test_a_row_of_many_columns(hip):
+    cols = (1 << 27) + 70
+    h = hip.empty((1, cols)).fill_uniform(3, 1.0, 1.0)
+    gy, gamma = hip.empty((1, cols)).fill_normal(4), hip.empty((cols,)).fill_normal(5)
+    r = np.float32(1 / np.sqrt(1 + np.float64(np.float32(1e-5))))
+    dg = hip.rms_norm_backward(h, gamma, gy)[1]
+    out = hip.rms_norm(h, gamma)
+    for first in (0, cols - 200):
+        np.testing.assert_array_equal(dg.read(first, 200), gy.read(first, 200) * r)
+        want = gamma.read(first, 200) / np.sqrt(1 + np.float64(np.float32(1e-5)))
+        within(out.read(first, 200), want, ref.rms_norm_bound(want))
 
 
 # ---- together --------------------------------------------------------------------
