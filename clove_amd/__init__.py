@@ -248,9 +248,9 @@ class Tensor:
         return self._h
 
     def free(self) -> None:
-        if self._h and self._h.value and _lib is not None:
-            _lib.clove_hip_tensor_free(self._h)
-        self._h = C.c_void_p(None)
+        h, self._h = self._h, None
+        if h and _lib is not None:
+            _lib.clove_hip_tensor_free(h)
 
     def __del__(self):
         try:

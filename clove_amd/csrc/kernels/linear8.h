@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "launch.hpp"
 #include "wave.h"
@@ -30,6 +31,19 @@ __device__ __forceinline__ unsigned lin8_mag(float x) {
     return u < 0x7f800000u ? u : 0u;
 }
 
+// Most waves hold nothing past 448 * 2^119, no infinity and no NaN.  There |x|'s
+// bits are lin8_mag and a code needs no clamp (PLAIN): rows of [2050, 3000] both ways
+// 12.3 us, 13.7 where every element takes the longer way.
+constexpr unsigned kLin8Plain = 0x7f600000u;
+__device__ __forceinline__ unsigned lin8_bits(float x) {
+    return __float_as_uint(x) & 0x7fffffffu;
+}
+__device__ __forceinline__ unsigned lin8_bits4(cl_f4 x) {
+    return max(max(lin8_bits(x.x), lin8_bits(x.y)), max(lin8_bits(x.z), lin8_bits(x.w)));
+}
+// Whether that holds for the whole wave, `bits` being the largest of a lane's.
+__device__ __forceinline__ bool lin8_plain(unsigned bits) { return __all(bits <= kLin8Plain); }
+
 // The smallest e in [-100, 119] with amax <= 448 * 2^e, amax >= 0 given by its
 // bits.  448 = 1.75 * 2^8, so the fraction decides between exponent - 8 and - 7.
 __device__ __forceinline__ int lin8_exp_of(unsigned amax) {
@@ -44,13 +58,18 @@ __device__ __forceinline__ float lin8_scaled(float x, float inv) {
 }
 
 // Four elements as four codes, rounded to nearest, ties to even.
+template <bool PLAIN>
 __device__ __forceinline__ unsigned lin8_encode4(cl_f4 x, float inv) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(lin8_scaled(x.x, inv), lin8_scaled(x.y, inv), 0, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(lin8_scaled(x.z, inv), lin8_scaled(x.w, inv), w, true);
-    return (unsigned)w;
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = PLAIN ? x[i] * inv : lin8_scaled(x[i], inv);
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true);
 }
 
+template <bool PLAIN>
 __device__ __forceinline__ unsigned lin8_mag4(cl_f4 x) {
+    if constexpr (PLAIN) return lin8_bits4(x);
     return max(max(lin8_mag(x.x), lin8_mag(x.y)), max(lin8_mag(x.z), lin8_mag(x.w)));
 }
 

@@ -74,10 +74,15 @@ __device__ __forceinline__ void emit(const RmsNormArgs &a, size_t row, int c, cl
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (4 * c + i >= a.cols) y[i] = 0.0f;
-        const int e = lin8_exp_of(half_umax(lin8_mag4(y)));
-        if (4 * c >= kp) return;
-        reinterpret_cast<unsigned *>(a.codes + row * kp)[c] = lin8_encode4(y, lin8_pow2(-e));
-        if ((c & 31) == 0) a.exps[row * (kp / 128) + c / 32] = e;
+        const auto write = [&](auto plain) {
+            constexpr bool P = decltype(plain)::value;
+            const int e = lin8_exp_of(half_umax(lin8_mag4<P>(y)));
+            if (4 * c >= kp) return;
+            reinterpret_cast<unsigned *>(a.codes + row * kp)[c] =
+                lin8_encode4<P>(y, lin8_pow2(-e));
+            if ((c & 31) == 0) a.exps[row * (kp / 128) + c / 32] = e;
+        };
+        lin8_plain(lin8_bits4(y)) ? write(std::true_type()) : write(std::false_type());
     } else {
         lin8_store4<ODD>(a.out + row * a.cols, c, a.cols, y);
     }

@@ -44,11 +44,18 @@ __global__ void __launch_bounds__(T) quantize_kernel(Quant8Args a, size_t col_ti
     // other threads' maxima arrive
     int e_tile = 0;
     lin8_u4 top = {0, 0, 0, 0};
-    if (TILES || a.codes_t)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) top[c] = max(top[c], lin8_bits(x[i][c]));
+    const bool plain = lin8_plain(max(max(top[0], top[1]), max(top[2], top[3])));
+    if (!plain) {
+        top = (lin8_u4){0, 0, 0, 0};
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int i = 0; i < RPT; ++i) top[c] = max(top[c], lin8_mag(x[i][c]));
+    }
     if constexpr (TILES) {
         unsigned all = half_umax(max(max(top[0], top[1]), max(top[2], top[3])));
         if (l == 0) tops[group][0] = all;
@@ -58,20 +65,22 @@ __global__ void __launch_bounds__(T) quantize_kernel(Quant8Args a, size_t col_ti
         e_tile = lin8_exp_of(all);
         if (t == 0 && a.codes) a.exps[row0 / 128 * (kp / 128) + col0 / 128] = e_tile;
         if (t == 0 && a.codes_t) a.exps_t[col0 / 128 * (rp / 128) + row0 / 128] = e_tile;
-    } else if (a.codes_t) {
+    } else {
         *reinterpret_cast<lin8_u4 *>(&tops[group][4 * l]) = top;
     }
-    if (a.codes) {
+    const auto straight = [&](auto p) {
+        constexpr bool P = decltype(p)::value;
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
             const int r = group * RPT + i;
-            const int e = TILES ? e_tile : lin8_exp_of(half_umax(lin8_mag4(x[i])));
+            const int e = TILES ? e_tile : lin8_exp_of(half_umax(lin8_mag4<P>(x[i])));
             if (r >= rows) continue;
             reinterpret_cast<unsigned *>(a.codes + (row0 + r) * kp + col0)[l] =
-                lin8_encode4(x[i], lin8_pow2(-e));
+                lin8_encode4<P>(x[i], lin8_pow2(-e));
             if (!TILES && l == 0) a.exps[(row0 + r) * (kp / 128) + col0 / 128] = e;
         }
-    }
+    };
+    if (a.codes) plain ? straight(std::true_type()) : straight(std::false_type());
     if (!a.codes_t) return;
     int e[4] = {e_tile, e_tile, e_tile, e_tile};
     if constexpr (!TILES) {
@@ -89,18 +98,22 @@ __global__ void __launch_bounds__(T) quantize_kernel(Quant8Args a, size_t col_ti
                 a.exps_t[(col0 + 4 * l + c) * (rp / 128) + row0 / 128] = e[c];
         }
     }
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const float inv = lin8_pow2(-e[c]);
+    const auto transposed = [&](auto p) {
         typedef unsigned piece __attribute__((ext_vector_type(WORDS)));
-        piece w;
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i)
-            w[i] = lin8_encode4((cl_f4){x[4 * i][c], x[4 * i + 1][c], x[4 * i + 2][c],
-                                        x[4 * i + 3][c]}, inv);
-        const int word = group * WORDS;  // of the column's 32
-        *reinterpret_cast<piece *>(&codes_t[4 * l + c][(word / 4 ^ (l & 7)) * 4 + word % 4]) = w;
-    }
+        for (int c = 0; c < 4; ++c) {
+            const float inv = lin8_pow2(-e[c]);
+            piece w;
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i)
+                w[i] = lin8_encode4<decltype(p)::value>(
+                    (cl_f4){x[4 * i][c], x[4 * i + 1][c], x[4 * i + 2][c], x[4 * i + 3][c]}, inv);
+            const int word = group * WORDS;  // of the column's 32
+            *reinterpret_cast<piece *>(&codes_t[4 * l + c][(word / 4 ^ (l & 7)) * 4 + word % 4]) =
+                w;
+        }
+    };
+    plain ? transposed(std::true_type()) : transposed(std::false_type());
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 1024 / T; ++i) {
@@ -134,11 +147,16 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(Quant8Args a, size_t
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-        const int e = lin8_exp_of(half_umax(lin8_mag4(x[u])));
-        if (row[u] >= a.rows || block[u] >= kb) continue;
-        const size_t i = row[u] * kb + block[u];
-        reinterpret_cast<unsigned *>(a.codes + i * 128)[l] = lin8_encode4(x[u], lin8_pow2(-e));
-        if (l == 0) a.exps[i] = e;
+        const auto write = [&](auto p) {
+            constexpr bool P = decltype(p)::value;
+            const int e = lin8_exp_of(half_umax(lin8_mag4<P>(x[u])));
+            if (row[u] >= a.rows || block[u] >= kb) return;
+            const size_t i = row[u] * kb + block[u];
+            reinterpret_cast<unsigned *>(a.codes + i * 128)[l] =
+                lin8_encode4<P>(x[u], lin8_pow2(-e));
+            if (l == 0) a.exps[i] = e;
+        };
+        lin8_plain(lin8_bits4(x[u])) ? write(std::true_type()) : write(std::false_type());
     }
 }
 
