@@ -285,26 +285,32 @@ __global__ void __launch_bounds__(T) grad_kernel(RmsNormGradArgs a) {
             *reinterpret_cast<cl_f4 *>(a.part + blockIdx.x * pitch + 4 * (t + TR * i)) = acc[i];
 }
 
-// grad_gamma: the rows of `part` added up, 64 columns to a workgroup, 64 threads
-// to four of them, every 64th row each and then in their order.
+// grad_gamma: the rows of `part` added up, 32 columns to a workgroup, every 128th
+// row to a thread and then those in halves, in one order: 2.7 us for 256 rows of
+// 2049, 3.0 for 512 (with 64 columns 2.8 and 3.3, with 16 2.8 and 3.6).
 __global__ void __launch_bounds__(1024) grad_join_kernel(RmsNormGradArgs a, int parts,
                                                           size_t done) {
-    __shared__ cl_f4 sums[64][16];
+    __shared__ cl_f4 sums[128][8];
     const size_t pitch = part_pitch(a.cols);
-    const int q = threadIdx.x & 15, group = threadIdx.x >> 4;
-    const size_t col0 = (done + blockIdx.x) * 64, at = col0 + 4 * q;
+    const int q = threadIdx.x & 7, group = threadIdx.x >> 3;
+    const size_t col0 = (done + blockIdx.x) * 32, at = col0 + 4 * q;
     cl_f4 s = {0.f, 0.f, 0.f, 0.f};
     if (at < pitch)
-#pragma unroll 8
-        for (int p = group; p < parts; p += 64)
+#pragma unroll 4
+        for (int p = group; p < parts; p += 128)
             s += *reinterpret_cast<const cl_f4 *>(a.part + p * pitch + at);
     sums[group][q] = s;
     __syncthreads();
-    if (threadIdx.x >= 64) return;
+#pragma unroll
+    for (int w = 64; w >= 16; w /= 2) {
+        if (group < w) sums[group][q] += sums[group + w][q];
+        __syncthreads();
+    }
+    if (threadIdx.x >= 32) return;
     const size_t col = col0 + threadIdx.x;
     float total = 0.0f;
-#pragma unroll 16
-    for (int g = 0; g < 64; ++g) total += sums[g][threadIdx.x / 4][threadIdx.x % 4];
+#pragma unroll
+    for (int g = 0; g < 16; ++g) total += sums[g][threadIdx.x / 4][threadIdx.x % 4];
     if (col < (size_t)a.cols) a.grad_gamma[col] = total;
 }
 
@@ -346,31 +352,39 @@ __global__ void __launch_bounds__(256) grad_apply_kernel(RmsNormGradArgs a, unsi
         *reinterpret_cast<cl_f4 *>(a.part + share * pitch + 4 * (size_t)c) = acc;
 }
 
-// Rows that a workgroup of grad_kernel takes at once.
-size_t grad_rows(int cols) { return cols <= 128 ? 8 : cols <= 1024 ? 4 : 1; }
-// Workgroups, and rows of `part`.  With a row on its way one a CU keeps the memory
-// busy where there are many rows of full registers ([8192, 4096] 101 us, 104 with
-// four, whose join takes 2.6 us more; without the row ahead 179 and 104); fewer or
-// shorter rows need two, narrow ones four ([32768, 200] 29 us with one, 18 with four).
+// Rows that a workgroup of grad_kernel takes at once, and workgroups, each a row of
+// `part`.  With the next row on its way one workgroup a CU keeps the memory busy, and
+// one that takes several rows leaves the join fewer to add: [1001, 2049] 12.6 us with
+// two rows in 512 threads, 13.3 with one in twice the workgroups; [32768, 200] 23 with
+// sixteen, 25 with four; [1554, 768] 8.0 with eight, 8.8 with four.  Many rows of full
+// registers keep one ([8192, 4096] 102 us, 104 with two), and so do those of up to 2048
+// columns, in two workgroups a CU ([4000, 1500] 23.6, 24.5).
+size_t grad_rows(size_t rows, int cols, int num_cus) {
+    return cols <= 128    ? 32
+           : cols <= 256  ? 16
+           : cols <= 1024 ? 8
+           : cols > 2048 && cols <= 4096 && rows < 16 * (size_t)num_cus ? 2
+                                                                        : 1;
+}
 size_t grad_parts(size_t rows, int cols, int num_cus) {
     const size_t cus = (size_t)num_cus;
     if (cols > kWideGrad) {  // so many shares for each group of 1024 columns
         const size_t groups = ((size_t)cols + 1023) / 1024;
         return std::min(rows, std::max(cus * 4 / groups, (size_t)1));
     }
-    const size_t per = grad_rows(cols);
-    const bool one = cols > 4096 || (cols > 2048 && rows >= 16 * cus);
-    return std::min((rows + per - 1) / per, cus * (one ? 1 : cols > 256 ? 2 : 4));
+    const size_t per = grad_rows(rows, cols, num_cus);
+    return std::min((rows + per - 1) / per, cols > 1024 && cols <= 2048 ? 2 * cus : cus);
 }
 
 template <bool ODD>
-void grad_any(const RmsNormGradArgs &a, unsigned n, hipStream_t s) {
+void grad_any(const RmsNormGradArgs &a, size_t per, unsigned n, hipStream_t s) {
     const auto go = [&](auto kernel, int t) { kernel<<<n, t, 0, s>>>(a); };
-    if (a.cols <= 128) return go(grad_kernel<256, 32, 1, ODD>, 256);
-    if (a.cols <= 256) return go(grad_kernel<256, 64, 1, ODD>, 256);
-    if (a.cols <= 512) return go(grad_kernel<256, 64, 2, ODD>, 256);
-    if (a.cols <= 1024) return go(grad_kernel<256, 64, 4, ODD>, 256);
+    if (a.cols <= 128) return go(grad_kernel<1024, 32, 1, ODD>, 1024);
+    if (a.cols <= 256) return go(grad_kernel<1024, 64, 1, ODD>, 1024);
+    if (a.cols <= 512) return go(grad_kernel<512, 64, 2, ODD>, 512);
+    if (a.cols <= 1024) return go(grad_kernel<512, 64, 4, ODD>, 512);
     if (a.cols <= 2048) return go(grad_kernel<256, 256, 2, ODD>, 256);
+    if (a.cols <= 4096 && per == 2) return go(grad_kernel<512, 256, 4, ODD>, 512);
     if (a.cols <= 4096) return go(grad_kernel<256, 256, 4, ODD>, 256);
     if (a.cols <= kWideGrad) return go(grad_kernel<512, 512, 4, ODD>, 512);
     lin8_grids(a.rows, [&](unsigned g, size_t done) {
@@ -403,10 +417,11 @@ void rms_norm_grad(const RmsNormGradArgs &a, int num_cus, hipStream_t s) {
     if (a.rows == 0 || a.cols == 0) return;
     const bool odd = a.cols % 4 || !aligned16(a.h) || !aligned16(a.gamma) ||
                      !aligned16(a.grad_out) || !aligned16(a.grad_sum) || !aligned16(a.grad_h);
-    const size_t parts = grad_parts(a.rows, a.cols, num_cus);
-    odd ? grad_any<true>(a, (unsigned)parts, s) : grad_any<false>(a, (unsigned)parts, s);
+    const size_t per = grad_rows(a.rows, a.cols, num_cus);
+    const unsigned parts = (unsigned)grad_parts(a.rows, a.cols, num_cus);
+    odd ? grad_any<true>(a, per, parts, s) : grad_any<false>(a, per, parts, s);
     if (a.grad_gamma)
-        lin8_grids(((size_t)a.cols + 63) / 64, [&](unsigned n, size_t done) {
+        lin8_grids(((size_t)a.cols + 31) / 32, [&](unsigned n, size_t done) {
             grad_join_kernel<<<n, 1024, 0, s>>>(a, (int)parts, done);
         });
 }

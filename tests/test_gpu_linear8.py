@@ -167,7 +167,9 @@ def test_rms_norm_extremes(hip):
 
 @pytest.mark.parametrize("stream", [False, True])
 @pytest.mark.parametrize("rows,cols", SHAPES + [(700, 64), (3000, 33), (1100, 1028), (600, 4100),
-                                                (1030, 9000)])
+                                                (1030, 9000), (20000, 33), (9000, 130),
+                                                (5000, 513), (5000, 700), (1000, 3001),
+                                                (4100, 2052)])
 def test_rms_norm_backward(hip, rows, cols, stream):
     g = rng(rows * 13 + cols)
     h = states(g, rows, cols)
