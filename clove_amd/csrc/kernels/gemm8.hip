@@ -248,6 +248,10 @@ __global__ void __launch_bounds__(BM / 64 * (BN / 64) * KG * 64)
 #pragma unroll
     for (int j = 0; j < JB; ++j)
         bias[j] = g.bias && p.splits == 1 && col0 + 32 * j < g.n ? g.bias[col0 + 32 * j] : 0.0f;
+    // (the loads are waited for here: behind a branch they are taken to be on their way
+    // still, and every store would wait for the store before it)
+#pragma unroll
+    for (int j = 0; j < JB; ++j) asm volatile("" : "+v"(bias[j]));
     const auto store = [&](auto whole) {
 #pragma unroll
         for (int o = 0; o < KG; ++o)
@@ -288,9 +292,14 @@ __global__ void __launch_bounds__(256) join_kernel(Gemm8Args g, int splits) {
 #pragma unroll
             for (int j = 1; j < kMaxSplits; ++j)
                 if (j < splits) s += v[j];
-            if (g.bias)
+            if (g.bias) {
+                int col = (int)(i % (size_t)g.n);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[e] += g.bias[(i + e) % g.n];
+                for (int e = 0; e < 4; ++e) {
+                    s[e] += g.bias[col];
+                    if (++col == g.n) col = 0;
+                }
+            }
             *reinterpret_cast<lin8_f4u *>(g.out + i) = s;
         } else {
             for (size_t e = i; e < n; ++e) {
@@ -425,11 +434,8 @@ __global__ void __launch_bounds__(64 * W) stream_kernel(Gemm8Args g) {
 #pragma unroll
         for (int w = 1; w < W; ++w) s += sums[(w * IB * JB * 4 + u) * 64 + lane];
         const int m = u / 4 % JB * 32 + l32, n = n0 + u / 4 / JB * 32 + 8 * (u % 4) + 4 * h;
-        if (m >= g.m) continue;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (n + e < g.n)
-                g.out[(size_t)m * g.n + n + e] = s[e] + (g.bias ? g.bias[n + e] : 0.0f);
+        if (g.bias) s += lin8_load4<true>(g.bias, n / 4, g.n);
+        if (m < g.m) lin8_store4<true>(g.out + (size_t)m * g.n, n / 4, g.n, s);
     }
 }
 

@@ -19,6 +19,38 @@ namespace {
 
 typedef unsigned lin8_u4 __attribute__((ext_vector_type(4)));
 
+// Columns 4l .. 4l + 3 of rows r0 .. r0 + RPT - 1 of a tile of `rows` x `left`, zeros
+// past its edges, where the addresses stay within it: with loads behind branches the
+// compiler waits for some before it sends the next.
+template <int RPT, bool ODD>
+__device__ __forceinline__ void load_tile(const float *src, size_t cols, int l, int left, int r0,
+                                          int rows, cl_f4 *x) {
+    if (rows == 128 && left == 128) {
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            const float *p = src + (size_t)(r0 + i) * cols + 4 * l;
+            x[i] = ODD ? (cl_f4)*reinterpret_cast<const lin8_f4u *>(p)
+                       : *reinterpret_cast<const cl_f4 *>(p);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        const float *p = src + (size_t)min(r0 + i, rows - 1) * cols;
+        if constexpr (ODD) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[i][c] = p[min(4 * l + c, left - 1)];
+        } else {
+            x[i] = *reinterpret_cast<const cl_f4 *>(p + min(4 * l, left - 4));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RPT; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (r0 + i >= rows || 4 * l + c >= left) x[i][c] = 0.0f;
+}
+
 template <int T, bool ODD, bool TILES>
 __global__ void __launch_bounds__(T) quantize_kernel(Quant8Args a, size_t col_tiles,
                                                      size_t done) {
@@ -33,13 +65,7 @@ __global__ void __launch_bounds__(T) quantize_kernel(Quant8Args a, size_t col_ti
     const int left = (int)min((size_t)128, a.cols - col0);       // columns of the tile
     const int rows = (int)min((size_t)128, a.rows - row0);       // and its rows
     cl_f4 x[RPT];
-    const float *src = a.x + row0 * a.cols + col0;
-#pragma unroll
-    for (int i = 0; i < RPT; ++i) {
-        const int r = group * RPT + i;
-        x[i] = (cl_f4){0.f, 0.f, 0.f, 0.f};
-        if (r < rows) x[i] = lin8_load4<ODD>(src + (size_t)r * a.cols, l, left);
-    }
+    load_tile<RPT, ODD>(a.x + row0 * a.cols + col0, a.cols, l, left, group * RPT, rows, x);
     // the maxima of this thread's columns, then its rows' codes on their way while the
     // other threads' maxima arrive
     int e_tile = 0;
