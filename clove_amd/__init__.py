@@ -252,6 +252,13 @@ class Tensor:
         if h and _lib is not None:
             _lib.clove_hip_tensor_free(h)
 
+    @classmethod
+    def _take(cls, cell: C.c_void_p) -> "Tensor":
+        """Owns the handle that an entry stored in `cell`."""
+        t = cls.__new__(cls)
+        t._h = cell
+        return t
+
     def __del__(self):
         try:
             self.free()
@@ -589,18 +596,19 @@ def rms_norm(x: Tensor, gamma: Tensor, residual: Optional[Tensor] = None, eps: f
     h = C.c_void_p()
     out = _handle(lib().clove_hip_rms_norm(x.handle, residual.handle, gamma.handle, eps,
                                            C.byref(h)))
-    return out, Tensor(h.value)
+    return out, Tensor._take(h)
 
 
 def rms_norm_e4m3(x: Tensor, gamma: Tensor, residual: Optional[Tensor] = None,
                   eps: float = 1e-5):
     """rms_norm's output in 8 bits, an exponent for each 128 elements of a row:
     (codes, exps), and h behind them with a residual."""
-    outs = [C.c_void_p() for _ in range(3)]
+    codes, exps, h = C.c_void_p(), C.c_void_p(), C.c_void_p()
     _check(lib().clove_hip_rms_norm_e4m3(x.handle, _opt(residual), gamma.handle, eps,
-                                         C.byref(outs[2]) if residual is not None else None,
-                                         C.byref(outs[0]), C.byref(outs[1])))
-    return tuple(Tensor(o.value) for o in outs[:2 if residual is None else 3])
+                                         None if residual is None else C.byref(h),
+                                         C.byref(codes), C.byref(exps)))
+    out = Tensor._take(codes), Tensor._take(exps)
+    return out if residual is None else out + (Tensor._take(h),)
 
 
 def rms_norm_backward(h: Tensor, gamma: Tensor, grad_out: Tensor,
@@ -610,7 +618,7 @@ def rms_norm_backward(h: Tensor, gamma: Tensor, grad_out: Tensor,
     gh, gg = C.c_void_p(), C.c_void_p()
     _check(lib().clove_hip_rms_norm_backward(h.handle, gamma.handle, grad_out.handle,
                                              _opt(grad_sum), eps, C.byref(gh), C.byref(gg)))
-    return Tensor(gh.value), Tensor(gg.value)
+    return Tensor._take(gh), Tensor._take(gg)
 
 
 def quantize_e4m3(x: Tensor, block_rows: int = 1, straight: bool = True,
@@ -621,7 +629,7 @@ def quantize_e4m3(x: Tensor, block_rows: int = 1, straight: bool = True,
                                                         transposed)]
     _check(lib().clove_hip_quantize_e4m3(x.handle, block_rows,
                                          *[None if o is None else C.byref(o) for o in outs]))
-    return tuple(Tensor(o.value) for o in outs if o is not None)
+    return tuple([Tensor._take(o) for o in outs if o is not None])
 
 
 def matmul_e4m3(a: Tensor, a_exps: Tensor, b: Tensor, b_exps: Tensor,

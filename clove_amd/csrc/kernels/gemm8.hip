@@ -34,10 +34,6 @@ __device__ __forceinline__ bf8 widen8(unsigned lo, unsigned hi, float scale) {
     return r.v;
 }
 
-struct Plan {
-    int bm, bn, splits, tiles_m, tiles_n, per_split;  // per_split: blocks of 128 of k
-};
-
 // Workgroups are dealt to the eight XCDs in turn, each with its own L2: workgroup L
 // takes the L / 8-th tile of its XCD's eighth of an order that goes through groups
 // of eight tile rows column by column, so that an XCD's workgroups share operands.
@@ -92,7 +88,7 @@ __device__ __forceinline__ int slot_of(int row, int k16) { return 16 * (k16 ^ (r
 // 1554 9.2 us, waves of 32 x 32 on 64 x 64 tiles 9.2-10.5.
 template <int BM, int BN, int KG, int MINW>
 __global__ void __launch_bounds__(BM / 64 * (BN / 64) * KG * 64)
-    __attribute__((amdgpu_waves_per_eu(MINW))) gemm8_kernel(Gemm8Args g, Plan p) {
+    __attribute__((amdgpu_waves_per_eu(MINW))) gemm8_kernel(Gemm8Args g, Gemm8Plan p) {
     constexpr int WG = BM / 64 * (BN / 64), NW = WG * KG;  // waves of a group, and all
     constexpr int IB = 2, JB = 2;                          // a wave's 32 x 32 blocks
     constexpr int OWN = IB * JB * 4 / KG;                  // quarter blocks that a group stores
@@ -457,7 +453,7 @@ constexpr Tiles kTiles[] = {
     {256, 256, 1, 3.0, {3.10}},
 };
 
-double tiles_us(const Gemm8Args &g, const Tiles &t, int splits, int num_cus, Plan *p) {
+double tiles_us(const Gemm8Args &g, const Tiles &t, int splits, int num_cus, Gemm8Plan *p) {
     p->bm = t.bm;
     p->bn = t.bn;
     p->tiles_m = (int)(((int64_t)g.m + t.bm - 1) / t.bm);
@@ -479,53 +475,24 @@ double tiles_us(const Gemm8Args &g, const Tiles &t, int splits, int num_cus, Pla
     return us;
 }
 
-// Waves of the streaming kernel for up to 32 or 64 rows of a; 0: none.  One
-// workgroup a CU has eight waves (six with 64 rows), more of them four, so that two
-// (for 64 rows: twice the rows of b) share a CU: 32 x 14336 x 4096 12.4 us, 15.9 with
-// eight; 32 x 4096 x 4096 6.4 us, 7.9 with four.
-struct Stream {
-    int rows_b = 0, rows_a = 0, waves = 0;
-    double us = 0;
-};
-Stream stream_of(const Gemm8Args &g, int num_cus) {
-    Stream r;
-    if (g.m > 64) return r;
+// The streaming kernel for up to 32 or 64 rows of a.  One workgroup a CU has eight
+// waves (six with 64 rows), more of them four, so that two (for 64 rows: twice the
+// rows of b) share a CU: 32 x 14336 x 4096 12.4 us, 15.9 with eight; 32 x 4096 x 4096
+// 6.4 us, 7.9 with four.
+double stream_us(const Gemm8Args &g, int num_cus, Gemm8Plan *p) {
     const bool one = ((int64_t)g.n + 31) / 32 <= num_cus;
-    r.rows_a = g.m <= 32 ? 32 : 64;
-    r.rows_b = r.rows_a == 64 && !one ? 64 : 32;
-    r.waves = !one ? 4 : r.rows_a == 32 ? 8 : 6;
-    const int per_cu = !one && r.rows_a == 32 ? 2 : 1;
-    const double step = r.rows_b == 64 ? 1.75 : r.rows_a == 64 ? 1.3 : one ? 0.95 : 1.25;
-    const double turns = std::ceil(std::ceil((double)g.n / r.rows_b) / ((double)num_cus * per_cu));
-    r.us = 2.5 + turns * ((g.blocks + r.waves - 1) / r.waves) * step;
-    return r;
-}
-
-struct Choice {
-    Stream stream;
-    Plan tiles{};
-};
-Choice choose(const Gemm8Args &g, int num_cus) {
-    Choice c;
-    const Stream s = stream_of(g, num_cus);
-    double best = 0;
-    for (const Tiles &t : kTiles)
-        for (int splits = 1; splits <= kMaxSplits; splits *= 2) {
-            Plan p{};
-            if (splits > 1 && g.blocks < 2 * splits) break;
-            const double us = tiles_us(g, t, splits, num_cus, &p);
-            if (c.tiles.bm == 0 || us < best) {
-                best = us;
-                c.tiles = p;
-            }
-        }
-    // (up to 32 rows no tiles measured faster)
-    if (s.waves && (g.m <= 32 || s.us <= best)) c.stream = s;
-    return c;
+    p->rows_a = g.m <= 32 ? 32 : 64;
+    p->rows_b = p->rows_a == 64 && !one ? 64 : 32;
+    p->waves = !one ? 4 : p->rows_a == 32 ? 8 : 6;
+    p->splits = 1;
+    const int per_cu = !one && p->rows_a == 32 ? 2 : 1;
+    const double step = p->rows_b == 64 ? 1.75 : p->rows_a == 64 ? 1.3 : one ? 0.95 : 1.25;
+    const double turns = std::ceil(std::ceil((double)g.n / p->rows_b) / ((double)num_cus * per_cu));
+    return 2.5 + turns * ((g.blocks + p->waves - 1) / p->waves) * step;
 }
 
 template <int BM, int BN, int KG, int MINW>
-void run_tiles(const Gemm8Args &g, const Plan &p, hipStream_t s) {
+void run_tiles(const Gemm8Args &g, const Gemm8Plan &p, hipStream_t s) {
     const dim3 grid((unsigned)((p.tiles_m * p.tiles_n + 7) / 8 * 8), (unsigned)p.splits);
     gemm8_kernel<BM, BN, KG, MINW><<<grid, BM / 64 * (BN / 64) * KG * 64, 0, s>>>(g, p);
 }
@@ -537,21 +504,35 @@ void run_stream(const Gemm8Args &g, hipStream_t s) {
 
 }  // namespace
 
-size_t gemm8_workspace(const Gemm8Args &a, int num_cus) {
-    if (a.m == 0 || a.n == 0) return 0;
-    const Choice c = choose(a, num_cus);
-    return !c.stream.waves && c.tiles.splits > 1 ? (size_t)c.tiles.splits * a.m * a.n : 0;
+Gemm8Plan gemm8_plan(const Gemm8Args &g, int num_cus) {
+    Gemm8Plan best{};
+    if (g.m == 0 || g.n == 0) return best;
+    double best_us = g.m <= 64 ? stream_us(g, num_cus, &best) : 0.0;
+    if (g.m <= 32) return best;  // (no tiles measured faster)
+    for (const Tiles &t : kTiles)
+        for (int splits = 1; splits <= kMaxSplits; splits *= 2) {
+            if (splits > 1 && g.blocks < 2 * splits) break;
+            Gemm8Plan p{};
+            const double us = tiles_us(g, t, splits, num_cus, &p);
+            if (best.splits == 0 || us < best_us) {
+                best_us = us;
+                best = p;
+            }
+        }
+    return best;
 }
 
-void gemm8(const Gemm8Args &a, int num_cus, hipStream_t s) {
+size_t gemm8_workspace(const Gemm8Args &a, const Gemm8Plan &p) {
+    return p.splits > 1 ? (size_t)p.splits * a.m * a.n : 0;
+}
+
+void gemm8(const Gemm8Args &a, const Gemm8Plan &p, int num_cus, hipStream_t s) {
     if (a.m == 0 || a.n == 0) return;
-    const Choice c = choose(a, num_cus);
-    if (const Stream &r = c.stream; r.waves) {
-        if (r.rows_a == 32) r.waves == 8 ? run_stream<32, 32, 8>(a, s) : run_stream<32, 32, 4>(a, s);
-        else r.rows_b == 32 ? run_stream<32, 64, 6>(a, s) : run_stream<64, 64, 4>(a, s);
+    if (p.waves) {
+        if (p.rows_a == 32) p.waves == 8 ? run_stream<32, 32, 8>(a, s) : run_stream<32, 32, 4>(a, s);
+        else p.rows_b == 32 ? run_stream<32, 64, 6>(a, s) : run_stream<64, 64, 4>(a, s);
         return;
     }
-    const Plan &p = c.tiles;
     if (p.bm == 256) run_tiles<256, 256, 1, 4>(a, p, s);
     else if (p.bm == 128) run_tiles<128, 128, 2, 2>(a, p, s);
     else if (p.bn == 128) run_tiles<64, 128, 2, 2>(a, p, s);

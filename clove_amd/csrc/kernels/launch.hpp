@@ -335,8 +335,16 @@ struct Gemm8Args {
     int m, n, blocks;   // blocks of 128 along k
     bool a_tiles, b_tiles;
 };
-size_t gemm8_workspace(const Gemm8Args &a, int num_cus);
-void gemm8(const Gemm8Args &a, int num_cus, hipStream_t s);
+// How a product is cut: with waves, the streaming kernel with rows_a rows of a and
+// rows_b of b to a workgroup of so many; else bm x bn tiles, `splits` along k of
+// per_split blocks each.
+struct Gemm8Plan {
+    int waves, rows_a, rows_b;
+    int bm, bn, tiles_m, tiles_n, splits, per_split;
+};
+Gemm8Plan gemm8_plan(const Gemm8Args &a, int num_cus);
+size_t gemm8_workspace(const Gemm8Args &a, const Gemm8Plan &p);
+void gemm8(const Gemm8Args &a, const Gemm8Plan &p, int num_cus, hipStream_t s);
 
 }  // namespace k
 }  // namespace clove

@@ -221,12 +221,13 @@ TensorNode HipBackend::matmul_e4m3(const Tensor &a, const Tensor &a_exps, const 
     g.n = (int)n;
     g.blocks = (int)ka;
     const int cus = ctx().num_cus;
+    const k::Gemm8Plan plan = k::gemm8_plan(g, cus);
     TensorNode ws;
-    if (const size_t floats = k::gemm8_workspace(g, cus)) {
+    if (const size_t floats = k::gemm8_workspace(g, plan)) {
         ws = new_tensor({floats}, CLOVE_HIP_F32);
         g.ws = ws->f32();
     }
-    k::gemm8(g, cus, ctx().stream);
+    k::gemm8(g, plan, cus, ctx().stream);
     return out;
 }
 
