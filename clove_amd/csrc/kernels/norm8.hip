@@ -314,8 +314,9 @@ __global__ void __launch_bounds__(1024) grad_join_kernel(RmsNormGradArgs a, int 
     if (col < (size_t)a.cols) a.grad_gamma[col] = total;
 }
 
-// Rows that registers do not hold (sixteen columns a thread and four arrays of them
-// leave 1024 threads no room): the sums first...
+// Rows that registers do not hold: the sums first ([2000, 16384] 134 us; 118 in one
+// pass of 512 threads that spill, which takes 140 where these take 124 for [3000, 9001]
+// and 33 where they take 27 for [300, 16380])...
 constexpr int kWideGrad = 8192;
 template <bool ODD>
 __global__ void __launch_bounds__(1024) grad_stats_kernel(RmsNormGradArgs a, size_t row0) {
@@ -356,8 +357,8 @@ __global__ void __launch_bounds__(256) grad_apply_kernel(RmsNormGradArgs a, unsi
 // `part`.  With the next row on its way one workgroup a CU keeps the memory busy, and
 // one that takes several rows leaves the join fewer to add: [1001, 2049] 12.6 us with
 // two rows in 512 threads, 13.3 with one in twice the workgroups; [32768, 200] 23 with
-// sixteen, 25 with four; [1554, 768] 8.0 with eight, 8.8 with four.  Many rows of full
-// registers keep one ([8192, 4096] 102 us, 104 with two), and so do those of up to 2048
+// sixteen, 25 with four; [1554, 768] 8.0 with eight, 8.8 with four.  Many long rows go
+// one by one ([8192, 4096] 101 us, 104 with two), and so do those of up to 2048
 // columns, in two workgroups a CU ([4000, 1500] 23.6, 24.5).
 size_t grad_rows(size_t rows, int cols, int num_cus) {
     return cols <= 128    ? 32
@@ -385,7 +386,7 @@ void grad_any(const RmsNormGradArgs &a, size_t per, unsigned n, hipStream_t s) {
     if (a.cols <= 1024) return go(grad_kernel<512, 64, 4, ODD>, 512);
     if (a.cols <= 2048) return go(grad_kernel<256, 256, 2, ODD>, 256);
     if (a.cols <= 4096 && per == 2) return go(grad_kernel<512, 256, 4, ODD>, 512);
-    if (a.cols <= 4096) return go(grad_kernel<256, 256, 4, ODD>, 256);
+    if (a.cols <= 4096) return go(grad_kernel<512, 512, 2, ODD>, 512);
     if (a.cols <= kWideGrad) return go(grad_kernel<512, 512, 4, ODD>, 512);
     lin8_grids(a.rows, [&](unsigned g, size_t done) {
         grad_stats_kernel<ODD><<<g, 1024, 0, s>>>(a, done);
