@@ -302,7 +302,7 @@ void rms_norm(const RmsNormArgs &a, hipStream_t s);
 struct RmsNormGradArgs {
     const float *h, *gamma, *grad_out, *grad_sum;  // grad_sum may be null
     float *grad_h, *grad_gamma;                    // either may be null
-    float *part;    // rms_norm_grad_floats() floats, null without grad_gamma
+    float *part;    // rms_norm_grad_floats() floats, null for 0 or without grad_gamma
     double *stats;  // rms_norm_grad_stats() doubles
     size_t rows;
     int cols;

@@ -208,9 +208,14 @@ __device__ __forceinline__ void grad_chunk(const RmsNormGradArgs &a, size_t row,
     if (a.grad_h) lin8_store4<ODD>(a.grad_h + row * a.cols, c, a.cols, dh);
 }
 
-// Floats of a row of `part`: whole vectors, zeros behind the columns.
+// Floats of a row of `part`: whole vectors.
 __host__ __device__ __forceinline__ size_t part_pitch(int cols) {
     return ((size_t)cols + 3) / 4 * 4;
+}
+// Where the sums of a share of the rows go: a row of `part`, the gradient itself if
+// there is one share, null if it is not wanted.
+__device__ __forceinline__ float *gamma_sums(const RmsNormGradArgs &a, size_t share) {
+    return a.part ? a.part + share * part_pitch(a.cols) : a.grad_gamma;
 }
 
 // TR threads a row.  A workgroup walks the rows from blockIdx.x * T / TR on, the
@@ -266,7 +271,8 @@ __global__ void __launch_bounds__(T) grad_kernel(RmsNormGradArgs a) {
         work(row0 + mine, 1);
         if ((row0 += step) >= a.rows) break;
     }
-    if (!a.part) return;
+    float *const out = gamma_sums(a, blockIdx.x);
+    if (!out) return;
     if constexpr (PER > 1) {
         if (mine)
 #pragma unroll
@@ -278,11 +284,8 @@ __global__ void __launch_bounds__(T) grad_kernel(RmsNormGradArgs a) {
 #pragma unroll
             for (int w = 1; w < PER; ++w) acc[i] += sums[w - 1][t + TR * i];
     }
-    const size_t pitch = part_pitch(a.cols);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (4 * (size_t)(t + TR * i) < pitch)
-            *reinterpret_cast<cl_f4 *>(a.part + blockIdx.x * pitch + 4 * (t + TR * i)) = acc[i];
+    for (int i = 0; i < NV; ++i) lin8_store4<ODD>(out, t + TR * i, a.cols, acc[i]);
 }
 
 // grad_gamma: the rows of `part` added up, 32 columns to a workgroup, every 128th
@@ -348,9 +351,7 @@ __global__ void __launch_bounds__(256) grad_apply_kernel(RmsNormGradArgs a, unsi
             lin8_load4<ODD>(a.grad_sum + row * a.cols, c, a.grad_sum ? a.cols : 0);
         grad_chunk<ODD>(a, row, c, h, gy, ds, gamma, a.stats[2 * row], a.stats[2 * row + 1], &acc);
     }
-    const size_t pitch = part_pitch(a.cols);
-    if (a.part && 4 * (size_t)c < pitch)
-        *reinterpret_cast<cl_f4 *>(a.part + share * pitch + 4 * (size_t)c) = acc;
+    if (float *out = gamma_sums(a, share)) lin8_store4<ODD>(out, c, a.cols, acc);
 }
 
 // Rows that a workgroup of grad_kernel takes at once, and workgroups, each a row of
@@ -368,12 +369,14 @@ size_t grad_rows(size_t rows, int cols, int num_cus) {
                                                                         : 1;
 }
 size_t grad_parts(size_t rows, int cols, int num_cus) {
-    const size_t cus = (size_t)num_cus;
+    const size_t cus = (size_t)num_cus, per = grad_rows(rows, cols, num_cus);
+    // few rows are one share, with no join: [20, 100] and [3, 1500] 4.8 us a call for
+    // 7.8, but with four turns of the workgroup [31, 1000] 9.2 and [8, 4000] 10.4
+    if (rows <= 2 * per) return 1;
     if (cols > kWideGrad) {  // so many shares for each group of 1024 columns
         const size_t groups = ((size_t)cols + 1023) / 1024;
         return std::min(rows, std::max(cus * 4 / groups, (size_t)1));
     }
-    const size_t per = grad_rows(rows, cols, num_cus);
     return std::min((rows + per - 1) / per, cols > 1024 && cols <= 2048 ? 2 * cus : cus);
 }
 
@@ -410,7 +413,8 @@ void rms_norm(const RmsNormArgs &a, hipStream_t s) {
 }
 
 size_t rms_norm_grad_floats(size_t rows, int cols, int num_cus) {
-    return grad_parts(rows, cols, num_cus) * part_pitch(cols);
+    const size_t parts = grad_parts(rows, cols, num_cus);
+    return parts > 1 ? parts * part_pitch(cols) : 0;
 }
 size_t rms_norm_grad_stats(size_t rows, int cols) { return cols > kWideGrad ? 2 * rows : 0; }
 
@@ -421,7 +425,7 @@ void rms_norm_grad(const RmsNormGradArgs &a, int num_cus, hipStream_t s) {
     const size_t per = grad_rows(a.rows, a.cols, num_cus);
     const unsigned parts = (unsigned)grad_parts(a.rows, a.cols, num_cus);
     odd ? grad_any<true>(a, per, parts, s) : grad_any<false>(a, per, parts, s);
-    if (a.grad_gamma)
+    if (a.part)
         lin8_grids(((size_t)a.cols + 31) / 32, [&](unsigned n, size_t done) {
             grad_join_kernel<<<n, 1024, 0, s>>>(a, (int)parts, done);
         });

@@ -155,8 +155,10 @@ void HipBackend::rms_norm_backward(const Tensor &h, const Tensor &gamma, const T
         *grad_gamma = new_tensor(gamma.shape, CLOVE_HIP_F32);
         a.grad_gamma = (*grad_gamma)->f32();
         if (a.rows == 0 && cols) k::fill_uniform(a.grad_gamma, cols, 0, 0.0f, 0.0f, s);
-        part = new_tensor({k::rms_norm_grad_floats(a.rows, a.cols, cus)}, CLOVE_HIP_F32);
-        a.part = part->f32();
+        if (const size_t n = k::rms_norm_grad_floats(a.rows, a.cols, cus)) {
+            part = new_tensor({n}, CLOVE_HIP_F32);
+            a.part = part->f32();
+        }
     }
     if (a.rows == 0 || cols == 0) return;
     if (const size_t n = k::rms_norm_grad_stats(a.rows, a.cols)) {

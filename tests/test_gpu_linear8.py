@@ -169,6 +169,7 @@ def test_rms_norm_extremes(hip):
 @pytest.mark.parametrize("rows,cols", SHAPES + [(700, 64), (3000, 33), (1100, 1028), (600, 4100),
                                                 (1030, 9000), (20000, 33), (9000, 130),
                                                 (5000, 513), (5000, 700), (1000, 3001),
+                                                (64, 100), (65, 100), (17, 800), (2, 3000),
                                                 (4100, 2052)])
 def test_rms_norm_backward(hip, rows, cols, stream):
     g = rng(rows * 13 + cols)
