@@ -310,16 +310,21 @@ __global__ void __launch_bounds__(256) join_kernel(Gemm8Args g, int splits) {
 // Up to MB rows of a: a workgroup of W waves takes RB rows of b and the waves share
 // out the blocks of k (w, w + W, ...).  Each streams its blocks of both operands
 // through two stages of its own in LDS, by DMA of whole 128-byte lines,
-// so no wave waits for another until their sums are added, in wave order.
+// so no wave waits for another until their sums are added, in wave order.  One
+// operand's exponents to a DMA: lanes of both in one take a loop over the two buffers
+// (1 x 64 x 14336 10.2 us, 9.2 without).  A third stage of 16 rows: 9.6 for 9.0.
 template <int RB, int MB, int W>
 __global__ void __launch_bounds__(64 * W) stream_kernel(Gemm8Args g) {
-    constexpr int IB = RB / 32, JB = MB / 32, STAGE = (RB + MB) * 128;
-    constexpr int ND = (RB + MB) / 8, XD = (RB + MB + 63) / 64, RING = STAGE + XD * 256;
-    static_assert(W * IB * JB * 4096 <= W * 2 * RING, "the sums fit");
+    constexpr int IB = (RB + 31) / 32, JB = MB / 32, Q = RB < 32 ? RB / 8 : 4;  // Q: quarters
+    constexpr int STAGE = (RB + MB) * 128, ND = (RB + MB) / 8;
+    constexpr int XB = (RB + 63) / 64, XA = (MB + 63) / 64;  // DMAs of exponents
+    constexpr int RING = STAGE + (XB + XA) * 256;
+    static_assert(W * IB * JB * Q * 1024 <= W * 2 * RING, "the sums fit");
     __shared__ __attribute__((aligned(16))) char smem[W * 2 * RING];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l32 = lane & 31, h = lane >> 5;
+    const int rb32 = RB < 32 ? l32 % RB : l32;  // (16 rows of b fill an operand twice)
     const int n0 = blockIdx.x * RB;
     const uint32_t kp = (uint32_t)g.blocks * 128u;
     const __amdgpu_buffer_rsrc_t rb = codes_from(g.b, n0, RB, g.n, kp);
@@ -328,39 +333,32 @@ __global__ void __launch_bounds__(64 * W) stream_kernel(Gemm8Args g) {
     const __amdgpu_buffer_rsrc_t rxa = exps_from(g.a_exps, 0, MB, g.a_tiles, g.blocks);
     // DMA d moves eight rows, those of b first
     const uint32_t off = (uint32_t)(lane / 8) * kp + (uint32_t)slot_of(lane / 8, lane % 8);
-    uint32_t xb[XD], xa[XD];  // where this lane's row of b or a has its exponents
+    uint32_t xb[XB], xa[XA];  // where this lane's rows have their exponents
 #pragma unroll
-    for (int u = 0; u < XD; ++u) {
-        const int at = u * 64 + lane;
-        xb[u] = exps_at(min(n0 + min(at, RB - 1), g.n - 1), n0, g.b_tiles, g.blocks);
-        xa[u] = exps_at(min(max(at - RB, 0), g.m - 1), 0, g.a_tiles, g.blocks);
-    }
+    for (int u = 0; u < XB; ++u)
+        xb[u] = exps_at(min(n0 + min(u * 64 + lane, RB - 1), g.n - 1), n0, g.b_tiles, g.blocks);
+#pragma unroll
+    for (int u = 0; u < XA; ++u)
+        xa[u] = exps_at(min(min(u * 64 + lane, MB - 1), g.m - 1), 0, g.a_tiles, g.blocks);
     char *const ring = smem + wave * (2 * RING);
+    const int a_dmas = min(MB / 8, (g.m + 7) / 8);  // (rows past g.m are not stored)
     const auto dma = [&](int i) {
         char *st = ring + (i & 1) * RING;
         const int kb = wave + i * W;
 #pragma unroll
-        for (int u = 0; u < XD; ++u) {
-            // (RB is a whole number of half waves: a lane's row is of one operand)
-            if (u * 64 + 64 <= RB)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rxb, (lds_void *)(st + STAGE + u * 256), 4,
-                                                         (int)xb[u], kb * 4, 0, 0);
-            else if (u * 64 >= RB)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rxa, (lds_void *)(st + STAGE + u * 256), 4,
-                                                         (int)xa[u], kb * 4, 0, 0);
-            else if (lane < RB % 64)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rxb, (lds_void *)(st + STAGE + u * 256), 4,
-                                                         (int)xb[u], kb * 4, 0, 0);
-            else
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rxa, (lds_void *)(st + STAGE + u * 256), 4,
-                                                         (int)xa[u], kb * 4, 0, 0);
-        }
+        for (int u = 0; u < XB; ++u)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rxb, (lds_void *)(st + STAGE + u * 256), 4,
+                                                     (int)xb[u], kb * 4, 0, 0);
+#pragma unroll
+        for (int u = 0; u < XA; ++u)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                rxa, (lds_void *)(st + STAGE + (XB + u) * 256), 4, (int)xa[u], kb * 4, 0, 0);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             if (d < RB / 8)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *)(st + d * 1024), 16,
                                                          (int)(off + d * 8 * kp), kb * 128, 0, 0);
-            else if (8 * (d - RB / 8) < g.m)  // (columns past g.m are not stored)
+            else if (d - RB / 8 < a_dmas)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
                     ra, (lds_void *)(st + d * 1024), 16, (int)(off + (d - RB / 8) * 8 * kp),
                     kb * 128, 0, 0);
@@ -383,16 +381,16 @@ __global__ void __launch_bounds__(64 * W) stream_kernel(Gemm8Args g) {
         const int *x = reinterpret_cast<const int *>(st + STAGE);
         float sb[IB], sa[JB];
 #pragma unroll
-        for (int r = 0; r < IB; ++r) sb[r] = lin8_pow2(x[32 * r + l32]);
+        for (int r = 0; r < IB; ++r) sb[r] = lin8_pow2(x[32 * r + rb32]);
 #pragma unroll
-        for (int t = 0; t < JB; ++t) sa[t] = lin8_pow2(x[RB + 32 * t + l32]);
+        for (int t = 0; t < JB; ++t) sa[t] = lin8_pow2(x[XB * 64 + 32 * t + l32]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const int slot = slot_of(l32, 2 * c + h);
             bf8 fb[IB][2], fa[JB][2];
 #pragma unroll
             for (int r = 0; r < IB; ++r) {
-                const u4 v = *reinterpret_cast<const u4 *>(st + (32 * r + l32) * 128 + slot);
+                const u4 v = *reinterpret_cast<const u4 *>(st + (32 * r + rb32) * 128 + slot);
                 fb[r][0] = widen8(v[0], v[1], sb[r]);
                 fb[r][1] = widen8(v[2], v[3], sb[r]);
             }
@@ -419,17 +417,17 @@ __global__ void __launch_bounds__(64 * W) stream_kernel(Gemm8Args g) {
 #pragma unroll
         for (int t = 0; t < JB; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                sums[((wave * IB * JB + r * JB + t) * 4 + e) * 64 + lane] =
+            for (int e = 0; e < Q; ++e)
+                sums[((wave * IB * JB + r * JB + t) * Q + e) * 64 + lane] =
                     (f4){acc[r][t][4 * e], acc[r][t][4 * e + 1], acc[r][t][4 * e + 2],
                          acc[r][t][4 * e + 3]};
     __syncthreads();
     // quarter e of block (r, t): rows 32 r + 8 e + 4 h .. of b, row 32 t + l % 32 of a
-    for (int u = wave; u < IB * JB * 4; u += W) {
+    for (int u = wave; u < IB * JB * Q; u += W) {
         f4 s = sums[u * 64 + lane];
 #pragma unroll
-        for (int w = 1; w < W; ++w) s += sums[(w * IB * JB * 4 + u) * 64 + lane];
-        const int m = u / 4 % JB * 32 + l32, n = n0 + u / 4 / JB * 32 + 8 * (u % 4) + 4 * h;
+        for (int w = 1; w < W; ++w) s += sums[(w * IB * JB * Q + u) * 64 + lane];
+        const int m = u / Q % JB * 32 + l32, n = n0 + u / Q / JB * 32 + 8 * (u % Q) + 4 * h;
         if (g.bias) s += lin8_load4<true>(g.bias, n / 4, g.n);
         if (m < g.m) lin8_store4<true>(g.out + (size_t)m * g.n, n / 4, g.n, s);
     }
@@ -478,11 +476,16 @@ double tiles_us(const Gemm8Args &g, const Tiles &t, int splits, int num_cus, Gem
 // The streaming kernel for up to 32 or 64 rows of a.  One workgroup a CU has eight
 // waves (six with 64 rows), more of them four, so that two (for 64 rows: twice the
 // rows of b) share a CU: 32 x 14336 x 4096 12.4 us, 15.9 with eight; 32 x 4096 x 4096
-// 6.4 us, 7.9 with four.
+// 6.4 us, 7.9 with four.  Sixteen rows of b to a workgroup read a more often, but leave
+// no CU idle and are quicker by the block: 32 x 4096 x 14336 18.8 us for 23.1, 32 x 1024 x
+// 14336 11.0 for 13.7, 1 x 1024 x 4096 4.3 for 4.4; but with a workgroup on every CU
+// and few blocks 1 x 4096 x 4096 6.4 for 5.7, 32 x 4096 x 4096 7.0 for 6.5.
 double stream_us(const Gemm8Args &g, int num_cus, Gemm8Plan *p) {
     const bool one = ((int64_t)g.n + 31) / 32 <= num_cus;
     p->rows_a = g.m <= 32 ? 32 : 64;
-    p->rows_b = p->rows_a == 64 && !one ? 64 : 32;
+    const bool half = p->rows_a == 32 && ((int64_t)g.n + 15) / 16 <= num_cus &&
+                      (((int64_t)g.n + 7) / 8 <= num_cus || g.blocks > 64);
+    p->rows_b = p->rows_a == 64 && !one ? 64 : half ? 16 : 32;
     p->waves = !one ? 4 : p->rows_a == 32 ? 8 : 6;
     p->splits = 1;
     const int per_cu = !one && p->rows_a == 32 ? 2 : 1;
@@ -529,7 +532,8 @@ size_t gemm8_workspace(const Gemm8Args &a, const Gemm8Plan &p) {
 void gemm8(const Gemm8Args &a, const Gemm8Plan &p, int num_cus, hipStream_t s) {
     if (a.m == 0 || a.n == 0) return;
     if (p.waves) {
-        if (p.rows_a == 32) p.waves == 8 ? run_stream<32, 32, 8>(a, s) : run_stream<32, 32, 4>(a, s);
+        if (p.rows_b == 16) run_stream<16, 32, 8>(a, s);
+        else if (p.rows_a == 32) p.waves == 8 ? run_stream<32, 32, 8>(a, s) : run_stream<32, 32, 4>(a, s);
         else p.rows_b == 32 ? run_stream<32, 64, 6>(a, s) : run_stream<64, 64, 4>(a, s);
         return;
     }

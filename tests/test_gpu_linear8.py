@@ -276,6 +276,8 @@ def test_matmul(hip, m, n, k, a_tiles, b_tiles):
 # few rows against a long b, and results of many tiles, past every tile's edge
 @pytest.mark.parametrize("m,n,k", [(1, 8200, 300), (32, 8225, 1200), (64, 1000, 1500),
                                    (48, 5000, 2100), (61, 16380, 700), (1930, 3970, 390),
+                                   (1, 37, 9000), (32, 1001, 3000), (19, 4000, 8400),
+                                   (3, 3900, 1000),
                                    (3841, 4000, 390)])
 @pytest.mark.parametrize("a_tiles", [False, True])
 def test_matmul_of_many(hip, m, n, k, a_tiles):
