@@ -78,7 +78,7 @@ __device__ __forceinline__ int slot_of(int row, int k16) { return 16 * (k16 ^ (r
 // filling while the other is multiplied (in registers the exponents would make every
 // block wait for all DMAs in flight).
 //
-// What bounds it: 4096^3 in 256 x 256 tiles of sixteen waves 114-117 us, 1180-1207
+// What bounds it: 4096^3 in 256 x 256 tiles of sixteen waves 111-115 us, 1190-1240
 // TFLOP/s, of which the 64 MiB of results are some 13 us at the end; a large bf16
 // library product runs at 1208 on the same card, at its power limit.  Four waves
 // of 128 x 64 on 256 x 128 tiles 134 us, of 64 x 64 on 128 x 128 124-134.  Results

@@ -325,7 +325,9 @@ int clove_hip_paged_evict(CTensor block_tables, CTensor context_lens, CTensor we
  * codes are x * 2^-e rounded to nearest, ties to even, so an element is off by at
  * most 2^-4 of itself (half of 2^(e-9) for the smallest).  Magnitudes past 448 *
  * 2^119 become that; infinities and NaN become NaN, which products carry on.
- * Leading dimensions of x are rows; codes (and exps of rows) keep them. */
+ * Leading dimensions of x are rows; codes (and exps of rows) keep them.
+ * The entries allocate their results and workspaces, like most here: not for code
+ * under HIP graph capture. */
 
 /* h = x + residual (or x where residual is NULL), out = h * gamma /
  * sqrt(mean(h^2) + eps) over the last dimension, x f32 [.., cols], residual x's
