@@ -235,6 +235,9 @@ def _shape_arr(shape: Sequence[int]):
     return (C.c_size_t * max(1, len(shape)))(*[int(s) for s in shape])
 
 
+_NULL = C.c_void_p()  # what every freed tensor holds; never written to
+
+
 class Tensor:
     """Owns one CTensor handle; freed with clove_hip_tensor_free."""
 
@@ -248,7 +251,7 @@ class Tensor:
         return self._h
 
     def free(self) -> None:
-        h, self._h = self._h, None
+        h, self._h = self._h, _NULL
         if h and _lib is not None:
             _lib.clove_hip_tensor_free(h)
 

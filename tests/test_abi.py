@@ -418,3 +418,22 @@ def test_graph_rope_rejects_bad_parameters():
         g.rope(99, 8)
     with pytest.raises(ca.CloveError):
         g.op("rope", x)          # two integer parameters: only through graph_rope
+
+
+def test_freed_tensors_are_refused():
+    """A freed tensor's handle is null: calls report it as a status code."""
+    t = ca.Tensor(None)
+    t.free()
+    t.free()
+    assert t.handle.value is None and t.device_ptr == 0 and t.numel == 0
+    for f in (lambda: ca.adamw_step([t], [t], [t], [t], step=1),
+              lambda: ca.FusedChain([("relu", -1, 0)], [t])(),
+              lambda: ca.relu(t)):
+        with pytest.raises(ca.CloveError) as e:
+            f()
+        assert e.value.code in (ca.ERR_INVALID, ca.ERR_NOT_INIT), e.value
+    g = ca.Graph()
+    m = g.compile([g.op("relu", g.input("4,8"))])
+    with pytest.raises(ca.CloveError) as e:
+        m.execute([t])
+    assert e.value.code == ca.ERR_INVALID
