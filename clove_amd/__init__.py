@@ -503,8 +503,7 @@ def adamw_step(weights, grads, m, v, step: int, lr: float = 1e-3, beta1: float =
 def paged_attention(q: Tensor, k: Optional[Tensor], v: Optional[Tensor], kv_cache: Tensor,
                     block_tables: Tensor, context_lens: Tensor,
                     scale: Optional[float] = None) -> Tensor:
-    kh = k.handle if k is not None else None
-    vh = v.handle if v is not None else None
+    kh, vh = _opt(k), _opt(v)
     if scale is None:
         p = lib().clove_hip_paged_attention(q.handle, kh, vh, kv_cache.handle,
                                             block_tables.handle, context_lens.handle)
@@ -536,7 +535,13 @@ def paged_kv8_cache(num_blocks: int, heads: int, block_size: int, head_dim: int)
 
 
 def _opt(t: Optional[Tensor]):
-    return t.handle if t is not None else None
+    """The handle of an operand that may be left out.  A freed tensor is refused here:
+    to the entries its null handle would mean none."""
+    if t is None:
+        return None
+    if not t.handle:
+        raise CloveError(ERR_INVALID, "an optional operand is a freed tensor")
+    return t.handle
 
 
 def paged_kv8_append(codes: Tensor, exps: Tensor, k: Tensor, v: Tensor, block_tables: Tensor,
@@ -576,7 +581,7 @@ def paged_kv8_attention(q: Tensor, codes: Tensor, exps: Tensor, block_tables: Te
     w = C.c_void_p()
     out = _handle(lib().clove_hip_paged_kv8_attention(
         q.handle, codes.handle, exps.handle, block_tables.handle, context_lens.handle,
-        _opt(row_starts), scale, weights.handle, C.byref(w)))
+        _opt(row_starts), scale, _opt(weights), C.byref(w)))
     return out, Tensor(w.value)
 
 
@@ -597,7 +602,7 @@ def rms_norm(x: Tensor, gamma: Tensor, residual: Optional[Tensor] = None, eps: f
     if residual is None:
         return _handle(lib().clove_hip_rms_norm(x.handle, None, gamma.handle, eps, None))
     h = C.c_void_p()
-    out = _handle(lib().clove_hip_rms_norm(x.handle, residual.handle, gamma.handle, eps,
+    out = _handle(lib().clove_hip_rms_norm(x.handle, _opt(residual), gamma.handle, eps,
                                            C.byref(h)))
     return out, Tensor._take(h)
 

@@ -437,3 +437,20 @@ def test_freed_tensors_are_refused():
     with pytest.raises(ca.CloveError) as e:
         m.execute([t])
     assert e.value.code == ca.ERR_INVALID
+
+
+def test_freed_optional_operands_are_refused():
+    """A null handle means none where an operand may be left out, so a freed tensor
+    must not get that far: the result would lack the operand without a word."""
+    t = ca.Tensor(None)
+    t.free()
+    for f in (lambda: ca.matmul_e4m3(t, t, t, t, t), lambda: ca.rms_norm_backward(t, t, t, t),
+              lambda: ca.rms_norm(t, t, t), lambda: ca.rms_norm_e4m3(t, t, t),
+              lambda: ca.paged_attention(t, t, t, t, t, t),
+              lambda: ca.paged_attention(t, None, t, t, t, t),
+              lambda: ca.paged_kv8_attention(t, t, t, t, t, t, 1.0),
+              lambda: ca.paged_kv8_attention(t, t, t, t, t, None, 1.0, t),
+              lambda: ca.paged_kv8_append(t, t, t, t, t, t, t)):
+        with pytest.raises(ca.CloveError, match="freed") as e:
+            f()
+        assert e.value.code == ca.ERR_INVALID

@@ -433,6 +433,22 @@ def test_refusals(hip):
     refused(hip.ERR_INVALID, hip.matmul_e4m3, moved, a[1], *b)
 
 
+def test_freed_operands_are_refused(hip):
+    """Not taken for operands that are left out."""
+    ones = hip.tensor(np.ones((3, 8), np.float32))
+    gamma = hip.tensor(np.ones(8, np.float32))
+    q = hip.quantize_e4m3(ones)
+    gone = hip.tensor(np.ones((3, 8), np.float32))
+    gone.free()
+    for f in (lambda: hip.matmul_e4m3(*q, *q, gone), lambda: hip.rms_norm(ones, gamma, gone),
+              lambda: hip.rms_norm_e4m3(ones, gamma, gone),
+              lambda: hip.rms_norm_backward(ones, gamma, ones, gone),
+              lambda: hip.rms_norm(gone, gamma), lambda: hip.quantize_e4m3(gone)):
+        with pytest.raises(hip.CloveError) as e:
+            f()
+        assert e.value.code == hip.ERR_INVALID
+
+
 # ---- more workgroups than one launch holds ------------------------------------------
 
 def test_many_rows(hip):
