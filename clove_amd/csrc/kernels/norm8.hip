@@ -10,7 +10,8 @@
 //   g = grad_out gamma, grad_h = r (g - h r^2 mean(g h)) + grad_sum,
 //   grad_gamma = sum over rows of grad_out h r
 //
-// with the two sums of a row in 64 bits (h^2 leaves f32's range from 2^64 on).
+// with g and the two sums of a row in 64 bits (h^2 leaves f32's range from 2^64 on, and g
+// can where r brings grad_h back into it).
 #include "linear8.h"
 
 namespace clove {
@@ -182,9 +183,12 @@ void norm_any(const RmsNormArgs &a, hipStream_t s) {
 
 // ---- the gradient ------------------------------------------------------------
 
-__device__ __forceinline__ double dot(cl_f4 a, cl_f4 b, double s) {
+// s + the sum of gy gamma h, gy gamma as the exact product: in 32 bits it leaves the
+// range, or loses its bits below 2^-126, where r brings the gradient back.
+__device__ __forceinline__ double dot(cl_f4 gy, cl_f4 gamma, cl_f4 h, double s) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s = __builtin_fma((double)a[e], (double)b[e], s);
+    for (int e = 0; e < 4; ++e)
+        s = __builtin_fma((double)gy[e] * (double)gamma[e], (double)h[e], s);
     return s;
 }
 
@@ -203,9 +207,11 @@ __device__ __forceinline__ void grad_chunk(const RmsNormGradArgs &a, size_t row,
     cl_f4 dh;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
+        // (h r is at most sqrt(cols): a rounding here and one in the product)
         (*acc)[e] += gy[e] * (float)((double)h[e] * r);
-        // in 64 bits where the two terms meet: they can cancel
-        dh[e] = (float)((double)(gy[e] * gamma[e]) * r - (double)h[e] * m + (double)ds[e]);
+        // in 64 bits where the terms meet, since they can cancel, and rounded once
+        dh[e] = (float)__builtin_fma((double)gy[e] * (double)gamma[e], r,
+                                     __builtin_fma(-(double)h[e], m, (double)ds[e]));
     }
     if (a.grad_h) lin8_store4<ODD>(a.grad_h + row * a.cols, c, a.cols, dh);
 }
@@ -245,16 +251,27 @@ __global__ void __launch_bounds__(T) grad_kernel(RmsNormGradArgs a) {
             ds[s][i] = lin8_load4<ODD>(a.grad_sum + row * a.cols, c, a.grad_sum ? cols : 0);
         }
     };
+    // Long rows are widened again behind their sums: kept in 64 bits, four chunks a thread
+    // spill, and of two [5000, 2100] takes 46.7 us for 45.2, [8192, 4096] 104.0 for 103.3.
+    // Short rows stay as they are: [5000, 400] 11.5 for 12.2, [4000, 1500] 21.6 for 22.7.
+    const auto widen_again = [&](cl_f4 (&v)[NV]) {
+        if constexpr (NV > 2 || TR > 256)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(v[i]));
+    };
     const auto work = [&](size_t row, int s) {
         double v[2] = {0.0, 0.0};
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             v[0] = square_sum(h[s][i], v[0]);
-            v[1] = dot(gy[s][i] * gamma[i], h[s][i], v[1]);
+            v[1] = dot(gy[s][i], gamma[i], h[s][i], v[1]);
         }
         row_sum<T, TR>(v, red);
         double r, m;
         coefficients(v[0], v[1], a.cols, a.eps, &r, &m);
+        widen_again(gamma);
+        widen_again(gy[s]);
+        widen_again(h[s]);
         if (row < a.rows)
 #pragma unroll
             for (int i = 0; i < NV; ++i)
@@ -332,7 +349,7 @@ __global__ void __launch_bounds__(1024) grad_stats_kernel(RmsNormGradArgs a, siz
         const cl_f4 h = lin8_load4<ODD>(a.h + row * a.cols, c, a.cols);
         const cl_f4 gy = lin8_load4<ODD>(a.grad_out + row * a.cols, c, a.cols);
         s[0] = square_sum(h, s[0]);
-        s[1] = dot(gy * lin8_load4<ODD>(a.gamma, c, a.cols), h, s[1]);
+        s[1] = dot(gy, lin8_load4<ODD>(a.gamma, c, a.cols), h, s[1]);
     }
     row_sum<1024, 1024>(s, red);
     if (threadIdx.x == 0)

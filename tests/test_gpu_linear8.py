@@ -192,6 +192,40 @@ def test_rms_norm_backward(hip, rows, cols, stream):
             np.testing.assert_array_equal(a, b)
 
 
+def test_rms_norm_backward_extremes(hip):
+    """Rows whose squares leave f32's range, a zero row, eps 0 and large, and grad_out
+    times gamma past f32's range and under it, where r brings the gradient back."""
+    g = rng(23)
+    sizes = np.array([1e30, 1e25, 1e-30, 1e-42, 1.0, 0.0])[:, None]
+    h = (g.standard_normal((6, 300)) * sizes).astype(np.float32)
+    for size in (1e10, 1.0, 1e-10):
+        gamma = (g.uniform(0.5, 2, 300) * size).astype(np.float32)
+        # r times these is near 1 in the first rows, which eps does not reach
+        gy = (g.standard_normal((6, 300)) * [[1e30], [1e20], [1e-32], [1e-35], [1e-3], [1e-3]]
+              ).astype(np.float32)
+        for eps in (1e-5, 0.0, 100.0):
+            good = slice(0, 5 if eps == 0 else 6)
+            args = h[good], gamma, gy[good]
+            (dh, th), (dg, tg) = ref.rms_norm_backward(*args, eps=eps)
+            a, b = (t.numpy() for t in hip.rms_norm_backward(*map(hip.tensor, args), eps=eps))
+            within(a, dh, th, f"grad_h, gamma {size}, eps {eps}")
+            within(b, dg, tg, f"grad_gamma, gamma {size}, eps {eps}")
+
+
+def test_rms_norm_backward_keeps_what_is_not_finite_in_its_row(hip):
+    g = rng(24)
+    for rows, cols in ((9, 300), (900, 130), (40, 2100), (9, 9000)):
+        h, gy = (g.standard_normal((rows, cols)).astype(np.float32) for _ in range(2))
+        gamma = g.uniform(0.5, 2, cols).astype(np.float32)
+        h[2, 7], h[5, cols - 1], gy[7, 3] = np.nan, np.inf, np.nan
+        bad = [2, 5, 7]
+        a, b = (t.numpy() for t in hip.rms_norm_backward(*map(hip.tensor, (h, gamma, gy))))
+        assert np.isnan(a[bad]).all() and np.isnan(b[[3, cols - 1]]).all() and np.isnan(b).all()
+        good = np.setdiff1d(np.arange(rows), bad)
+        (dh, th), _ = ref.rms_norm_backward(h[good], gamma, gy[good])
+        within(a[good], dh, th)
+
+
 def test_rms_norm_backward_against_differences(hip):
     """The gradients are those of the forward pass: central differences of it, in
     32 bits, whose error is the outputs' rounding over the step."""
