@@ -253,6 +253,39 @@ def test_rms_norm_backward_against_differences(hip):
         assert abs((loss(h, gamma + e) - loss(h, gamma - e)) / (2 * d) - dg[i]) <= tol
 
 
+# every class of columns, a workgroup walking its rows in turns: an odd and an even number
+# of them, the last one not full
+@pytest.mark.parametrize("rows,cols", [(60001, 33), (17000, 128), (20001, 130), (9000, 256),
+                                       (5000, 400), (7001, 512), (5000, 700), (4100, 1024),
+                                       (2000, 1500), (1030, 2048), (1001, 2049), (3000, 3001),
+                                       (4095, 2052), (5000, 2100), (1030, 5000), (700, 8192),
+                                       (700, 9000), (2000, 8196), (65, 100), (64, 100), (3, 1500),
+                                       (2, 20000)])
+@pytest.mark.parametrize("wanted", ["both", "gamma"])
+def test_rms_norm_backward_of_whole_numbers_is_exact(hip, rows, cols, wanted):
+    """With h of +-1 and eps 0 every row's root mean square is 1 and grad_gamma a sum of
+    whole numbers below 2^24 in magnitude, of which none is 0: a row lost or taken
+    twice shows."""
+    g = rng(rows + cols)
+    h = g.choice(np.float32([-1, 1]), (rows, cols))
+    gy = (g.integers(1, 9, (rows, cols)) * g.choice([-1, 1], (rows, cols))).astype(np.float32)
+    assert 8 * rows < 1 << 24
+    gamma = np.ones(cols, np.float32)
+    t = [hip.tensor(v) for v in (h, gamma, gy)]
+    if wanted == "both":
+        a, b = (v.numpy() for v in hip.rms_norm_backward(*t, eps=0.0))
+        # a row's sum of whole numbers is exact too: cols divides it with one rounding in 64
+        # bits, and the difference is rounded to 32
+        want = gy - h * ((gy * h).sum(1, keepdims=True, dtype=np.float64) / cols)
+        within(a, want, ref.U * 1.0001 * np.abs(want) + 2.0 ** -48)
+    else:
+        out = C.c_void_p()
+        assert hip.lib().clove_hip_rms_norm_backward(*[v.handle for v in t], None, 0.0, None,
+                                                     C.byref(out)) == hip.OK
+        b = hip.Tensor(out.value).numpy()
+    np.testing.assert_array_equal(b, (gy * h).sum(0, dtype=np.float64))
+
+
 def test_rms_norm_backward_skips_what_is_not_wanted(hip):
     g = rng(22)
     h, gamma, gy = (hip.tensor(g.standard_normal(s).astype(np.float32))
