@@ -369,6 +369,40 @@ def test_matmul_of_small_whole_numbers_is_exact(hip, m, n, k):
     np.testing.assert_array_equal(got, a.astype(np.float64) @ b.T.astype(np.float64) + bias)
 
 
+# a size for every kernel, whole and cut along k, with ragged edges (which one takes which
+# is checked on the CPU)
+FORMS = [(32, 1001, 2900), (3, 3900, 1000), (30, 8225, 1200), (40, 5000, 2100),
+         (61, 16380, 700), (65, 130, 257), (70, 60, 4100), (3654, 133, 2435), (300, 700, 400),
+         (70, 9596, 4290), (66, 50, 977), (1930, 3970, 390), (1880, 1608, 21156),
+         (849, 1672, 15122), (840, 853, 31240), (3841, 4001, 390), (1927, 4065, 13493),
+         (1967, 1928, 20452), (997, 1980, 25421)]
+
+
+@pytest.mark.parametrize("m,n,k", FORMS)
+def test_matmul_of_every_form_is_exact(hip, m, n, k):
+    """Whole numbers of up to 8 with exponents of 0 and 1: sums below 2^24, exact in 32
+    bits in any order, so a block lost, taken twice or scaled by another's exponent
+    shows; a bias on top."""
+    g = rng(m + n + k)
+    code = ref.encode(np.arange(9, dtype=np.float32))
+
+    def operand(rows, tiles):
+        x = g.integers(0, 9, (rows, ref.up(k)), np.uint8)
+        x[:, k:] = 0
+        minus = g.integers(0, 2, x.shape, np.uint8)
+        e = g.integers(0, 2, (-(-rows // 128) if tiles else rows, ref.up(k) // 128)).astype(np.int32)
+        scale = np.repeat(e, 128, 0)[:rows] if tiles else e
+        v = np.where(minus, -x.astype(np.float32), x).reshape(rows, -1, 128)
+        v *= np.exp2(scale.astype(np.float32))[..., None]
+        return code[x] | minus << 7, e, v.reshape(rows, -1)
+
+    (a, ea, va), (b, eb, vb) = operand(m, False), operand(n, True)
+    assert 256 * k < 1 << 24
+    bias = g.integers(-50, 50, n).astype(np.float32)
+    got = hip.matmul_e4m3(*put(hip, a, ea, b, eb), hip.tensor(bias)).numpy()
+    np.testing.assert_array_equal(got, va @ vb.T + bias)
+
+
 @pytest.mark.parametrize("m,n,k", [(8, 512, 1024), (512, 512, 1024), (300, 600, 4096)])
 def test_matmul_sums_in_32_bits(hip, m, n, k):
     """K additions, each off by at most a step of a partial sum no larger than the

@@ -70,3 +70,36 @@ def test_missing_handles_are_refused():
         assert "together" in ca.last_error()
     assert not lib.clove_hip_matmul_e4m3(None, None, None, None, None)
     assert lib.clove_hip_last_status() == ca.ERR_INVALID
+
+
+class Gemm8Args(C.Structure):  # kernels/launch.hpp
+    _fields_ = ([(n, C.c_void_p) for n in ("a", "b", "a_exps", "b_exps", "bias", "out", "ws")]
+                + [(n, C.c_int) for n in ("m", "n", "blocks")]
+                + [(n, C.c_bool) for n in ("a_tiles", "b_tiles")])
+
+
+class Gemm8Plan(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("waves", "rows_a", "rows_b", "bm", "bn", "tiles_m",
+                                       "tiles_n", "splits", "per_split")]
+
+
+def test_the_products_tested_reach_every_form():
+    """The kernel that a product takes is chosen by price: the sizes of the GPU test have
+    to reach each, and each way of tiles that k is cut, whatever the prices become."""
+    from test_gpu_linear8 import FORMS
+
+    plan = ca.lib()["_ZN5clove1k10gemm8_planERKNS0_9Gemm8ArgsEi"]
+    plan.restype, plan.argtypes = Gemm8Plan, [C.POINTER(Gemm8Args), C.c_int]
+    seen = set()
+    for m, n, k in FORMS:
+        p = plan(C.byref(Gemm8Args(m=m, n=n, blocks=-(-k // 128))), 256)
+        if p.waves:
+            seen.add(("stream", p.rows_b, p.rows_a, p.waves))
+        else:
+            blocks = -(-k // 128)
+            assert (p.splits - 1) * p.per_split < blocks <= p.splits * p.per_split
+            seen.add(("tiles", p.bm, p.bn, "cut" if p.splits > 1 else "whole"))
+    assert seen == {("stream", 16, 32, 8), ("stream", 32, 32, 8), ("stream", 32, 32, 4),
+                    ("stream", 32, 64, 6), ("stream", 64, 64, 4)} | {
+        ("tiles", bm, bn, how) for bm, bn in ((64, 64), (64, 128), (128, 128), (256, 256))
+        for how in ("whole", "cut")}
