@@ -475,16 +475,19 @@ double tiles_us(const Gemm8Args &g, const Tiles &t, int splits, int num_cus, Gem
 
 // The streaming kernel for up to 32 or 64 rows of a.  One workgroup a CU has eight
 // waves (six with 64 rows), more of them four, so that two (for 64 rows: twice the
-// rows of b) share a CU: 32 x 14336 x 4096 12.4 us, 15.9 with eight; 32 x 4096 x 4096
-// 6.4 us, 7.9 with four.  Sixteen rows of b to a workgroup read a more often, but leave
-// no CU idle and are quicker by the block: 32 x 4096 x 14336 18.8 us for 23.1, 32 x 1024 x
-// 14336 11.0 for 13.7, 1 x 1024 x 4096 4.3 for 4.4; but with a workgroup on every CU
-// and few blocks 1 x 4096 x 4096 6.4 for 5.7, 32 x 4096 x 4096 7.0 for 6.5.
+// rows of b) share a CU: with b from memory (copies in turn, more than the last-level
+// cache holds) 32 x 14336 x 4096 16.1 us, 17.7 with eight; 32 x 4096 x 4096 in 32 rows of
+// b 8.6 us, 9.7 with four; 64 x 14336 x 4096 18.7 us, 24.3 with 32 rows of b; 64 x 8000 x
+// 4096 13.6, 16.7 with 64.  Sixteen rows of b to a workgroup read a more often, but leave no
+// CU idle and are quicker by the block, as long as one round of them is enough (32 x
+// 14336 x 4096 23.5 us).  From memory and from the last-level cache, for 32 rows of b:
+//   32 x 4096 x 14336 19.2 us for 23.8, 12.6 for 15.0; 32 x 4096 x 8192 11.6 for 14.5, 9.0 for 12.5
+//   32 x 4096 x 4096 7.4 for 8.7, 5.8 for 6.2; 1 x 4096 x 4096 6.3 for 6.7, 5.6 for 5.6
+//   32 x 1024 x 14336 17.0 for 21.7, 9.8 for 11.2; 32 x 4096 x 512 3.8 for 3.8 (the launch)
 double stream_us(const Gemm8Args &g, int num_cus, Gemm8Plan *p) {
     const bool one = ((int64_t)g.n + 31) / 32 <= num_cus;
     p->rows_a = g.m <= 32 ? 32 : 64;
-    const bool half = p->rows_a == 32 && ((int64_t)g.n + 15) / 16 <= num_cus &&
-                      (((int64_t)g.n + 7) / 8 <= num_cus || g.blocks > 64);
+    const bool half = p->rows_a == 32 && ((int64_t)g.n + 15) / 16 <= num_cus;
     p->rows_b = p->rows_a == 64 && !one ? 64 : half ? 16 : 32;
     p->waves = !one ? 4 : p->rows_a == 32 ? 8 : 6;
     p->splits = 1;

@@ -371,7 +371,7 @@ def test_matmul_of_small_whole_numbers_is_exact(hip, m, n, k):
 
 # a size for every kernel, whole and cut along k, with ragged edges (which one takes which
 # is checked on the CPU)
-FORMS = [(32, 1001, 2900), (3, 3900, 1000), (30, 8225, 1200), (40, 5000, 2100),
+FORMS = [(32, 1001, 2900), (3, 3900, 1000), (3, 5000, 1000), (30, 8225, 1200), (40, 5000, 2100),
          (61, 16380, 700), (65, 130, 257), (70, 60, 4100), (3654, 133, 2435), (300, 700, 400),
          (70, 9596, 4290), (66, 50, 977), (1930, 3970, 390), (1880, 1608, 21156),
          (849, 1672, 15122), (840, 853, 31240), (3841, 4001, 390), (1927, 4065, 13493),
