@@ -435,8 +435,14 @@ __global__ void __launch_bounds__(64 * W) stream_kernel(Gemm8Args g) {
 
 // ---- which kernel ------------------------------------------------------------
 //
-// Every kernel is priced in microseconds with what it measured: a start, so much
-// for a step along k of the workgroups that share a CU (step[i] with i + 1 of them),
+// Up to 32 rows of a go to the streaming kernel.  No tiles did them faster, whole or cut
+// along k (32 x 1024 x 14336 17.2 us from memory and 9.8 from the last-level cache, 18.2 and
+// 12.0 in tiles; 32 x 128 x 16384 16.3 and 10.9, 19.1 and 12.2; 32 x 14336 x 4096 16.2 and
+// 10.7, 19.6 and 16.4), though it does not cut k over workgroups: such a long k with so few
+// rows of b leaves most CUs idle, three times the time of its bytes.
+//
+// More rows are priced in microseconds, every kernel with what it measured: a start, so
+// much for a step along k of the workgroups that share a CU (step[i] with i + 1 of them),
 // the results on their way out at 5.5 TB/s, and for products cut along k a second
 // launch that joins them.  The cheapest runs.
 
@@ -484,17 +490,18 @@ double tiles_us(const Gemm8Args &g, const Tiles &t, int splits, int num_cus, Gem
 //   32 x 4096 x 14336 19.2 us for 23.8, 12.6 for 15.0; 32 x 4096 x 8192 11.6 for 14.5, 9.0 for 12.5
 //   32 x 4096 x 4096 7.4 for 8.7, 5.8 for 6.2; 1 x 4096 x 4096 6.3 for 6.7, 5.6 for 5.6
 //   32 x 1024 x 14336 17.0 for 21.7, 9.8 for 11.2; 32 x 4096 x 512 3.8 for 3.8 (the launch)
-double stream_us(const Gemm8Args &g, int num_cus, Gemm8Plan *p) {
+void stream_form(const Gemm8Args &g, int num_cus, Gemm8Plan *p) {
     const bool one = ((int64_t)g.n + 31) / 32 <= num_cus;
     p->rows_a = g.m <= 32 ? 32 : 64;
     const bool half = p->rows_a == 32 && ((int64_t)g.n + 15) / 16 <= num_cus;
     p->rows_b = p->rows_a == 64 && !one ? 64 : half ? 16 : 32;
     p->waves = !one ? 4 : p->rows_a == 32 ? 8 : 6;
     p->splits = 1;
-    const int per_cu = !one && p->rows_a == 32 ? 2 : 1;
-    const double step = p->rows_b == 64 ? 1.75 : p->rows_a == 64 ? 1.3 : one ? 0.95 : 1.25;
-    const double turns = std::ceil(std::ceil((double)g.n / p->rows_b) / ((double)num_cus * per_cu));
-    return 2.5 + turns * ((g.blocks + p->waves - 1) / p->waves) * step;
+}
+// What it takes for 33 to 64 rows, where tiles can be quicker.
+double stream_us(const Gemm8Args &g, int num_cus, const Gemm8Plan &p) {
+    const double turns = std::ceil(std::ceil((double)g.n / p.rows_b) / num_cus);
+    return 2.5 + turns * ((g.blocks + p.waves - 1) / p.waves) * (p.rows_b == 64 ? 1.75 : 1.3);
 }
 
 template <int BM, int BN, int KG, int MINW>
@@ -513,8 +520,9 @@ void run_stream(const Gemm8Args &g, hipStream_t s) {
 Gemm8Plan gemm8_plan(const Gemm8Args &g, int num_cus) {
     Gemm8Plan best{};
     if (g.m == 0 || g.n == 0) return best;
-    double best_us = g.m <= 64 ? stream_us(g, num_cus, &best) : 0.0;
-    if (g.m <= 32) return best;  // (no tiles measured faster)
+    if (g.m <= 64) stream_form(g, num_cus, &best);
+    if (g.m <= 32) return best;
+    double best_us = g.m <= 64 ? stream_us(g, num_cus, best) : 0.0;
     for (const Tiles &t : kTiles)
         for (int splits = 1; splits <= kMaxSplits; splits *= 2) {
             if (splits > 1 && g.blocks < 2 * splits) break;
