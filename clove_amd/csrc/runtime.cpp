@@ -56,10 +56,17 @@ Context &ctx() {
 }
 bool ctx_ready() { return g_ready; }
 
+// The dimensions' product, without its zeros, has to stay below 2^60: bytes, and rows
+// counted from some of the dimensions, then fit 64 bits.
 size_t numel_of(const std::vector<size_t> &shape) {
     size_t n = 1;
-    for (size_t d : shape) n *= d;
-    return n;
+    bool none = false;
+    for (size_t d : shape) {
+        none |= d == 0;
+        CLOVE_REQUIRE(!__builtin_mul_overflow(n, d ? d : 1, &n) && n < (size_t(1) << 60),
+                      CLOVE_HIP_ERR_SHAPE, "shape " + shape_str(shape) + " is too large");
+    }
+    return none ? 0 : n;
 }
 
 std::string shape_str(const std::vector<size_t> &shape) {

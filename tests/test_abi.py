@@ -454,3 +454,14 @@ def test_freed_optional_operands_are_refused():
         with pytest.raises(ca.CloveError, match="freed") as e:
             f()
         assert e.value.code == ca.ERR_INVALID
+
+
+def test_shapes_whose_size_wraps_are_refused():
+    """Before the device is asked: a product of dimensions past 64 bits would name a small
+    tensor of a large shape, whose rows no kernel could count."""
+    for shape in ((1 << 62,), (1 << 32, 1 << 32), (1 << 40, 1 << 40, 0), (3, 1 << 63, 2),
+                  ((1 << 32) + 1, (1 << 32) - 1)):
+        for dtype in (np.float32, np.uint8):
+            with pytest.raises(ca.CloveError) as e:
+                ca.empty(shape, dtype)
+            assert e.value.code == ca.ERR_SHAPE, shape
