@@ -33,7 +33,7 @@ __device__ __forceinline__ unsigned lin8_mag(float x) {
 
 // Most waves hold nothing past 448 * 2^119, no infinity and no NaN.  There |x|'s
 // bits are lin8_mag and a code needs no clamp (PLAIN): rows of [2050, 3000] both ways
-// 12.3 us, 13.7 where every element takes the longer way.
+// 11.0 us a call, 12.1 where every element takes the longer way; of [4096, 11008] 55.1, 57.6.
 constexpr unsigned kLin8Plain = 0x7f600000u;
 __device__ __forceinline__ unsigned lin8_bits(float x) {
     return __float_as_uint(x) & 0x7fffffffu;

@@ -123,7 +123,9 @@ __global__ void __launch_bounds__(T) norm_kernel(RmsNormArgs a, size_t row0) {
     }
 }
 
-// Rows that registers do not hold: stats[row] = r first, a workgroup a row...
+// Rows that registers do not hold: stats[row] = r first, a workgroup a row, so that x and
+// the residual are read twice: [2000, 16400] in 32 bits 77 us, 150 with the residual (3.4
+// and 3.5 TB/s of what has to move), [2000, 16384] in one pass 57 and 102...
 constexpr int kWide = 16384;
 template <bool ODD>
 __global__ void __launch_bounds__(1024) norm_stats_kernel(RmsNormArgs a, size_t row0) {
@@ -308,8 +310,10 @@ __global__ void __launch_bounds__(T) grad_kernel(RmsNormGradArgs a) {
 }
 
 // grad_gamma: the rows of `part` added up, 32 columns to a workgroup, every 128th
-// row to a thread and then those in halves, in one order: 2.7 us for 256 rows of
-// 2049, 3.0 for 512 (with 64 columns 2.8 and 3.3, with 16 2.8 and 3.6).
+// row to a thread and then those in halves, in one order.  It follows the kernel whose
+// rows it adds: with it a call takes 13.5 us for 8.75 at [1001, 2049] (256 rows) and 83.3
+// for 79.6 at [8192, 4096]; 4.0 and 4.9 of kernel in a trace.  Launched behind itself it
+// takes 2.7 for 256 or 512 rows of 2049, 2.65 and 2.9 with 64 columns to a workgroup.
 __global__ void __launch_bounds__(1024) grad_join_kernel(RmsNormGradArgs a, int parts,
                                                           size_t done) {
     __shared__ cl_f4 sums[128][8];
@@ -336,9 +340,9 @@ __global__ void __launch_bounds__(1024) grad_join_kernel(RmsNormGradArgs a, int 
     if (col < (size_t)a.cols) a.grad_gamma[col] = total;
 }
 
-// Rows that registers do not hold: the sums first ([2000, 16384] 134 us; 118 in one
+// Rows that registers do not hold: the sums first ([2000, 16384] 131-134 us; 118 in one
 // pass of 512 threads that spill, which takes 140 where these take 124 for [3000, 9001]
-// and 33 where they take 27 for [300, 16380])...
+// and 33 where they take 27 for [300, 16380]; rows kept in LDS are not tried)...
 constexpr int kWideGrad = 8192;
 template <bool ODD>
 __global__ void __launch_bounds__(1024) grad_stats_kernel(RmsNormGradArgs a, size_t row0) {

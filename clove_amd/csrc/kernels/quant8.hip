@@ -11,8 +11,9 @@
 // wave, its codes 128, and a column's RPT codes one piece of the transposed tile,
 // which goes through LDS to leave in lines: x is read once for both ways.
 //
-// What bounds it: memory, 4096 x 14336 in 128 x 128 blocks both ways 67.5 us, 5.2 TB/s;
-// 2050 x 3000 in rows both ways 11.8 us for 7.8 of bytes, 408 tiles on 256 CUs.
+// What bounds it: memory, 4096 x 14336 in 128 x 128 blocks both ways 67.4 us, 5.2 TB/s;
+// 16384 x 8192 in rows both ways 157 us, 5.2 TB/s, transposed alone 134, 5.05; 2050 x 3000
+// in rows both ways 11-12 us for 7.8 of bytes, 408 tiles on 256 CUs.
 #include "linear8.h"
 
 namespace clove {
@@ -196,7 +197,7 @@ void quantize8(const Quant8Args &a, hipStream_t s) {
     const bool odd = a.cols % 4 || (reinterpret_cast<uintptr_t>(a.x) & 15);
     const size_t col_tiles = (a.cols + 127) / 128, n = (a.rows + 127) / 128 * col_tiles;
     if (a.block_rows == 1 && !a.codes_t) {
-        // [2050, 3000] 7 us, 9.6 as tiles; [4096, 11008] 4.9 TB/s both ways
+        // [2050, 3000] 7 us, 9.6 as tiles; [16384, 8192] 5.7 TB/s
         int lx = 0;
         while (lx < 5 && (size_t(1) << lx) < col_tiles) ++lx;
         const size_t parts = (col_tiles + (1 << lx) - 1) >> lx, per = 32 >> lx;

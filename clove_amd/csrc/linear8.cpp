@@ -209,7 +209,8 @@ TensorNode HipBackend::matmul_e4m3(const Tensor &a, const Tensor &a_exps, const 
                       "bias must hold " + std::to_string(n) + " elements, got " +
                           shape_str(bias->shape));
     }
-    // (a grid holds 2^32 threads, up to 512 a tile)
+    // (a grid holds 2^32 threads: 2^22 tiles of 64 x 64 are 2^30, larger ones fewer, and 64
+    // rows or less in the streaming kernel 2^31; tiles are counted in 31 bits)
     CLOVE_REQUIRE(((m + 63) / 64) * ((n + 63) / 64) < (size_t(1) << 22), CLOVE_HIP_ERR_SHAPE,
                   "matmul_e4m3: the result has 2^22 tiles of 64 x 64 or more");
     TensorNode out = new_tensor(with_last(a, n), CLOVE_HIP_F32);

@@ -325,7 +325,8 @@ int clove_hip_paged_evict(CTensor block_tables, CTensor context_lens, CTensor we
  * codes are x * 2^-e rounded to nearest, ties to even, so an element is off by at
  * most 2^-4 of itself (half of 2^(e-9) for the smallest).  Magnitudes past 448 *
  * 2^119 become that; infinities and NaN become NaN, which products carry on.
- * Leading dimensions of x are rows; codes (and exps of rows) keep them.
+ * Leading dimensions of x are rows; codes (and exps of rows) keep them.  Rows and
+ * columns of these entries stay below 2^31 - 4096 each.
  * The entries allocate their results and workspaces, like most here: not for code
  * under HIP graph capture. */
 
@@ -341,7 +342,8 @@ int clove_hip_rms_norm_e4m3(CTensor x, CTensor residual, CTensor gamma, float ep
 /* Gradients of out with respect to h and gamma (with respect to x and residual:
  * h's).  grad_sum (h's shape, or NULL) is the gradient that reaches h from
  * elsewhere, the residual stream, and is added to *grad_h.  Either output may be
- * NULL.  Sums run in a fixed order. */
+ * NULL.  *grad_h is computed in 64 bits and rounded once; *grad_gamma's terms and
+ * sums are 32 bits wide, in a fixed order. */
 int clove_hip_rms_norm_backward(CTensor h, CTensor gamma, CTensor grad_out, CTensor grad_sum,
                                 float eps, CTensor *grad_h, CTensor *grad_gamma);
 /* x f32 [.., K] in 8 bits with blocks of block_rows (1 or 128) rows by 128
@@ -354,8 +356,10 @@ int clove_hip_quantize_e4m3(CTensor x, int block_rows, CTensor *codes, CTensor *
                             CTensor *codes_t, CTensor *exps_t);
 /* out[.., n] = sum_k a[.., k] * b[n, k] (+ bias[n]): a [.., Kp] and b [N, Kp] in 8
  * bits, each with exponents of rows or of 128 x 128 blocks, bias f32 of N elements
- * or NULL.  Products are exact and sums 32 bits wide, in a fixed order.  Kp is a
- * multiple of 128 below 2^23, codes are 16-byte aligned, exponents in [-100, 119]. */
+ * or NULL.  A product of two elements is exact where f32 holds it, subnormal values
+ * among them; past its range it is infinite, below it 0 or the smallest.  Sums are 32 bits
+ * wide, in a fixed order.  Kp is a multiple of 128 below 2^23, codes are 16-byte aligned,
+ * exponents in [-100, 119], and the result has fewer than 2^22 tiles of 64 x 64. */
 CTensor clove_hip_matmul_e4m3(CTensor a, CTensor a_exps, CTensor b, CTensor b_exps, CTensor bias);
 
 /* ---------------------------------------------------------------------- */

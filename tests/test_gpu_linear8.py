@@ -439,6 +439,21 @@ def test_matmul_extreme_exponents(hip):
                     within(got, want, tol)
 
 
+@pytest.mark.parametrize("m,n", [(4, 40), (80, 200)])
+@pytest.mark.parametrize("exps", [(-70, -66), (-70, -76), (-100, -52), (-59, -100)])
+def test_matmul_keeps_subnormal_products(hip, m, n, exps):
+    """Products of 448 * 448 * 2^(ea + eb), whole multiples of 2^-149, and their sums."""
+    for count in (1, 100):
+        x = [np.zeros((r, 256), np.float32) for r in (m, n)]
+        for v in x:
+            v[:, :count] = 448
+        a, b = (ref.quantize(v)[0] for v in x)
+        ea, eb = (np.full((r, 2), e, np.int32) for r, e in zip((m, n), exps))
+        got = hip.matmul_e4m3(*put(hip, a, ea, b, eb)).numpy()
+        want = count * 448.0 * 448.0 * 2.0 ** sum(exps)
+        np.testing.assert_array_equal(got, np.full((m, n), want))
+
+
 def test_matmul_carries_nan_to_its_row_and_column_alone(hip):
     g = rng(32)
     for m, n in ((10, 100), (150, 200)):
