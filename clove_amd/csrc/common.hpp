@@ -68,6 +68,8 @@ inline bool known_dtype(int dtype) {
     return dtype == CLOVE_HIP_F32 || dtype == CLOVE_HIP_I32 || dtype == CLOVE_HIP_E4M3;
 }
 std::string shape_str(const std::vector<size_t> &shape);
+// Refuses a tensor of another dtype; `what` names the argument.
+void need_dtype(const Tensor &t, int dtype, const char *what);
 
 // Allocates a device tensor through the caching allocator.
 TensorNode new_tensor(const std::vector<size_t> &shape, int dtype);

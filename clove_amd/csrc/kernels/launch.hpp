@@ -11,6 +11,9 @@
 namespace clove {
 namespace k {
 
+// Whether vectors of four floats may be read and written at p.
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
 // fill.hip -- seeded synthetic data (counter-based splitmix64 stream).
 void fill_normal(float *p, size_t n, uint64_t seed, float mean, float stddev, hipStream_t s);
 void fill_uniform(float *p, size_t n, uint64_t seed, float lo, float hi, hipStream_t s);

@@ -154,8 +154,6 @@ __global__ void __launch_bounds__(256) norm_apply_kernel(RmsNormArgs a, unsigned
     emit<ODD, OUT8>(a, row, c, normed(h, g, a.stats[row]));
 }
 
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 template <bool ODD, bool OUT8>
 void norm_any(const RmsNormArgs &a, hipStream_t s) {
     // (with an 8-bit output the lanes behind the row write its padding)

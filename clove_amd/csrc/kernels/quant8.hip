@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(Quant8Args a, size_t
 
 void quantize8(const Quant8Args &a, hipStream_t s) {
     if (a.rows == 0 || a.cols == 0 || (!a.codes && !a.codes_t)) return;
-    const bool odd = a.cols % 4 || (reinterpret_cast<uintptr_t>(a.x) & 15);
+    const bool odd = a.cols % 4 || !aligned16(a.x);
     const size_t col_tiles = (a.cols + 127) / 128, n = (a.rows + 127) / 128 * col_tiles;
     if (a.block_rows == 1 && !a.codes_t) {
         // [2050, 3000] 7 us, 9.6 as tiles; [16384, 8192] 5.7 TB/s

@@ -987,8 +987,6 @@ int pick_vpt(int cols) {
     return v <= 32 ? v : 0;
 }
 
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 // launch(first row, rows) of the row-per-workgroup kernels, whose grid holds
 // under 2^32 threads: 2^23 rows and more go in several launches.
 constexpr size_t kRowsPerLaunch = 1 << 22;

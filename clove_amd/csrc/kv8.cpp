@@ -12,12 +12,6 @@ namespace clove {
 
 namespace {
 
-void need_dtype(const Tensor &t, int dtype, const char *what) {
-    static const char *names[] = {"f32", "int32", "e4m3"};
-    CLOVE_REQUIRE(t.dtype == dtype, CLOVE_HIP_ERR_INVALID,
-                  std::string(what) + " must be an " + names[dtype] + " tensor");
-}
-
 void tables_rule(const Tensor &bt, const Tensor &cl, size_t block_size) {
     need_dtype(bt, CLOVE_HIP_I32, "block_tables");
     need_dtype(cl, CLOVE_HIP_I32, "context_lens");

@@ -11,12 +11,6 @@ namespace clove {
 
 namespace {
 
-void need_dtype(const Tensor &t, int dtype, const char *what) {
-    static const char *names[] = {"f32", "int32", "e4m3"};
-    CLOVE_REQUIRE(t.dtype == dtype, CLOVE_HIP_ERR_INVALID,
-                  std::string(what) + " must be an " + names[dtype] + " tensor");
-}
-
 // (the kernels count a row's columns in 31 bits, a little past its end)
 constexpr size_t kMaxDim = (size_t(1) << 31) - 4096;
 
@@ -101,7 +95,7 @@ void operand_rule(const Tensor &codes, const Tensor &exps, const char *what, siz
                       std::to_string(blocks_of(*rows)) + " blocks of rows, [.., " +
                       std::to_string(*blocks) + "], got " + shape_str(exps.shape));
     *tiles = lines != *rows;
-    CLOVE_REQUIRE((reinterpret_cast<uintptr_t>(codes.data) & 15) == 0, CLOVE_HIP_ERR_INVALID,
+    CLOVE_REQUIRE(k::aligned16(codes.data), CLOVE_HIP_ERR_INVALID,
                   name + " must be 16-byte aligned");
 }
 

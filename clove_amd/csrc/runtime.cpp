@@ -78,6 +78,12 @@ std::string shape_str(const std::vector<size_t> &shape) {
     return s + "]";
 }
 
+void need_dtype(const Tensor &t, int dtype, const char *what) {
+    static const char *names[] = {"f32", "int32", "e4m3"};
+    CLOVE_REQUIRE(t.dtype == dtype, CLOVE_HIP_ERR_INVALID,
+                  std::string(what) + " must be an " + names[dtype] + " tensor");
+}
+
 // ---- allocator -----------------------------------------------------------
 
 static size_t size_class(size_t bytes) {
