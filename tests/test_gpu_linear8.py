@@ -192,16 +192,17 @@ def test_rms_norm_backward(hip, rows, cols, stream):
             np.testing.assert_array_equal(a, b)
 
 
-def test_rms_norm_backward_extremes(hip):
+@pytest.mark.parametrize("cols", [33, 200, 300, 700, 1500, 2100, 5000, 9000])
+def test_rms_norm_backward_extremes(hip, cols):
     """Rows whose squares leave f32's range, a zero row, eps 0 and large, and grad_out
     times gamma past f32's range and under it, where r brings the gradient back."""
-    g = rng(23)
+    g = rng(23 + cols)
     sizes = np.array([1e30, 1e25, 1e-30, 1e-42, 1.0, 0.0])[:, None]
-    h = (g.standard_normal((6, 300)) * sizes).astype(np.float32)
+    h = (g.standard_normal((6, cols)) * sizes).astype(np.float32)
     for size in (1e10, 1.0, 1e-10):
-        gamma = (g.uniform(0.5, 2, 300) * size).astype(np.float32)
+        gamma = (g.uniform(0.5, 2, cols) * size).astype(np.float32)
         # r times these is near 1 in the first rows, which eps does not reach
-        gy = (g.standard_normal((6, 300)) * [[1e30], [1e20], [1e-32], [1e-35], [1e-3], [1e-3]]
+        gy = (g.standard_normal((6, cols)) * [[1e30], [1e20], [1e-32], [1e-35], [1e-3], [1e-3]]
               ).astype(np.float32)
         for eps in (1e-5, 0.0, 100.0):
             good = slice(0, 5 if eps == 0 else 6)
