@@ -113,7 +113,8 @@ CTensor clove_hip_tensor_create(const float *data, size_t rows, size_t cols);
 /* N-d f32 / int32 tensors (block tables and context lengths are int32). */
 CTensor clove_hip_tensor_create_nd(const float *data, const size_t *shape, size_t ndim);
 CTensor clove_hip_tensor_create_i32(const int32_t *data, const size_t *shape, size_t ndim);
-/* Uninitialised device tensor of the given dtype. */
+/* Uninitialised device tensor of the given dtype.  The product of a shape's non-zero
+ * dimensions stays below 2^60, here as everywhere (CLOVE_HIP_ERR_SHAPE). */
 CTensor clove_hip_tensor_empty(const size_t *shape, size_t ndim, int dtype);
 /* Non-owning view of caller-owned device memory (freed by the caller). */
 CTensor clove_hip_tensor_wrap(void *device_ptr, const size_t *shape, size_t ndim, int dtype);
